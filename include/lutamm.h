@@ -24,6 +24,7 @@
 #ifndef LUTAMM_H
 #define LUTAMM_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -226,6 +227,98 @@ int lutamm_index_calculation(lutamm_ctx* ctx, int layer_id, const float* input, 
  * accumulator of the token (both kernel variants), and nothing outside the table is read. */
 int lutamm_pim_lut(lutamm_ctx* ctx, int layer_id, const uint8_t* index, float* output,
                    uint32_t n_tokens, uint32_t flags);
+
+/* ---- the layer's dense operators ---------------------------------------------------- */
+
+/* What stands between the linears of an encoder layer, for callers that keep the whole layer on the context's stream:
+ * layer norm with the residual behind it (layer_norm() and the additions of src/host/transformer_layer.cpp:50-90, :440-480),
+ * attention (:217-229), here with a window and padded sequences, and rotary positions, which the reference has not.
+ * All buffers are memory of the context's device.  A call queues its kernels on the context's stream; without
+ * LUTAMM_FLAG_ASYNC, the only flag, it waits for them.  Tensors are of one `dtype`; parameters, their gradients and statistics
+ * are fp32, and so is all arithmetic on the way; a result is rounded once, to nearest.  Strides count elements and are
+ * not negative; the last axis is contiguous; an output's elements lie apart from one another.  Tensors whose rows all start on
+ * 16 bytes are read and written 16 bytes at a time, others an element at a time. */
+#define LUTAMM_F32   0u
+#define LUTAMM_F16   1u
+#define LUTAMM_BF16  2u
+
+/* out = residual + (x - mean) * rstd * weight + bias over the last axis, rstd = 1 / sqrt(var + eps).
+ * residual, weight, bias and stats may be NULL; stats [rows][2] takes mean and rstd for the backward pass.  out may be x
+ * or residual (same address and stride). */
+typedef struct lutamm_norm_params {
+    uint32_t dtype, rows, width;      /* rows and width below 2^31 */
+    float    eps;                     /* not negative */
+    const void* x;        int64_t x_stride;         /* [rows][width] */
+    const void* residual; int64_t residual_stride;
+    void*       out;      int64_t out_stride;
+    const float* weight;              /* [width] */
+    const float* bias;
+    float*       stats;
+} lutamm_norm_params;
+int lutamm_layer_norm(lutamm_ctx* ctx, const lutamm_norm_params* p, uint32_t flags);
+
+/* Its gradients: with g = dout * weight and xh = (x - mean) * rstd
+ *   dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dweight = sum over rows of dout * xh,  dbias = sum over rows of dout
+ * (that of the residual is dout).  weight NULL counts as ones; dx, dweight and dbias may be NULL; dx may be dout or x.
+ * Sums over rows are made in a fixed order: equal calls give equal bits.  They pass through
+ * lutamm_layer_norm_backward_workspace() bytes of `workspace`, device memory on 16 bytes that the caller keeps, or, where that is
+ * NULL, through memory of the context.  Graphs captured from calls on one context share the latter and must not be replayed
+ * at the same time. */
+typedef struct lutamm_norm_grad_params {
+    uint32_t dtype, rows, width;
+    const void* dout;     int64_t dout_stride;
+    const void* x;        int64_t x_stride;
+    void*       dx;       int64_t dx_stride;
+    const float* weight;
+    const float* stats;               /* [rows][2], as lutamm_layer_norm left it */
+    float* dweight;
+    float* dbias;
+    void*  workspace;
+} lutamm_norm_grad_params;
+int lutamm_layer_norm_backward(lutamm_ctx* ctx, const lutamm_norm_grad_params* p, uint32_t flags);
+size_t lutamm_layer_norm_backward_workspace(const lutamm_ctx* ctx, uint32_t rows, uint32_t width);
+
+/* A tensor [batch][tokens][heads][head_dim] by its strides. */
+typedef struct lutamm_heads {
+    void*   data;
+    int64_t batch_stride, token_stride, head_stride;
+} lutamm_heads;
+
+/* Rotary positions with several axes (rows and columns of an image, time of a video).  The first 2 * (sum of sections) elements
+ * of a head are pairs, (i, i + pairs) or, interleaved, (2i, 2i + 1); the first sections[0] pairs follow the first axis and
+ * so on, and pair i turns by positions[axis] * inv_freq[i] (inverse: back, which is the gradient's way).  The rest of a head is
+ * copied.  Angles are formed in 64 bits: any int32 position keeps fp32's accuracy.  positions are int32 [batch][tokens][axes], strides
+ * for batch (0: the same for all sequences) and tokens.  out may be x, with the same strides; otherwise the two share no memory. */
+#define LUTAMM_MAX_AXES 4
+typedef struct lutamm_rotary_params {
+    uint32_t dtype, batch, tokens, heads, head_dim;   /* head_dim up to 4096, heads * head_dim up to 2^24 */
+    uint32_t axes, sections[LUTAMM_MAX_AXES];
+    uint32_t interleaved, inverse;
+    lutamm_heads x, out;
+    const int32_t* positions; int64_t position_batch_stride, position_token_stride;
+    const float* inv_freq;
+} lutamm_rotary_params;
+int lutamm_rotary(lutamm_ctx* ctx, const lutamm_rotary_params* p, uint32_t flags);
+
+/* out = softmax(scale * q k^T) v over the keys that a query sees.  Query i of sequence b stands at position first[b] + i
+ * (first NULL: i) and sees key j if j < lengths[b] (NULL: keys), j <= position + right and (j >= position - left or
+ * j < sinks); left or right negative: no bound on that side.  So a padded batch of whole sequences has lengths alone, new
+ * tokens behind a cache have first = lengths - queries and right = 0, a sliding window has left, and sinks are the
+ * first keys, which stay visible.  A query that sees no key gives zeros.  Keys from lengths[b] on are not read; lengths are taken between 0
+ * and keys.  Head h reads key head h / (heads / kv_heads).  A key that a query does not see has no part in its result, whatever it holds,
+ * with one exception: a value that is not finite spreads to the queries whose tile of up to 128 query rows has another one that sees it.
+ * q and out are [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim]; out shares no memory with the
+ * others.  For serving: there is no backward pass. */
+typedef struct lutamm_attention_params {
+    uint32_t dtype, batch, queries, keys, heads, kv_heads, head_dim;  /* head_dim a multiple of 8 up to 128, keys below 2^31 */
+    uint32_t sinks;
+    int32_t  left, right;
+    float    scale;
+    lutamm_heads q, k, v, out;
+    const int32_t* lengths;   /* [batch], device */
+    const int32_t* first;     /* [batch], device */
+} lutamm_attention_params;
+int lutamm_attention(lutamm_ctx* ctx, const lutamm_attention_params* p, uint32_t flags);
 
 /* ---- one AMM across the GPUs of a box ---------------------------------------------- */
 

@@ -26,6 +26,8 @@ INDEX_U8_ROWMAJOR, INDEX_U16_TILED = 0, 1
 LUT_CANONICAL, LUT_DPU_TILED = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_TANH_F16 = 0, 1, 2
 EPILOGUE_AUTO, EPILOGUE_TRANSPOSE, EPILOGUE_COPY_ENGINE = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2
+MAX_AXES = 4
 
 # every symbol include/lutamm.h declares
 ABI_SYMBOLS = [
@@ -38,6 +40,7 @@ ABI_SYMBOLS = [
     "lutamm_shard_unique_id", "lutamm_shard_init", "lutamm_shard_finalize", "lutamm_amm_column_sharded",
     "lutamm_amm_token_sharded", "lutamm_tune_sharding", "lutamm_plan_cache_save", "lutamm_plan_cache_load",
     "lutamm_selftest_bounded_wait", "lutamm_shard_alloc_gathered", "lutamm_shard_free_gathered",
+    "lutamm_layer_norm", "lutamm_layer_norm_backward", "lutamm_layer_norm_backward_workspace", "lutamm_rotary", "lutamm_attention",
 ]
 SHARD_SEARCH_REPLICATED, SHARD_SEARCH_SPLIT = 0, 1
 SHARD_ID_BYTES = 128
@@ -90,6 +93,42 @@ class ShardingReport(ctypes.Structure):
 class Timings(ctypes.Structure):
     _fields_ = [("index_calc_ms", ctypes.c_float), ("lut_kernel_ms", ctypes.c_float),
                 ("data_transfer_ms", ctypes.c_float), ("total_ms", ctypes.c_float)]
+
+
+def _fields(text: str):
+    """ctypes fields from "type name, name; type name"."""
+    types = {"u32": ctypes.c_uint32, "i32": ctypes.c_int32, "i64": ctypes.c_int64, "f32": ctypes.c_float, "ptr": ctypes.c_void_p}
+    return [(n.strip(), types[part.split()[0]]) for part in text.split(";") for n in part.strip().split(" ", 1)[1].split(",")]
+
+
+class NormParams(ctypes.Structure):
+    """lutamm_norm_params."""
+    _fields_ = _fields("u32 dtype, rows, width; f32 eps; ptr x; i64 x_stride; ptr residual; i64 residual_stride; ptr out; i64 out_stride;"
+                       "ptr weight, bias, stats")
+
+
+class NormGradParams(ctypes.Structure):
+    """lutamm_norm_grad_params."""
+    _fields_ = _fields("u32 dtype, rows, width; ptr dout; i64 dout_stride; ptr x; i64 x_stride; ptr dx; i64 dx_stride;"
+                       "ptr weight, stats, dweight, dbias, workspace")
+
+
+class Heads(ctypes.Structure):
+    """lutamm_heads: a tensor [batch][tokens][heads][head_dim] by its strides."""
+    _fields_ = _fields("ptr data; i64 batch_stride, token_stride, head_stride")
+
+
+class RotaryParams(ctypes.Structure):
+    """lutamm_rotary_params."""
+    _fields_ = (_fields("u32 dtype, batch, tokens, heads, head_dim, axes") + [("sections", ctypes.c_uint32 * MAX_AXES)] +
+                _fields("u32 interleaved, inverse") + [("x", Heads), ("out", Heads)] +
+                _fields("ptr positions; i64 position_batch_stride, position_token_stride; ptr inv_freq"))
+
+
+class AttentionParams(ctypes.Structure):
+    """lutamm_attention_params."""
+    _fields_ = (_fields("u32 dtype, batch, queries, keys, heads, kv_heads, head_dim, sinks; i32 left, right; f32 scale") +
+                [(n, Heads) for n in ("q", "k", "v", "out")] + _fields("ptr lengths, first"))
 
 
 _lib = None
@@ -168,10 +207,17 @@ def load_library() -> ctypes.CDLL:
     L.lutamm_generation.restype = ctypes.c_uint64
     L.lutamm_amm_static_scratch.argtypes = [i32, vp, vp, vp, vp, vp, vp, ctypes.POINTER(IndexCalcParams),
                                             ctypes.POINTER(LUTParams)]
+    L.lutamm_layer_norm.argtypes = [vp, ctypes.POINTER(NormParams), u32]
+    L.lutamm_layer_norm_backward.argtypes = [vp, ctypes.POINTER(NormGradParams), u32]
+    L.lutamm_layer_norm_backward_workspace.argtypes = [vp, u32, u32]
+    L.lutamm_layer_norm_backward_workspace.restype = ctypes.c_size_t
+    L.lutamm_rotary.argtypes = [vp, ctypes.POINTER(RotaryParams), u32]
+    L.lutamm_attention.argtypes = [vp, ctypes.POINTER(AttentionParams), u32]
     L.lutamm_static_scratch_last_error.argtypes = []
     L.lutamm_static_scratch_last_error.restype = ctypes.c_char_p
     for name in ABI_SYMBOLS:
-        if name not in ("lutamm_version", "lutamm_last_error", "lutamm_launch_count", "lutamm_generation", "lutamm_static_scratch_last_error"):
+        if name not in ("lutamm_version", "lutamm_last_error", "lutamm_launch_count", "lutamm_generation", "lutamm_static_scratch_last_error",
+                        "lutamm_layer_norm_backward_workspace"):
             getattr(L, name).restype = i32
     _lib = L
     return L
@@ -188,6 +234,38 @@ def _ptr(a) -> int:
         assert a.is_contiguous(), "tensors handed to the C ABI must be contiguous"
         return a.data_ptr()
     return int(a)
+
+
+def _dtype_of(t) -> int:
+    """LUTAMM_F32 / F16 / BF16 of a tensor."""
+    code = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}.get(str(getattr(t, "dtype", None)))
+    if code is None:
+        raise ValueError(f"float32, float16 or bfloat16 tensors are wanted, got {getattr(t, 'dtype', type(t))}")
+    return code
+
+
+def _operand(name: str, t, dtype, shape) -> int:
+    """Address of a tensor of this type and shape whose last axis is contiguous; None is null."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: {dtype} {tuple(shape)} is wanted, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    return t.data_ptr()
+
+
+def _packed(name: str, t, dtype, shape) -> int:
+    """... of a tensor that is contiguous throughout."""
+    at = _operand(name, t, dtype, shape)
+    if t is not None and not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous tensor is wanted")
+    return at
+
+
+def _heads(name: str, t, dtype, shape) -> Heads:
+    at = _operand(name, t, dtype, shape)
+    return Heads(at, *t.stride()[:3])
 
 
 def make_params(M: int, K: int, N: int, CB: int, CT: int, scale: float, lut_bias: float = 0.0, *,
@@ -349,6 +427,77 @@ class LutAmmContext:
         """pim_lut() of the reference (src/host/pim_lut_host.cpp:121-222)."""
         M = int(n_tokens if n_tokens is not None else input_index.shape[0])
         self._check(self._L.lutamm_pim_lut(self._h, layer_id, _ptr(input_index), _ptr(output_tensor), M, flags))
+
+    # -- the layer's dense operators (device tensors; include/lutamm.h has the formulas)
+    def layer_norm(self, x, weight, bias, out, eps: float = 1e-6, residual=None, stats=None, flags: int = 0):
+        """out = residual + layer norm of x over the last axis (layer_norm() of the reference, transformer_layer.cpp:50-90, and the
+        addition behind it).  x, residual, out [rows, width] float32, float16 or bfloat16, rows of any stride; weight and bias
+        float32 [width] or None; stats float32 [rows, 2] takes mean and 1 / sqrt(var + eps) for layer_norm_backward.  out may
+        be x or residual."""
+        import torch
+        rows, width = x.shape
+        f32 = torch.float32
+        p = NormParams(_dtype_of(x), rows, width, eps, _operand("x", x, x.dtype, (rows, width)), x.stride(0),
+                       _operand("residual", residual, x.dtype, (rows, width)), residual.stride(0) if residual is not None else 0,
+                       _operand("out", out, x.dtype, (rows, width)), out.stride(0),
+                       _operand("weight", weight, f32, (width,)), _operand("bias", bias, f32, (width,)),
+                       _packed("stats", stats, f32, (rows, 2)))
+        self._check(self._L.lutamm_layer_norm(self._h, ctypes.byref(p), flags))
+
+    def layer_norm_backward(self, dout, x, weight, stats, dx=None, dweight=None, dbias=None, workspace=None, flags: int = 0):
+        """Gradients of layer_norm: dx like x, dweight and dbias float32 [width], each only where a tensor is given (that of the
+        residual is dout).  stats as layer_norm left them.  workspace: a uint8 tensor of layer_norm_backward_workspace() bytes
+        in place of the context's own, for captured calls that may run beside others of this context."""
+        import torch
+        rows, width = x.shape
+        f32 = torch.float32
+        if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
+                                      or workspace.numel() < self.layer_norm_backward_workspace(rows, width)):
+            raise ValueError("workspace: a contiguous uint8 tensor of layer_norm_backward_workspace() bytes is wanted")
+        p = NormGradParams(_dtype_of(x), rows, width, _operand("dout", dout, x.dtype, (rows, width)), dout.stride(0),
+                           _operand("x", x, x.dtype, (rows, width)), x.stride(0),
+                           _operand("dx", dx, x.dtype, (rows, width)), dx.stride(0) if dx is not None else 0,
+                           _operand("weight", weight, f32, (width,)), _packed("stats", stats, f32, (rows, 2)),
+                           _operand("dweight", dweight, f32, (width,)), _operand("dbias", dbias, f32, (width,)),
+                           workspace.data_ptr() if workspace is not None else 0)
+        self._check(self._L.lutamm_layer_norm_backward(self._h, ctypes.byref(p), flags))
+
+    def layer_norm_backward_workspace(self, rows: int, width: int) -> int:
+        return int(self._L.lutamm_layer_norm_backward_workspace(self._h, rows, width))
+
+    def rotary(self, x, positions, inv_freq, sections, out, interleaved: bool = False, inverse: bool = False, flags: int = 0):
+        """Rotary positions with several axes.  x and out [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], float32, float16
+        or bfloat16, of any strides (the query and key heads of a fused projection are one view); out may be x.  positions
+        int32 [tokens, axes], or [batch, tokens, axes]; inv_freq float32 [sum(sections)]; sections the pairs of each axis.
+        Pairs are (i, i + pairs) of a head, or (2i, 2i + 1) if interleaved.  inverse turns back: the gradient."""
+        import torch
+        if x.dim() == 3:
+            x, out = x.unsqueeze(0), out.unsqueeze(0)
+        if positions.dim() == 2:
+            positions = positions.expand(x.shape[0], -1, -1)
+        axes = len(sections)
+        if x.dim() != 4 or not 1 <= axes <= MAX_AXES or min(sections) < 0:
+            raise ValueError(f"x has three or four axes, sections 1 to {MAX_AXES} counts")
+        p = RotaryParams(_dtype_of(x), *x.shape, axes, tuple(sections), bool(interleaved), bool(inverse), _heads("x", x, x.dtype, x.shape),
+                         _heads("out", out, x.dtype, x.shape), _operand("positions", positions, torch.int32, (*x.shape[:2], axes)),
+                         positions.stride(0), positions.stride(1), _packed("inv_freq", inv_freq, torch.float32, (sum(sections),)))
+        self._check(self._L.lutamm_rotary(self._h, ctypes.byref(p), flags))
+
+    def attention(self, q, k, v, out, scale: float | None = None, window=(-1, -1), sinks: int = 0, lengths=None, first=None, flags: int = 0):
+        """softmax(scale * q k^T) v over the keys that each query sees (the reference's attention, transformer_layer.cpp:217-229, sees
+        all).  q and out [batch, queries, heads, head_dim], k and v [batch, keys, kv_heads, head_dim], float32, float16 or bfloat16, of any
+        strides; heads a multiple of kv_heads; head_dim a multiple of 8 up to 128; scale 1/sqrt(head_dim) by default.  Query i of
+        sequence b is at position first[b] + i (first: int32 [batch] on the device, None: 0) and sees the keys from window[0]
+        in front of it to window[1] behind it (negative: no bound), and of those in front also the first `sinks`, up to
+        lengths[b] (int32 [batch] on the device, None: all).  A query that sees none gives zeros."""
+        import torch
+        B, Q, H, D = q.shape
+        K, G = k.shape[1:3]
+        p = AttentionParams(_dtype_of(q), B, Q, K, H, G, D, sinks, *window, D ** -0.5 if scale is None else scale,
+                            _heads("q", q, q.dtype, (B, Q, H, D)), _heads("k", k, q.dtype, (B, K, G, D)),
+                            _heads("v", v, q.dtype, (B, K, G, D)), _heads("out", out, q.dtype, (B, Q, H, D)),
+                            _packed("lengths", lengths, torch.int32, (B,)), _packed("first", first, torch.int32, (B,)))
+        self._check(self._L.lutamm_attention(self._h, ctypes.byref(p), flags))
 
     # -- one AMM across the GPUs of a box (one process per GPU)
     def shard_init(self, rank: int | None = None, world: int | None = None, group=None):

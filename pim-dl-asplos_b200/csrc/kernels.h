@@ -155,6 +155,60 @@ cudaError_t launch_spread_input(const float* centroid, float* x, uint32_t M, uin
 // Self-test: a bounded wait on a barrier nobody arrives at; the kernel reports through *dev_err and returns.
 cudaError_t launch_stalled_wait(uint32_t polls, uint32_t* dev_err, cudaStream_t s);
 
+// ---- the layer's dense operators -------------------------------------------------------
+// dtype: LUTAMM_F32 / F16 / BF16 of every tensor; parameters, their gradients and statistics are fp32.  Strides in elements.
+struct NormArgs {
+    const void *x, *residual;    // residual may be null
+    const float *weight, *bias;  // [width], either may be null
+    void* out;
+    float* stats;                // [rows][2] mean and 1 / sqrt(var + eps), may be null
+    int64_t x_stride, residual_stride, out_stride;
+    uint32_t rows, width;
+    float eps;
+    bool param_vec;              // weight and bias start on 16 bytes
+};
+cudaError_t launch_norm(const NormArgs& a, uint32_t dtype, cudaStream_t s);
+struct NormGradArgs {
+    const void *dout, *x;
+    const float *weight, *stats;
+    void* dx;                    // may be null
+    float *dweight, *dbias;      // may be null
+    float* partial;              // norm_grad_workspace() bytes where either gradient is wanted, else null
+    int64_t dout_stride, x_stride, dx_stride;
+    uint32_t rows, width;
+    bool param_vec;
+};
+size_t norm_grad_workspace(uint32_t rows, uint32_t width, int sm_count);
+uint32_t norm_grad_launches(const NormGradArgs& a);
+cudaError_t launch_norm_grad(const NormGradArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
+
+struct RotaryArgs {
+    const void* x;
+    void* out;
+    int64_t x_batch, x_token, x_head, out_batch, out_token, out_head;
+    const int32_t* positions;    // [batch][tokens][axes]
+    int64_t position_batch_stride, position_token_stride;
+    const float* inv_freq;       // [pairs]
+    uint32_t batch, tokens, heads, head_dim, pairs;
+    uint32_t ends[3];            // first pair of the second, third and fourth axis
+    bool interleaved, inverse, in_place;
+    bool vec;                    // heads of both tensors start on 16 bytes
+};
+cudaError_t launch_rotary(const RotaryArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
+
+struct AttentionArgs {
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head, out_batch, out_token, out_head;
+    const int32_t *lengths, *first;   // [batch], may be null: all keys, position 0
+    uint32_t batch, queries, keys, heads, kv_heads, head_dim, sinks;
+    int32_t left, right;              // negative: no bound
+    float scale;                      // of the scores, times log2 e
+    bool vec;                         // rows of all four tensors start on 16 bytes
+};
+// Few rows (query tokens x heads of a key head): one pass over keys and values on the CUDA cores.
+cudaError_t launch_attention_rows(const AttentionArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
+
 // The opt-in to more than 48 KB of dynamic shared memory, asked for once per kernel, device and size (the call takes a
 // good part of a microsecond): remembers, per kernel, the largest size asked for on each device.
 struct SmemOptIn {

@@ -7,6 +7,7 @@
 #include "nccl_shard.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -110,7 +111,7 @@ struct lutamm_ctx {
     cudaStream_t own_stream = nullptr;
     cudaStream_t stream = nullptr;
     std::map<int, Layer> layers;
-    Buf d_in, d_out, d_idx, d_idx16, d_acc_dbg, d_acc_scratch, d_counters, d_build, d_build_words;
+    Buf d_in, d_out, d_idx, d_idx16, d_acc_dbg, d_acc_scratch, d_counters, d_build, d_build_words, d_norm;
     // host-buffer pipeline: copy-in and copy-out streams, kHostSlots staging slots
     cudaStream_t s_in = nullptr, s_out = nullptr;
     Buf p_in[kHostSlots], p_out[kHostSlots];
@@ -648,7 +649,7 @@ int lutamm_destroy(lutamm_ctx* c) {
     if (c->s_in) cudaStreamDestroy(c->s_in);
     if (c->s_out) cudaStreamDestroy(c->s_out);
     for (Buf* b : {&c->d_in, &c->d_out, &c->d_idx, &c->d_idx16, &c->d_acc_dbg, &c->d_acc_scratch, &c->d_counters,
-                   &c->d_build, &c->d_build_words})
+                   &c->d_build, &c->d_build_words, &c->d_norm})
         cudaFree(b->p);
     cudaFreeHost(c->h_err);
     for (auto& ev : c->ev)
@@ -862,6 +863,207 @@ int lutamm_pim_lut(lutamm_ctx* c, int layer_id, const uint8_t* index, float* out
     if (!out_dev) CU_TRY(c, cudaMemcpyAsync(output, d_y, out_bytes, cudaMemcpyDeviceToHost, c->stream));
     if (flags & LUTAMM_FLAG_ASYNC) return LUTAMM_OK;
     return check_dev_err(c);
+}
+
+// ---- the layer's dense operators
+static int dense_args(lutamm_ctx* c, const void* params, uint32_t flags) {
+    if (!c) return fail(nullptr, LUTAMM_EINVAL, "null context");
+    if (!params) return fail(c, LUTAMM_EINVAL, "null params");
+    if (flags & ~LUTAMM_FLAG_ASYNC) return fail(c, LUTAMM_EINVAL, "flags: LUTAMM_FLAG_ASYNC alone");
+    return LUTAMM_OK;
+}
+
+static size_t dtype_size(uint32_t dtype) { return dtype == LUTAMM_F32 ? 4 : dtype == LUTAMM_F16 || dtype == LUTAMM_BF16 ? 2 : 0; }
+
+// A buffer of the context's device, aligned to its elements.
+static int dense_pointer(lutamm_ctx* c, const char* name, const void* p, size_t size, bool optional) {
+    if (!p) return optional ? LUTAMM_OK : fail(c, LUTAMM_EINVAL, std::string("null ") + name);
+    if (reinterpret_cast<uintptr_t>(p) % size) return fail(c, LUTAMM_EINVAL, std::string(name) + " is not aligned to its elements");
+    if (pointer_device(p) != c->device) return fail(c, LUTAMM_EINVAL, std::string(name) + " is not memory of the context's device");
+    return LUTAMM_OK;
+}
+
+// Strides of a tensor whose last axis is contiguous.  Those of an output keep its elements apart: sorted by stride, each axis steps
+// over all that the axes below it cover.
+static int dense_strides(lutamm_ctx* c, const char* name, const int64_t* stride, const uint64_t* extent, int axes, uint64_t inner, bool output) {
+    int order[3];
+    for (int i = 0; i < axes; ++i) {
+        if (stride[i] < 0 || (stride[i] >> 40)) return fail(c, LUTAMM_EINVAL, std::string(name) + ": strides must be 0 .. 2^40 - 1");
+        order[i] = i;
+    }
+    if (!output) return LUTAMM_OK;
+    std::sort(order, order + axes, [&](int i, int j) { return stride[i] < stride[j]; });
+    uint64_t covered = inner;
+    for (int k = 0; k < axes; ++k) {
+        const int i = order[k];
+        if (extent[i] <= 1) continue;
+        if ((uint64_t)stride[i] < covered) return fail(c, LUTAMM_EINVAL, std::string(name) + ": the elements of an output must lie apart");
+        covered += (extent[i] - 1) * (uint64_t)stride[i];
+    }
+    return LUTAMM_OK;
+}
+
+static int dense_heads(lutamm_ctx* c, const char* name, const lutamm_heads& h, size_t size, uint64_t batch, uint64_t tokens, uint64_t heads, uint64_t dim, bool output) {
+    if (int r = dense_pointer(c, name, h.data, size, false)) return r;
+    const int64_t stride[3] = {h.batch_stride, h.token_stride, h.head_stride};
+    const uint64_t extent[3] = {batch, tokens, heads};
+    return dense_strides(c, name, stride, extent, 3, dim, output);
+}
+
+static bool on_16(const lutamm_heads& h, size_t size, uint64_t batch, uint64_t tokens, uint64_t heads) {
+    auto even = [&](int64_t stride, uint64_t n) { return n <= 1 || (uint64_t)stride * size % 16 == 0; };
+    return reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && even(h.batch_stride, batch) && even(h.token_stride, tokens) && even(h.head_stride, heads);
+}
+
+static int dense_done(lutamm_ctx* c, cudaError_t e, const char* what, uint32_t launched, uint32_t flags) {
+    if (e != cudaSuccess) return fail(c, LUTAMM_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
+    c->launches += launched;
+    return (flags & LUTAMM_FLAG_ASYNC) ? LUTAMM_OK : check_dev_err(c);
+}
+
+int lutamm_layer_norm(lutamm_ctx* c, const lutamm_norm_params* p, uint32_t flags) {
+    if (int r = dense_args(c, p, flags)) return r;
+    const size_t size = dtype_size(p->dtype);
+    if (!size) return fail(c, LUTAMM_EINVAL, "unknown dtype");
+    if (!p->width || p->width >> 31 || p->rows >> 31) return fail(c, LUTAMM_EINVAL, "width must be 1 .. 2^31 - 1 and rows below 2^31");
+    if (!(p->eps >= 0.f)) return fail(c, LUTAMM_EINVAL, "eps must not be negative");
+    if (!p->rows) return LUTAMM_OK;
+    DeviceGuard g(c->device);
+    const uint64_t rows = p->rows;
+    int r;
+    if ((r = dense_pointer(c, "x", p->x, size, false)) || (r = dense_pointer(c, "residual", p->residual, size, true)) ||
+        (r = dense_pointer(c, "out", p->out, size, false)) || (r = dense_pointer(c, "weight", p->weight, 4, true)) ||
+        (r = dense_pointer(c, "bias", p->bias, 4, true)) || (r = dense_pointer(c, "stats", p->stats, 4, true)) ||
+        (r = dense_strides(c, "x", &p->x_stride, &rows, 1, p->width, false)) ||
+        (r = dense_strides(c, "residual", &p->residual_stride, &rows, 1, p->width, false)) ||
+        (r = dense_strides(c, "out", &p->out_stride, &rows, 1, p->width, true)))
+        return r;
+    if ((p->out == p->x && p->out_stride != p->x_stride && rows > 1) || (p->out == p->residual && p->out_stride != p->residual_stride && rows > 1))
+        return fail(c, LUTAMM_EINVAL, "out in place of an input needs that input's stride");
+    NormArgs a{p->x, p->residual, p->weight, p->bias, p->out, p->stats, p->x_stride, p->residual_stride, p->out_stride, p->rows, p->width, p->eps,
+               (reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->bias)) % 16 == 0};
+    return dense_done(c, launch_norm(a, p->dtype, c->stream), "layer norm", 1, flags);
+}
+
+size_t lutamm_layer_norm_backward_workspace(const lutamm_ctx* c, uint32_t rows, uint32_t width) {
+    return c ? norm_grad_workspace(rows, width, c->sm_count) : 0;
+}
+
+int lutamm_layer_norm_backward(lutamm_ctx* c, const lutamm_norm_grad_params* p, uint32_t flags) {
+    if (int r = dense_args(c, p, flags)) return r;
+    const size_t size = dtype_size(p->dtype);
+    if (!size) return fail(c, LUTAMM_EINVAL, "unknown dtype");
+    if (!p->width || p->width >> 31 || p->rows >> 31) return fail(c, LUTAMM_EINVAL, "width must be 1 .. 2^31 - 1 and rows below 2^31");
+    if (!p->dx && !p->dweight && !p->dbias) return fail(c, LUTAMM_EINVAL, "no gradient is asked for");
+    DeviceGuard g(c->device);
+    const uint64_t rows = p->rows;
+    const bool any = rows > 0;   // without rows the inputs may be null, and dweight and dbias become zero
+    int r;
+    if ((r = dense_pointer(c, "dout", p->dout, size, !any)) || (r = dense_pointer(c, "x", p->x, size, !any)) ||
+        (r = dense_pointer(c, "stats", p->stats, 4, !any)) || (r = dense_pointer(c, "dx", p->dx, size, true)) ||
+        (r = dense_pointer(c, "weight", p->weight, 4, true)) || (r = dense_pointer(c, "dweight", p->dweight, 4, true)) ||
+        (r = dense_pointer(c, "dbias", p->dbias, 4, true)) || (r = dense_pointer(c, "workspace", p->workspace, 16, true)) ||
+        (r = dense_strides(c, "dout", &p->dout_stride, &rows, 1, p->width, false)) ||
+        (r = dense_strides(c, "x", &p->x_stride, &rows, 1, p->width, false)) ||
+        (p->dx && (r = dense_strides(c, "dx", &p->dx_stride, &rows, 1, p->width, true))))
+        return r;
+    if (any && p->dx && ((p->dx == p->dout && p->dx_stride != p->dout_stride && rows > 1) || (p->dx == p->x && p->dx_stride != p->x_stride && rows > 1)))
+        return fail(c, LUTAMM_EINVAL, "dx in place of an input needs that input's stride");
+    NormGradArgs a{p->dout, p->x, p->weight, p->stats, p->dx, p->dweight, p->dbias, nullptr, p->dout_stride, p->x_stride, p->dx_stride, p->rows, p->width,
+                   reinterpret_cast<uintptr_t>(p->weight) % 16 == 0};
+    if (p->dweight || p->dbias) {
+        if (p->workspace) {
+            a.partial = static_cast<float*>(p->workspace);
+        } else {
+            if ((r = ensure(c, c->d_norm, norm_grad_workspace(p->rows, p->width, c->sm_count)))) return r;
+            a.partial = static_cast<float*>(c->d_norm.p);
+        }
+    }
+    return dense_done(c, launch_norm_grad(a, p->dtype, c->sm_count, c->stream), "layer norm backward", norm_grad_launches(a), flags);
+}
+
+int lutamm_rotary(lutamm_ctx* c, const lutamm_rotary_params* p, uint32_t flags) {
+    if (int r = dense_args(c, p, flags)) return r;
+    const size_t size = dtype_size(p->dtype);
+    if (!size) return fail(c, LUTAMM_EINVAL, "unknown dtype");
+    if (!p->axes || p->axes > LUTAMM_MAX_AXES) return fail(c, LUTAMM_EINVAL, "axes must be 1 .. 4");
+    if (!p->head_dim || p->head_dim > 4096 || (uint64_t)p->heads * p->head_dim > (1u << 24) || p->batch >> 31 || p->tokens >> 31 ||
+        (uint64_t)p->batch * p->tokens >> 34)
+        return fail(c, LUTAMM_EINVAL, "head_dim must be 1 .. 4096, heads * head_dim at most 2^24, batch * tokens below 2^34");
+    uint64_t pairs = 0;
+    RotaryArgs a{};
+    for (uint32_t i = 0; i < p->axes; ++i) {
+        pairs += p->sections[i];
+        if (i < 3) a.ends[i] = (uint32_t)std::min<uint64_t>(pairs, 0xFFFFFFFFu);
+    }
+    for (uint32_t i = p->axes - 1; i < 3; ++i) a.ends[i] = 0xFFFFFFFFu;
+    if (2 * pairs > p->head_dim) return fail(c, LUTAMM_EINVAL, "sections have more pairs than half of head_dim");
+    if (!p->batch || !p->tokens || !p->heads) return LUTAMM_OK;
+    DeviceGuard g(c->device);
+    int r;
+    if ((r = dense_heads(c, "x", p->x, size, p->batch, p->tokens, p->heads, p->head_dim, false)) ||
+        (r = dense_heads(c, "out", p->out, size, p->batch, p->tokens, p->heads, p->head_dim, true)) ||
+        (r = dense_pointer(c, "positions", p->positions, 4, false)) || (r = dense_pointer(c, "inv_freq", p->inv_freq, 4, pairs == 0)))
+        return r;
+    const int64_t stride[2] = {p->position_batch_stride, p->position_token_stride};
+    if ((r = dense_strides(c, "positions", stride, nullptr, 2, 0, false))) return r;
+    a.in_place = p->x.data == p->out.data;
+    if (a.in_place && ((p->batch > 1 && p->x.batch_stride != p->out.batch_stride) || (p->tokens > 1 && p->x.token_stride != p->out.token_stride) ||
+                       (p->heads > 1 && p->x.head_stride != p->out.head_stride)))
+        return fail(c, LUTAMM_EINVAL, "out in place of x needs its strides");
+    a.x = p->x.data;
+    a.out = p->out.data;
+    a.x_batch = p->x.batch_stride; a.x_token = p->x.token_stride; a.x_head = p->x.head_stride;
+    a.out_batch = p->out.batch_stride; a.out_token = p->out.token_stride; a.out_head = p->out.head_stride;
+    a.positions = p->positions;
+    a.position_batch_stride = p->position_batch_stride;
+    a.position_token_stride = p->position_token_stride;
+    a.inv_freq = p->inv_freq;
+    a.batch = p->batch; a.tokens = p->tokens; a.heads = p->heads; a.head_dim = p->head_dim;
+    a.pairs = (uint32_t)pairs;
+    a.interleaved = p->interleaved != 0;
+    a.inverse = p->inverse != 0;
+    a.vec = on_16(p->x, size, p->batch, p->tokens, p->heads) && on_16(p->out, size, p->batch, p->tokens, p->heads);
+    return dense_done(c, launch_rotary(a, p->dtype, c->sm_count, c->stream), "rotary", 1, flags);
+}
+
+int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t flags) {
+    if (int r = dense_args(c, p, flags)) return r;
+    const size_t size = dtype_size(p->dtype);
+    if (!size) return fail(c, LUTAMM_EINVAL, "unknown dtype");
+    if (!p->head_dim || p->head_dim % 8 || p->head_dim > 128) return fail(c, LUTAMM_EINVAL, "head_dim must be a multiple of 8 up to 128");
+    if (!p->kv_heads || p->heads % p->kv_heads) return fail(c, LUTAMM_EINVAL, "heads must be a multiple of kv_heads");
+    if (p->keys >> 31 || p->queries >> 31) return fail(c, LUTAMM_EINVAL, "keys and queries must be below 2^31");
+    if (!std::isfinite(p->scale)) return fail(c, LUTAMM_EINVAL, "scale must be finite");
+    if (!p->batch || !p->queries || !p->heads) return LUTAMM_OK;
+    if ((uint64_t)p->batch * p->queries > (1ull << 40) / p->heads) return fail(c, LUTAMM_EINVAL, "batch * queries * heads must be at most 2^40");
+    DeviceGuard g(c->device);
+    int r;
+    lutamm_heads k = p->k, v = p->v;
+    if (!p->keys) k.data = v.data = p->q.data;   // nothing is read
+    if ((r = dense_heads(c, "q", p->q, size, p->batch, p->queries, p->heads, p->head_dim, false)) ||
+        (r = dense_heads(c, "k", k, size, p->batch, p->keys, p->kv_heads, p->head_dim, false)) ||
+        (r = dense_heads(c, "v", v, size, p->batch, p->keys, p->kv_heads, p->head_dim, false)) ||
+        (r = dense_heads(c, "out", p->out, size, p->batch, p->queries, p->heads, p->head_dim, true)) ||
+        (r = dense_pointer(c, "lengths", p->lengths, 4, true)) || (r = dense_pointer(c, "first", p->first, 4, true)))
+        return r;
+    if (p->out.data == p->q.data || (p->keys && (p->out.data == k.data || p->out.data == v.data))) return fail(c, LUTAMM_EINVAL, "out must not be an input");
+    AttentionArgs a{};
+    a.q = p->q.data; a.k = k.data; a.v = v.data; a.out = p->out.data;
+    a.q_batch = p->q.batch_stride; a.q_token = p->q.token_stride; a.q_head = p->q.head_stride;
+    a.k_batch = k.batch_stride; a.k_token = k.token_stride; a.k_head = k.head_stride;
+    a.v_batch = v.batch_stride; a.v_token = v.token_stride; a.v_head = v.head_stride;
+    a.out_batch = p->out.batch_stride; a.out_token = p->out.token_stride; a.out_head = p->out.head_stride;
+    a.lengths = p->lengths;
+    a.first = p->first;
+    a.batch = p->batch; a.queries = p->queries; a.keys = p->keys; a.heads = p->heads; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
+    a.sinks = p->sinks;
+    a.left = p->left < 0 ? -1 : p->left;
+    a.right = p->right < 0 ? -1 : p->right;
+    a.scale = p->scale * 1.4426950408889634f;
+    a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
+            on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
+    return dense_done(c, launch_attention_rows(a, p->dtype, c->sm_count, c->stream), "attention", 1, flags);
 }
 
 int lutamm_set_plan(lutamm_ctx* c, int layer_id, const lutamm_plan* plan) {
