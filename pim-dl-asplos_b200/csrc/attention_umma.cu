@@ -1,0 +1,651 @@
+// Attention for many rows, on the tensor cores:  out = softmax(scale q k^T) v  over the keys that a query sees (attention.cuh).
+//
+// A CTA takes 128 rows - query tokens times the query heads that share a key head - of one sequence through the keys that any of
+// them sees, 64 keys a tile: first the tiles of the sinks, then those of the window; tiles in between are never loaded.  With S = Q K^T
+// (tcgen05.mma, queries in tensor memory, keys in shared memory) in tensor memory, a thread owns a row: it reads the 64 scores,
+// keeps the running maximum m and sum l, and writes p = exp2(s - m) back over S, where the next product P V reads it as its operand;
+// the sum of the tiles' products, rescaled by exp2(m_old - m_new), stays in the thread's registers.  What is exchanged between
+// threads is two barriers a tile.  While a tile's weights are formed, the tensor core works on the next tile's scores and the last
+// tile's product: S is double, and two CTAs share an SM where head_dim is at most 64.
+//
+// Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.
+// fp32 operands are split into two f16 numbers, x = hi + lo to 22 bits, and hi hi + hi lo + lo hi is summed; the product of the rests, 2^-22
+// of the whole, is left out.  f16 ends at 65504 and thins out below 2^-14, so operands carry a power of two: queries one per row, keys
+// and values one per tile, kept from tile to tile for as long as the tile's largest value lies in 1/4 .. 32768 under it; the loading
+// warps look at that while they convert, and convert a tile once more where it does not.  Weights carry 2^14, the sum l with
+// them.  Maxima, sums and outputs are fp32.
+//
+// The loading warps read global memory with plain loads: any strides, no tensor maps, and rows behind the last key become zeros.
+// Where there are few CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no
+// scratch memory and one order of summation.
+#include "attention.cuh"
+#include "ptx.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace lutamm {
+namespace {
+
+constexpr int kRows = 128, kKeys = 64, kThreads = 384;
+constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
+constexpr float kBoost = 14.f;        // log2 of what weights are multiplied by
+
+template <typename T, int DP>
+struct Form {
+    static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
+    static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
+    static constexpr int kStages = kTile <= 8192 ? 4 : 2;
+    static constexpr int kSmem = 2 * kStages * kTile + 1024;
+    static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;
+    static constexpr int kColumns = kUsed <= 256 ? 256 : 512;
+    static constexpr int kCtas = DP <= 64 ? 2 : 1;                   // per SM
+    // Registers a thread by role.  Their sum is what the three warpgroups are launched with, 3 x 80 or 3 x 168.
+    static constexpr int kRowRegs = DP <= 64 ? 152 : 232, kLoadRegs = DP <= 64 ? 64 : 136, kIssueRegs = DP <= 64 ? 24 : 136;
+};
+static_assert(152 + 64 + 24 == 3 * 80 && 232 + 136 + 136 == 3 * 168);
+
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// kind::f16, fp32 sums, 128 rows: A in tensor memory, two elements a column; B in shared memory.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t idesc_f16(uint32_t n) {
+    constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (bf << 7) | (bf << 10) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
+}
+// B whose rows are the contraction axis: 64 elements, one swizzle row of 128 bytes, a row; eight rows a group.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t smem_addr) {
+    return umma_desc_k_sw128(smem_addr) | (static_cast<uint64_t>(1024u >> 4) << 16);
+}
+
+__device__ __forceinline__ uint32_t vote_or_128(uint32_t v) {   // barrier 1, the loading warps'
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.or.pred p, 1, 128, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r) : "r"(v) : "memory");
+    return r;
+}
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
+// The power of two that takes a largest value to 8 .. 16, up to 2^108 (results below 1e-32 have fewer bits); 0 for 0.
+__device__ __forceinline__ int exponent_for(uint32_t top_bits) { return top_bits == 0 ? 0 : min(108, 130 - (int)(top_bits >> 23)); }
+// x = hi + lo in f16, two at a time
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2(a, b, static_cast<__half*>(nullptr));
+    const float2 h = unpack2(hi, static_cast<__half*>(nullptr));
+    lo = pack2(a - h.x, b - h.y, static_cast<__half*>(nullptr));
+}
+// ... of numbers that may be infinite: their rest is none
+__device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2(a, b, static_cast<__half*>(nullptr));
+    const float2 h = unpack2(hi, static_cast<__half*>(nullptr));
+    const float x = a - h.x, y = b - h.y;
+    lo = pack2(x == x ? x : 0.f, y == y ? y : 0.f, static_cast<__half*>(nullptr));
+}
+
+// ones below bit n
+__device__ __forceinline__ uint64_t below(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+
+struct Bars {
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_full, pv_free, q_full;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, Form<T, DP>::kCtas)
+attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tiles, uint32_t* dev_err) {
+    using F = Form<T, DP>;
+    constexpr int kStages = F::kStages;
+    extern __shared__ unsigned char s_raw[];
+    __shared__ __align__(8) Bars s_bar;
+    __shared__ uint32_t s_tmem, s_abort, s_top[4];
+    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most kStages + 1 tiles ahead of who reads these
+    __shared__ float s_m[kRows], s_l[kRows];
+    unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
+    const uint32_t smem_at = smem_u32(smem);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+
+    const uint32_t shares = cluster_size_x(), share = cluster_rank();
+    uint64_t item = blockIdx.x / shares;
+    const uint32_t rt = (uint32_t)(item % row_tiles);
+    item /= row_tiles;
+    const uint32_t g = (uint32_t)(item % a.kv_heads), b = (uint32_t)(item / a.kv_heads);
+    const uint32_t per_head = a.heads / a.kv_heads;
+    const uint64_t rows = (uint64_t)a.queries * per_head, r0 = (uint64_t)rt * kRows;
+    const uint32_t n_rows = rows - r0 < kRows ? (uint32_t)(rows - r0) : kRows;
+    const int32_t length = key_count(a, b);
+    const int64_t first = a.first ? __ldg(a.first + b) : 0;
+    const int64_t p0 = first + (int64_t)(r0 / per_head), p1 = first + (int64_t)((r0 + n_rows - 1) / per_head);
+    KeySpan span = key_span(a, p0, p1, length);
+    if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;   // the window begins in the sinks' last tile
+    const uint32_t sink_tiles = (uint32_t)(span.sinks + kKeys - 1) / kKeys;
+    const uint32_t all_tiles = sink_tiles + (uint32_t)(((int64_t)span.hi - span.lo + kKeys - 1) / kKeys);
+    const uint32_t t0 = (uint32_t)((uint64_t)all_tiles * share / shares), tiles = (uint32_t)((uint64_t)all_tiles * (share + 1) / shares) - t0;
+    auto tile_keys = [&](uint32_t j, int32_t& k0, int32_t& end) {
+        const uint32_t t = t0 + j;
+        const bool sink = t < sink_tiles;
+        k0 = sink ? (int32_t)(t * kKeys) : span.lo + (int32_t)((t - sink_tiles) * kKeys);
+        end = sink ? span.sinks : span.hi;
+    };
+
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&s_tmem), F::kColumns);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(smem_u32(&s_bar.k_full[i]), 4);
+            mbar_init(smem_u32(&s_bar.k_empty[i]), 1);
+            mbar_init(smem_u32(&s_bar.v_full[i]), 4);
+            mbar_init(smem_u32(&s_bar.v_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s_bar.s_full[i]), 1);
+            mbar_init(smem_u32(&s_bar.p_full[i]), 4);
+        }
+        mbar_init(smem_u32(&s_bar.pv_full), 1);
+        mbar_init(smem_u32(&s_bar.pv_free), 4);
+        mbar_init(smem_u32(&s_bar.q_full), 4);
+        fence_barrier_init();
+        s_abort = 0;
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = s_tmem;
+    const uint32_t dim = a.head_dim;
+
+    auto write_row = [&](uint32_t r, uint32_t c, const float (&v)[4], float norm) {   // four elements from column c
+        const uint64_t row = r0 + r, qi = row / per_head;
+        const uint32_t head = g * per_head + (uint32_t)(row - qi * per_head);
+        T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
+        const float w[4] = {v[0] * norm, v[1] * norm, v[2] * norm, v[3] * norm};
+        if (a.vec) {
+            if constexpr (sizeof(T) == 4) store_elems<T, 4>(p, w);
+            else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(w[0], w[1], static_cast<T*>(nullptr)), pack2(w[2], w[3], static_cast<T*>(nullptr)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = from_float<T>(w[i]);
+        }
+    };
+    float4* s_o = reinterpret_cast<float4*>(smem);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
+
+    if (warp < 4) {
+        // ---------------------------------------------------------------- a row a thread
+        regs_up<F::kRowRegs>();
+        const uint32_t lanes = (warp * 32u) << 16;
+        const bool real = tid < n_rows;
+        const uint64_t row = r0 + (real ? tid : n_rows - 1);
+        const uint64_t qi = row / per_head;
+        const uint32_t head = g * per_head + (uint32_t)(row - qi * per_head);
+        const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
+        float factor = fabsf(a.scale);   // of this row's scores
+        {
+            const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)qi * a.q_token + (int64_t)head * a.q_head;
+            auto load8 = [&](uint32_t c, float (&v)[8]) {
+                if (!real || c >= dim) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+                } else if (a.vec) {
+                    if constexpr (sizeof(T) == 4) {
+                        float x[4], y[4];
+                        load_elems<T, 4>(qp + c, x);
+                        load_elems<T, 4>(qp + c + 4, y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { v[i] = x[i]; v[4 + i] = y[i]; }
+                    } else {
+                        load_elems<T, 8>(qp + c, v);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = to_float(qp[c + i]);
+                }
+            };
+            const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+            float up = sign;
+            if (a.scale == 0.f) factor = 1.f;
+            if constexpr (F::kParts == 2) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < DP; c += 8) {
+                    float v[8];
+                    load8(c, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+                        if (bits < 0x7F800000u) top = max(top, bits);
+                    }
+                }
+                const int e = exponent_for(top);
+                up *= power2(e);
+                factor *= power2(-e);
+            }
+#pragma unroll
+            for (int half = 0; half < F::kPanels; ++half) {
+                uint32_t hi[32], lo[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 8) {
+                    float v[8];
+                    load8(half * 64 + c, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = v[2 * i] * up, y = v[2 * i + 1] * up;
+                        if constexpr (F::kParts == 2) split2_any(x, y, hi[c / 2 + i], lo[c / 2 + i]);
+                        else hi[c / 2 + i] = pack2(x, y, static_cast<T*>(nullptr));
+                    }
+                }
+                tmem_st_32x32b_x32(tmem + lanes + F::kQuery + half * 32, hi);
+                if constexpr (F::kParts == 2) tmem_st_32x32b_x32(tmem + lanes + F::kQuery + DP / 2 + half * 32, lo);
+            }
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_bar.q_full));
+        }
+        float o[DP], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP; ++c) o[c] = 0.f;
+
+        // All rows see all of a tile that lies between these.
+        const int32_t common_hi = key_bounds(a, p0, length).hi, common_lo = key_bounds(a, p1, length).lo;
+        float shrink = 1.f;   // of o, by the last tile's new maximum
+        auto add_product = [&](uint32_t j) -> bool {
+            const bool ok = mbar_wait_warp(smem_u32(&s_bar.pv_full), j & 1u, &s_abort);
+            if (!ok) return false;
+            tc_fence_after_sync();
+            float up = power2(-(int)kBoost);
+            if constexpr (F::kParts == 2) up *= power2(-s_exp_v[j % 8]);
+            const bool same = __all_sync(0xffffffffu, shrink == 1.f);
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + lanes + F::kProduct + c, v);
+                if (!same) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[c + i] *= shrink;
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[c + i] = fmaf(__uint_as_float(v[i]), up, o[c + i]);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_bar.pv_free));
+            return true;
+        };
+        for (uint32_t j = 0; j < tiles; ++j) {
+            if (!mbar_wait_warp(smem_u32(&s_bar.s_full[j & 1u]), (j >> 1) & 1u, &s_abort)) break;
+            tc_fence_after_sync();
+            const uint32_t at = tmem + lanes + F::kScores + (j & 1u) * kKeys;
+            float c = factor;
+            if constexpr (F::kParts == 2) c *= power2(-s_exp_k[j % 8]);
+            uint32_t s0[32], s1[32];
+            tmem_ld_32x32b_x32(at, s0);
+            tmem_ld_32x32b_x32(at + 32, s1);
+            tmem_ld_wait();
+            int32_t k0, end;
+            tile_keys(j, k0, end);
+            if (!((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks))) {
+                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+                const uint32_t seen0 = (uint32_t)seen, seen1 = (uint32_t)(seen >> 32);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (!(seen0 >> i & 1u)) s0[i] = 0xFF800000u;
+                    if (!(seen1 >> i & 1u)) s1[i] = 0xFF800000u;
+                }
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                top[i & 1] = fmaxf(top[i & 1], __uint_as_float(s0[i]));
+                top[2 + (i & 1)] = fmaxf(top[2 + (i & 1)], __uint_as_float(s1[i]));
+            }
+            const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+            const float against = m_new == -INFINITY ? 0.f : m_new;
+            const float shrink_new = exp2_approx(m - against);
+            m = m_new;
+            const float off = kBoost - against;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t hi[32];
+            uint32_t lo[F::kParts == 2 ? 32 : 1];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float x = exp2_approx(fmaf(__uint_as_float(s0[i]), c, off)), y = exp2_approx(fmaf(__uint_as_float(s0[i + 1]), c, off));
+                sum[0] += x;
+                sum[1] += y;
+                if constexpr (F::kParts == 2) split2(x, y, hi[i / 2], lo[i / 2]);
+                else hi[i / 2] = pack2(x, y, static_cast<T*>(nullptr));
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float x = exp2_approx(fmaf(__uint_as_float(s1[i]), c, off)), y = exp2_approx(fmaf(__uint_as_float(s1[i + 1]), c, off));
+                sum[2] += x;
+                sum[3] += y;
+                if constexpr (F::kParts == 2) split2(x, y, hi[16 + i / 2], lo[16 + i / 2]);
+                else hi[16 + i / 2] = pack2(x, y, static_cast<T*>(nullptr));
+            }
+            tmem_st_32x32b_x32(at, hi);
+            if constexpr (F::kParts == 2) tmem_st_32x32b_x32(at + 32, lo);
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_bar.p_full[j & 1u]));
+            l = fmaf(l, shrink_new, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (j > 0 && !add_product(j - 1)) break;
+            shrink = shrink_new;
+        }
+        if (tiles > 0) add_product(tiles - 1);
+        l *= power2(-(int)kBoost);
+        if (shares == 1) {
+            if (tid < n_rows) {
+                const float norm = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int c = 0; c < DP; c += 4) {
+                    const float v[4] = {o[c], o[c + 1], o[c + 2], o[c + 3]};
+                    if ((uint32_t)c < dim) write_row(tid, c, v, norm);
+                }
+            }
+        } else {   // all products are done, so nothing reads the tiles any more
+#pragma unroll
+            for (int c = 0; c < DP / 4; ++c) s_o[tid * (DP / 4) + (c ^ (tid & (DP / 4 - 1)))] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            s_m[tid] = m;
+            s_l[tid] = l;
+        }
+    } else if (warp < 8) {
+        // ---------------------------------------------------------------- keys and values into shared memory
+        regs_down<F::kLoadRegs>();
+        const uint32_t t = tid - 128;
+        constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements
+        constexpr int kPerRow = DP / 8;
+        const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
+        const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head;
+        const uint32_t jobs = 2 * tiles;   // keys of a tile, values of a tile, ...
+        auto source = [&](uint32_t job, int i, const T*& p) -> bool {   // group i of this thread; false: zeros
+            int32_t k0, end;
+            tile_keys(job / 2, k0, end);
+            const uint32_t n = t + i * 128u, r = n / kPerRow, c = (n % kPerRow) * 8;
+            const int64_t key = (int64_t)k0 + r;
+            p = (job & 1u ? vp + key * a.v_token : kp + key * a.k_token) + c;
+            return key < end && c < dim;
+        };
+        auto slot = [&](uint32_t job) -> uint32_t { return (job & 1u ? kStages * F::kTile : 0) + (job / 2 % kStages) * F::kTile; };
+        auto place = [&](int i) -> uint32_t {
+            const uint32_t n = t + i * 128u, r = n / kPerRow, c = n % kPerRow;
+            return (c / 8) * kPanel + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
+        };
+        auto wait_empty = [&](uint32_t job) {   // no early way out: the four warps meet at a barrier for every tile
+            const uint32_t use = job / 2 / kStages, st = job / 2 % kStages;
+            if (use > 0) mbar_wait_warp(smem_u32(job & 1u ? &s_bar.v_empty[st] : &s_bar.k_empty[st]), (use - 1) & 1u, &s_abort);
+        };
+        auto publish = [&](uint32_t job) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            const uint32_t st = job / 2 % kStages;
+            if (lane == 0) mbar_arrive(smem_u32(job & 1u ? &s_bar.v_full[st] : &s_bar.k_full[st]));
+        };
+        if constexpr (F::kParts == 2) {
+            float buf[kPerThread][8];
+            auto fetch = [&](uint32_t job, int i) {
+                const T* p;
+                const bool in = source(job, i, p);
+                if (in && a.vec) {
+                    float x[4], y[4];
+                    load_elems<float, 4>(reinterpret_cast<const float*>(p), x);
+                    load_elems<float, 4>(reinterpret_cast<const float*>(p) + 4, y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { buf[i][e] = x[e]; buf[i][4 + e] = y[e]; }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) buf[i][e] = in ? to_float(p[e]) : 0.f;
+                }
+            };
+            auto convert = [&](uint32_t at, int i, float up, bool any) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (any) split2_any(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
+                    else split2(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
+                }
+                unsigned char* p = smem + at + place(i);
+                *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(p + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            };
+            int exps[2] = {0, 0};   // keys', values'
+            if (jobs > 0) {
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) fetch(0, i);
+            }
+            for (uint32_t job = 0; job < jobs; ++job) {
+                wait_empty(job);
+                const uint32_t at = slot(job), which = job & 1u;
+                const float up = power2(which ? exps[1] : exps[0]);
+                uint32_t top = 0;
+                const bool more = job + 1 < jobs;
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(buf[i][e]) & 0x7FFFFFFFu);
+                    convert(at, i, up, false);
+                    if (more) fetch(job + 1, i);
+                }
+                // largest value of this thread: 0, or 2^-2 .. 2^15 under the power of two in use (2^-2 of some thread is enough)
+                const int reach = (int)(top >> 23) - 127 + (which ? exps[1] : exps[0]);
+                const bool high = reach >= 15, enough = reach >= -2 && top != 0;
+                const uint32_t any_high = vote_or_128(high), any_enough = vote_or_128(enough), any_value = vote_or_128(top != 0);
+                if (any_high || (any_value && !any_enough)) {   // this tile again, with a power of two of its own
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int i = 0; i < kPerThread; ++i) {
+                        fetch(job, i);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
+                            if (bits < 0x7F800000u) big = max(big, bits);
+                        }
+                    }
+                    big = __reduce_max_sync(0xffffffffu, big);
+                    if (lane == 0) s_top[warp - 4] = big;
+                    vote_or_128(0);
+                    big = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+                    vote_or_128(0);   // s_top is read
+                    const int e = exponent_for(big);
+                    if (which) exps[1] = e; else exps[0] = e;
+#pragma unroll
+                    for (int i = 0; i < kPerThread; ++i) {
+                        convert(at, i, power2(e), true);
+                        if (more) fetch(job + 1, i);
+                    }
+                }
+                if (t == 0) (which ? s_exp_v : s_exp_k)[job / 2 % 8] = which ? exps[1] : exps[0];
+                publish(job);
+            }
+        } else {
+            constexpr uint32_t kAhead = 2;   // tiles whose copies are in flight
+            for (uint32_t job = 0; job < jobs; ++job) {
+                wait_empty(job);
+                const uint32_t at = slot(job);
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+                    const T* p;
+                    const bool in = source(job, i, p);
+                    const uint32_t to = at + place(i);
+                    if (a.vec) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + to), "l"(in ? p : kp), "r"(in ? 16 : 0) : "memory");
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = in ? pack2(to_float(p[2 * e]), to_float(p[2 * e + 1]), static_cast<T*>(nullptr)) : 0u;
+                        *reinterpret_cast<uint4*>(smem + to) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (job >= kAhead) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+                    publish(job - kAhead);
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            for (uint32_t job = jobs > kAhead ? jobs - kAhead : 0; job < jobs; ++job) publish(job);
+        }
+    } else {
+        // ---------------------------------------------------------------- the tensor core's instructions
+        regs_down<F::kIssueRegs>();
+        if (warp == 8 && tiles > 0) {
+            const uint32_t k_steps = (dim + 15) / 16;
+            auto scores = [&](uint32_t j) {   // S = Q K^T, the small products first
+                const uint32_t d = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + (j % kStages) * F::kTile;
+                const uint32_t idesc = idesc_f16<T>(kKeys);
+                uint32_t more = 0;
+#pragma unroll
+                for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+                    const uint32_t qa = tmem + F::kQuery + (term == 1 ? DP / 2 : 0);
+                    const uint32_t kb = at + (term == 0 ? F::kPanels * kPanel : 0);
+                    for (uint32_t s = 0; s < k_steps; ++s) {
+                        umma_f16_ts(d, qa + s * 8, umma_desc_k_sw128(kb + (s / 4) * kPanel + (s % 4) * 32), idesc, more);
+                        more = 1;
+                    }
+                }
+            };
+            auto product = [&](uint32_t j) {
+                const uint32_t p = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + kStages * F::kTile + (j % kStages) * F::kTile;
+#pragma unroll
+                for (int panel = 0; panel < F::kPanels; ++panel) {
+                    const uint32_t left = dim - panel * 64u, n = left >= 64 ? 64 : (left + 15) / 16 * 16;
+                    const uint32_t idesc = idesc_f16<T>(n) | kIdescColumnMajorB;
+                    uint32_t more = 0;
+#pragma unroll
+                    for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+                        const uint32_t pa = p + (term == 1 ? 32 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
+#pragma unroll
+                        for (uint32_t s = 0; s < 4; ++s) {
+                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + s * 8, desc_rows(vb + s * 2048), idesc, more);
+                            more = 1;
+                        }
+                    }
+                }
+            };
+            bool ok = mbar_wait_warp(smem_u32(&s_bar.q_full), 0, &s_abort);
+            ok = ok && mbar_wait_warp(smem_u32(&s_bar.k_full[0]), 0, &s_abort);
+            if (ok) {
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    scores(0);
+                    umma_commit(smem_u32(&s_bar.s_full[0]));
+                    umma_commit(smem_u32(&s_bar.k_empty[0]));
+                }
+                __syncwarp();
+            }
+            for (uint32_t j = 0; ok && j < tiles; ++j) {
+                if (j + 1 < tiles) {
+                    // the next tile's scores go where the weights of the tile before this one lie: its product has to be done
+                    if (j > 0) ok = mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort);
+                    ok = ok && mbar_wait_warp(smem_u32(&s_bar.k_full[(j + 1) % kStages]), ((j + 1) / kStages) & 1u, &s_abort);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    if (elect_one()) {
+                        scores(j + 1);
+                        umma_commit(smem_u32(&s_bar.s_full[(j + 1) & 1u]));
+                        umma_commit(smem_u32(&s_bar.k_empty[(j + 1) % kStages]));
+                    }
+                    __syncwarp();
+                }
+                ok = mbar_wait_warp(smem_u32(&s_bar.p_full[j & 1u]), (j >> 1) & 1u, &s_abort);
+                ok = ok && mbar_wait_warp(smem_u32(&s_bar.v_full[j % kStages]), (j / kStages) & 1u, &s_abort);
+                if (ok && j > 0) ok = mbar_wait_warp(smem_u32(&s_bar.pv_free), (j - 1) & 1u, &s_abort);
+                if (!ok) break;
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    product(j);
+                    umma_commit(smem_u32(&s_bar.pv_full));
+                    umma_commit(smem_u32(&s_bar.v_empty[j % kStages]));
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (shares > 1) {
+        cluster_sync();
+        const uint32_t per_row = dim / 4;
+        for (uint32_t i = share * kThreads + tid; i < n_rows * per_row; i += shares * kThreads) {
+            const uint32_t r = i / per_row, c = i - r * per_row;
+            const uint32_t at_m = smem_u32(&s_m[r]), at_l = smem_u32(&s_l[r]), at_o = smem_u32(&s_o[r * (DP / 4) + (c ^ (r & (DP / 4 - 1)))]);
+            float top = -INFINITY, total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t k = 0; k < shares; ++k) top = fmaxf(top, load_shared_cluster(map_to_rank(at_m, k)));
+            for (uint32_t k = 0; k < shares; ++k) {
+                const float mk = load_shared_cluster(map_to_rank(at_m, k)), lk = load_shared_cluster(map_to_rank(at_l, k));
+                const float f = mk == -INFINITY ? 0.f : exp2_approx(mk - top);
+                total += f == 0.f ? (lk != lk ? lk : 0.f) : lk * f;   // a sum that is no number stays one
+                if (f != 0.f) {
+                    const uint32_t at = map_to_rank(at_o, k);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = fmaf(load_shared_cluster(at + 4 * e), f, v[e]);
+                }
+            }
+            write_row(r, c * 4, v, total == 0.f ? 0.f : 1.f / total);
+        }
+        cluster_sync();   // what the others read is read
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == 8 && s_abort) {   // what is in flight gets time to end before its columns are handed back
+        const long long from = clock64();
+        while (clock64() - from < 200000) {}
+        if (lane == 0) report_error(dev_err, 7);
+    }
+    if (warp == 8) tmem_dealloc(tmem, F::kColumns);
+}
+
+template <typename T, int DP>
+cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
+    using F = Form<T, DP>;
+    static SmemOptIn memo;
+    cudaError_t e = allow_smem(memo, attention_umma_kernel<T, DP>, F::kSmem);
+    if (e != cudaSuccess) return e;
+    const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads), tiles = (rows + kRows - 1) / kRows;
+    const uint64_t items = (uint64_t)a.batch * a.kv_heads * tiles;
+    // Keys that a tile of rows sees at most.
+    uint64_t keys = a.keys;
+    if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
+    uint32_t shares = 1;
+    while (shares < 8 && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kKeys) shares *= 2;
+    if (items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((uint32_t)(items * shares));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = F::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = shares;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP>, a, (uint32_t)tiles, dev_err);
+}
+
+template <typename T>
+cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
+    return a.head_dim <= 64 ? run<T, 64>(a, sm_count, dev_err, s) : run<T, 128>(a, sm_count, dev_err, s);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_umma(const AttentionArgs& a, uint32_t dtype, int sm_count, uint32_t* dev_err, cudaStream_t s) {
+    if (!a.batch || !a.queries || !a.heads) return cudaSuccess;
+    return dtype == 0 ? pick<float>(a, sm_count, dev_err, s) : dtype == 1 ? pick<__half>(a, sm_count, dev_err, s) : pick<__nv_bfloat16>(a, sm_count, dev_err, s);
+}
+
+}  // namespace lutamm

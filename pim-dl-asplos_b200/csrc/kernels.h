@@ -208,6 +208,8 @@ struct AttentionArgs {
 };
 // Few rows (query tokens x heads of a key head): one pass over keys and values on the CUDA cores.
 cudaError_t launch_attention_rows(const AttentionArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
+// Many rows: on the tensor cores.
+cudaError_t launch_attention_umma(const AttentionArgs& a, uint32_t dtype, int sm_count, uint32_t* dev_err, cudaStream_t s);
 
 // The opt-in to more than 48 KB of dynamic shared memory, asked for once per kernel, device and size (the call takes a
 // good part of a microsecond): remembers, per kernel, the largest size asked for on each device.

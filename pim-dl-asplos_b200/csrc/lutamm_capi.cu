@@ -1063,7 +1063,10 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.scale = p->scale * 1.4426950408889634f;
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
-    return dense_done(c, launch_attention_rows(a, p->dtype, c->sm_count, c->stream), "attention", 1, flags);
+    const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
+    const cudaError_t e = rows <= 8 ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
+                                    : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
+    return dense_done(c, e, "attention", 1, flags);
 }
 
 int lutamm_set_plan(lutamm_ctx* c, int layer_id, const lutamm_plan* plan) {
