@@ -15,7 +15,8 @@
 // warps look at that while they convert, and convert a tile once more where it does not.  Weights carry 2^14, the sum l with
 // them.  Maxima, sums and outputs are fp32.
 //
-// The loading warps read global memory with plain loads: any strides, no tensor maps, and rows behind the last key become zeros.
+// The loading warps read global memory with plain 16-byte loads: no tensor maps, and rows behind the last key become zeros.  Tensors that
+// do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.
 // Where there are few CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no
 // scratch memory and one order of summation.
 #include "attention.cuh"
@@ -29,6 +30,7 @@ namespace {
 
 constexpr int kRows = 128, kKeys = 64, kThreads = 384;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
+constexpr uint32_t kMostShares = 8;
 constexpr float kBoost = 14.f;        // log2 of what weights are multiplied by
 
 template <typename T, int DP>
@@ -67,24 +69,48 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t smem_addr) {
     return umma_desc_k_sw128(smem_addr) | (static_cast<uint64_t>(1024u >> 4) << 16);
 }
 
-__device__ __forceinline__ uint32_t vote_or_128(uint32_t v) {   // barrier 1, the loading warps'
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %1, 0;\n\t"
-        "barrier.cta.red.or.pred p, 1, 128, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(r) : "r"(v) : "memory");
-    return r;
-}
+__device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }   // the loading warps
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
 // The power of two that takes a largest value to 8 .. 16, up to 2^108 (results below 1e-32 have fewer bits); 0 for 0.
 __device__ __forceinline__ int exponent_for(uint32_t top_bits) { return top_bits == 0 ? 0 : min(108, 130 - (int)(top_bits >> 23)); }
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // x = hi + lo in f16, two at a time
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = pack2(a, b, static_cast<__half*>(nullptr));
     const float2 h = unpack2(hi, static_cast<__half*>(nullptr));
-    lo = pack2(a - h.x, b - h.y, static_cast<__half*>(nullptr));
+    const float2 rest = unpair(fma2(pair(h.x, h.y), pair(-1.f, -1.f), pair(a, b)));
+    lo = pack2(rest.x, rest.y, static_cast<__half*>(nullptr));
 }
 // ... of numbers that may be infinite: their rest is none
 __device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -108,24 +134,24 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     constexpr int kStages = F::kStages;
     extern __shared__ unsigned char s_raw[];
     __shared__ __align__(8) Bars s_bar;
-    __shared__ uint32_t s_tmem, s_abort, s_top[4];
+    __shared__ uint32_t s_tmem, s_abort, s_top[3][4];
     __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most kStages + 1 tiles ahead of who reads these
-    __shared__ float s_m[kRows], s_l[kRows];
+    __shared__ float s_m[kRows], s_l[kRows], s_part[kMostShares][kRows];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
 
     const uint32_t shares = cluster_size_x(), share = cluster_rank();
-    uint64_t item = blockIdx.x / shares;
-    const uint32_t rt = (uint32_t)(item % row_tiles);
+    uint32_t item = blockIdx.x / shares;
+    const uint32_t rt = item % row_tiles;
     item /= row_tiles;
-    const uint32_t g = (uint32_t)(item % a.kv_heads), b = (uint32_t)(item / a.kv_heads);
+    const uint32_t g = item % a.kv_heads, b = item / a.kv_heads;
     const uint32_t per_head = a.heads / a.kv_heads;
-    const uint64_t rows = (uint64_t)a.queries * per_head, r0 = (uint64_t)rt * kRows;
-    const uint32_t n_rows = rows - r0 < kRows ? (uint32_t)(rows - r0) : kRows;
+    const uint32_t rows = a.queries * per_head, r0 = rt * kRows;   // below 2^31
+    const uint32_t n_rows = min(rows - r0, (uint32_t)kRows);
     const int32_t length = key_count(a, b);
     const int64_t first = a.first ? __ldg(a.first + b) : 0;
-    const int64_t p0 = first + (int64_t)(r0 / per_head), p1 = first + (int64_t)((r0 + n_rows - 1) / per_head);
+    const int64_t p0 = first + r0 / per_head, p1 = first + (r0 + n_rows - 1) / per_head;
     KeySpan span = key_span(a, p0, p1, length);
     if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;   // the window begins in the sinks' last tile
     const uint32_t sink_tiles = (uint32_t)(span.sinks + kKeys - 1) / kKeys;
@@ -166,17 +192,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     const uint32_t dim = a.head_dim;
 
     auto write_row = [&](uint32_t r, uint32_t c, const float (&v)[4], float norm) {   // four elements from column c
-        const uint64_t row = r0 + r, qi = row / per_head;
-        const uint32_t head = g * per_head + (uint32_t)(row - qi * per_head);
+        const uint32_t row = r0 + r, qi = row / per_head, head = g * per_head + (row - qi * per_head);
         T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
         const float w[4] = {v[0] * norm, v[1] * norm, v[2] * norm, v[3] * norm};
-        if (a.vec) {
-            if constexpr (sizeof(T) == 4) store_elems<T, 4>(p, w);
-            else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(w[0], w[1], static_cast<T*>(nullptr)), pack2(w[2], w[3], static_cast<T*>(nullptr)));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = from_float<T>(w[i]);
-        }
+        if constexpr (sizeof(T) == 4) store_elems<T, 4>(p, w);
+        else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(w[0], w[1], static_cast<T*>(nullptr)), pack2(w[2], w[3], static_cast<T*>(nullptr)));
     };
     float4* s_o = reinterpret_cast<float4*>(smem);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
 
@@ -185,76 +205,79 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         regs_up<F::kRowRegs>();
         const uint32_t lanes = (warp * 32u) << 16;
         const bool real = tid < n_rows;
-        const uint64_t row = r0 + (real ? tid : n_rows - 1);
-        const uint64_t qi = row / per_head;
-        const uint32_t head = g * per_head + (uint32_t)(row - qi * per_head);
+        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = row / per_head, head = g * per_head + (row - qi * per_head);
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
-        float factor = fabsf(a.scale);   // of this row's scores
+        float factor = fabsf(a.scale), q_up = 1.f;   // of this row's scores; of its query
         {
             const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)qi * a.q_token + (int64_t)head * a.q_head;
-            auto load8 = [&](uint32_t c, float (&v)[8]) {
-                if (!real || c >= dim) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                } else if (a.vec) {
-                    if constexpr (sizeof(T) == 4) {
-                        float x[4], y[4];
-                        load_elems<T, 4>(qp + c, x);
-                        load_elems<T, 4>(qp + c + 4, y);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) { v[i] = x[i]; v[4 + i] = y[i]; }
-                    } else {
-                        load_elems<T, 8>(qp + c, v);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = to_float(qp[c + i]);
-                }
-            };
             const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
-            float up = sign;
             if (a.scale == 0.f) factor = 1.f;
-            if constexpr (F::kParts == 2) {
-                uint32_t top = 0;
+            constexpr int E = kPer16<T>;
 #pragma unroll
-                for (int c = 0; c < DP; c += 8) {
-                    float v[8];
-                    load8(c, v);
+            for (int panel = 0; panel < F::kPanels; ++panel) {   // (fp32: the power of two is the row's, so its largest value comes first)
+                uint4 raw[64 / E];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-                        if (bits < 0x7F800000u) top = max(top, bits);
+                for (int i = 0; i < 64 / E; ++i) {
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (real && panel * 64u + i * E < dim) raw[i] = __ldg(reinterpret_cast<const uint4*>(qp + panel * 64 + i * E));
+                }
+                if constexpr (F::kParts == 2) {
+                    if (panel == 0) {
+                        uint32_t top = 0;
+                        auto look = [&](uint32_t bits) {
+                            bits &= 0x7FFFFFFFu;
+                            if (bits < 0x7F800000u) top = max(top, bits);
+                        };
+#pragma unroll
+                        for (int i = 0; i < 64 / E; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
+                        if constexpr (F::kPanels == 2) {
+#pragma unroll 4
+                            for (uint32_t c = 64; c < dim; c += E) {
+                                if (real) {
+                                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(qp + c));
+                                    look(w.x); look(w.y); look(w.z); look(w.w);
+                                }
+                            }
+                        }
+                        const int e = exponent_for(top);
+                        q_up = power2(e);
+                        factor *= power2(-e);
                     }
                 }
-                const int e = exponent_for(top);
-                up *= power2(e);
-                factor *= power2(-e);
-            }
+                const float up = sign * q_up;
 #pragma unroll
-            for (int half = 0; half < F::kPanels; ++half) {
-                uint32_t hi[32], lo[32];
+                for (int part = 0; part < 64 / E / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
+                    if constexpr (F::kParts == 2) {
+                        uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int c = 0; c < 64; c += 8) {
-                    float v[8];
-                    load8(half * 64 + c, v);
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 w = raw[part * 4 + i];
+                            split2_any(__uint_as_float(w.x) * up, __uint_as_float(w.y) * up, hi[2 * i], lo[2 * i]);
+                            split2_any(__uint_as_float(w.z) * up, __uint_as_float(w.w) * up, hi[2 * i + 1], lo[2 * i + 1]);
+                        }
+                        tmem_st_32x32b_x8(tmem + lanes + F::kQuery + panel * 32 + part * 8, hi);
+                        tmem_st_32x32b_x8(tmem + lanes + F::kQuery + DP / 2 + panel * 32 + part * 8, lo);
+                    } else {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = v[2 * i] * up, y = v[2 * i + 1] * up;
-                        if constexpr (F::kParts == 2) split2_any(x, y, hi[c / 2 + i], lo[c / 2 + i]);
-                        else hi[c / 2 + i] = pack2(x, y, static_cast<T*>(nullptr));
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t u[4] = {raw[part * 4 + i].x, raw[part * 4 + i].y, raw[part * 4 + i].z, raw[part * 4 + i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w[4 * i + k] = a.scale > 0.f ? u[k] : a.scale < 0.f ? u[k] ^ 0x80008000u : 0u;
+                        }
+                        tmem_st_32x32b_x16(tmem + lanes + F::kQuery + panel * 32 + part * 16, w);
                     }
                 }
-                tmem_st_32x32b_x32(tmem + lanes + F::kQuery + half * 32, hi);
-                if constexpr (F::kParts == 2) tmem_st_32x32b_x32(tmem + lanes + F::kQuery + DP / 2 + half * 32, lo);
             }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_bar.q_full));
         }
-        float o[DP], m = -INFINITY, l = 0.f;
+        uint64_t o[DP / 2];   // two columns each
+        float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int c = 0; c < DP; ++c) o[c] = 0.f;
+        for (int c = 0; c < DP / 2; ++c) o[c] = 0;
 
         // All rows see all of a tile that lies between these.
         const int32_t common_hi = key_bounds(a, p0, length).hi, common_lo = key_bounds(a, p1, length).lo;
@@ -271,12 +294,14 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 uint32_t v[32];
                 tmem_ld_32x32b_x32(tmem + lanes + F::kProduct + c, v);
                 if (!same) {
+                    const uint64_t f = pair(shrink, shrink);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[c + i] *= shrink;
+                    for (int i = 0; i < 16; ++i) o[c / 2 + i] = mul2(o[c / 2 + i], f);
                 }
                 tmem_ld_wait();
+                const uint64_t u = pair(up, up);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[c + i] = fmaf(__uint_as_float(v[i]), up, o[c + i]);
+                for (int i = 0; i < 16; ++i) o[c / 2 + i] = fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), u, o[c / 2 + i]);
             }
             tc_fence_before_sync();
             __syncwarp();
@@ -289,58 +314,72 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             const uint32_t at = tmem + lanes + F::kScores + (j & 1u) * kKeys;
             float c = factor;
             if constexpr (F::kParts == 2) c *= power2(-s_exp_k[j % 8]);
-            uint32_t s0[32], s1[32];
-            tmem_ld_32x32b_x32(at, s0);
-            tmem_ld_32x32b_x32(at + 32, s1);
-            tmem_ld_wait();
             int32_t k0, end;
             tile_keys(j, k0, end);
-            if (!((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks))) {
-                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
-                const uint32_t seen0 = (uint32_t)seen, seen1 = (uint32_t)(seen >> 32);
+            uint32_t seen0 = 0xFFFFFFFFu, seen1 = 0xFFFFFFFFu;
+            const bool edge = !((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks));
+            if (edge) {
+                const uint64_t all = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+                seen0 = (uint32_t)all;
+                seen1 = (uint32_t)(all >> 32);
+            }
+            auto hide = [&](uint32_t (&sc)[32], uint32_t bits) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (!(seen0 >> i & 1u)) s0[i] = 0xFF800000u;
-                    if (!(seen1 >> i & 1u)) s1[i] = 0xFF800000u;
+                for (int i = 0; i < 32; ++i)
+                    if (!(bits >> i & 1u)) sc[i] = 0xFF800000u;
+            };
+            // The scores are read twice, for the maximum and for the weights: 64 of them and the output are more than the registers hold.
+            float top = -INFINITY;
+            {
+                uint32_t s0[32], s1[32];
+                tmem_ld_32x32b_x32(at, s0);
+                tmem_ld_32x32b_x32(at + 32, s1);
+                tmem_ld_wait();
+                if (edge) {
+                    hide(s0, seen0);
+                    hide(s1, seen1);
                 }
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                top[i & 1] = fmaxf(top[i & 1], __uint_as_float(s0[i]));
-                top[2 + (i & 1)] = fmaxf(top[2 + (i & 1)], __uint_as_float(s1[i]));
+                for (int i = 0; i < 32; i += 4) {
+                    t4[0] = max3(t4[0], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+                    t4[1] = max3(t4[1], __uint_as_float(s0[i + 2]), __uint_as_float(s0[i + 3]));
+                    t4[2] = max3(t4[2], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+                    t4[3] = max3(t4[3], __uint_as_float(s1[i + 2]), __uint_as_float(s1[i + 3]));
+                }
+                top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
             }
-            const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
+            const float m_new = fmaxf(m, top * c);
             const float against = m_new == -INFINITY ? 0.f : m_new;
             const float shrink_new = exp2_approx(m - against);
             m = m_new;
-            const float off = kBoost - against;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t hi[32];
-            uint32_t lo[F::kParts == 2 ? 32 : 1];
+            const uint64_t off = pair(kBoost - against, kBoost - against), cc = pair(c, c);
+            uint64_t sum[2] = {0, 0};
+            // Weights of 32 keys where the first scores of those lay: 16 columns, and fp32's rests in the 16 behind them.
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                uint32_t sc[32], hi[16];
+                tmem_ld_32x32b_x32(at + half * 32, sc);
+                tmem_ld_wait();
+                if (edge) hide(sc, half ? seen1 : seen0);
+                uint32_t lo[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float x = exp2_approx(fmaf(__uint_as_float(s0[i]), c, off)), y = exp2_approx(fmaf(__uint_as_float(s0[i + 1]), c, off));
-                sum[0] += x;
-                sum[1] += y;
-                if constexpr (F::kParts == 2) split2(x, y, hi[i / 2], lo[i / 2]);
-                else hi[i / 2] = pack2(x, y, static_cast<T*>(nullptr));
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
+                    const float p = exp2_approx(x.x), q = exp2_approx(x.y);
+                    sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
+                    if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
+                    else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
+                }
+                tmem_st_32x32b_x16(at + half * 32, hi);
+                if constexpr (F::kParts == 2) tmem_st_32x32b_x16(at + half * 32 + 16, lo);
             }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float x = exp2_approx(fmaf(__uint_as_float(s1[i]), c, off)), y = exp2_approx(fmaf(__uint_as_float(s1[i + 1]), c, off));
-                sum[2] += x;
-                sum[3] += y;
-                if constexpr (F::kParts == 2) split2(x, y, hi[16 + i / 2], lo[16 + i / 2]);
-                else hi[16 + i / 2] = pack2(x, y, static_cast<T*>(nullptr));
-            }
-            tmem_st_32x32b_x32(at, hi);
-            if constexpr (F::kParts == 2) tmem_st_32x32b_x32(at + 32, lo);
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_bar.p_full[j & 1u]));
-            l = fmaf(l, shrink_new, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            const float2 sums = unpair(add2(sum[0], sum[1]));
+            l = fmaf(l, shrink_new, sums.x + sums.y);
             if (j > 0 && !add_product(j - 1)) break;
             shrink = shrink_new;
         }
@@ -351,13 +390,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 const float norm = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
                 for (int c = 0; c < DP; c += 4) {
-                    const float v[4] = {o[c], o[c + 1], o[c + 2], o[c + 3]};
+                    const float2 x = unpair(o[c / 2]), y = unpair(o[c / 2 + 1]);
+                    const float v[4] = {x.x, x.y, y.x, y.y};
                     if ((uint32_t)c < dim) write_row(tid, c, v, norm);
                 }
             }
         } else {   // all products are done, so nothing reads the tiles any more
 #pragma unroll
-            for (int c = 0; c < DP / 4; ++c) s_o[tid * (DP / 4) + (c ^ (tid & (DP / 4 - 1)))] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            for (int c = 0; c < DP / 4; ++c) {
+                const float2 x = unpair(o[2 * c]), y = unpair(o[2 * c + 1]);
+                s_o[tid * (DP / 4) + (c ^ (tid & (DP / 4 - 1)))] = make_float4(x.x, x.y, y.x, y.y);
+            }
             s_m[tid] = m;
             s_l[tid] = l;
         }
@@ -365,24 +408,35 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
         const uint32_t t = tid - 128;
-        constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements
-        constexpr int kPerRow = DP / 8;
-        const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
-        const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head;
+        constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements: of one column, kStepRows rows apart
+        constexpr int kPerRow = DP / 8, kStepRows = 128 / kPerRow;
+        const uint32_t my_row = t / kPerRow, my_col = t % kPerRow;
+        const bool in_dim = my_col * 8 < dim;
+        const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head + (in_dim ? my_col * 8 : 0);
+        const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head + (in_dim ? my_col * 8 : 0);
+        const int64_t k_step = a.k_token * kStepRows, v_step = a.v_token * kStepRows;
+        // where this thread's first group lies in a tile; the rows of its others differ by multiples of eight, which leaves the swizzle as it is
+        const uint32_t place = (my_col / 8) * kPanel + my_row * 128u + (((my_col & 7u) ^ (my_row & 7u)) << 4);
+        constexpr uint32_t kPlaceStep = kStepRows * 128;
         const uint32_t jobs = 2 * tiles;   // keys of a tile, values of a tile, ...
-        auto source = [&](uint32_t job, int i, const T*& p) -> bool {   // group i of this thread; false: zeros
+        // A job's source: this thread's first group, the step between its groups and how many of the groups hold keys.
+        struct Source {
+            const T* p;
+            int64_t step;
+            int n;
+        };
+        auto source = [&](uint32_t job) -> Source {
             int32_t k0, end;
             tile_keys(job / 2, k0, end);
-            const uint32_t n = t + i * 128u, r = n / kPerRow, c = (n % kPerRow) * 8;
-            const int64_t key = (int64_t)k0 + r;
-            p = (job & 1u ? vp + key * a.v_token : kp + key * a.k_token) + c;
-            return key < end && c < dim;
+            const int32_t rows_left = end - k0 - (int32_t)my_row;
+            Source s;
+            s.n = !in_dim || rows_left <= 0 ? 0 : min(kPerThread, (rows_left + kStepRows - 1) / kStepRows);
+            const int64_t key = (int64_t)k0 + my_row;
+            s.p = job & 1u ? vp + key * a.v_token : kp + key * a.k_token;
+            s.step = job & 1u ? v_step : k_step;
+            return s;
         };
         auto slot = [&](uint32_t job) -> uint32_t { return (job & 1u ? kStages * F::kTile : 0) + (job / 2 % kStages) * F::kTile; };
-        auto place = [&](int i) -> uint32_t {
-            const uint32_t n = t + i * 128u, r = n / kPerRow, c = n % kPerRow;
-            return (c / 8) * kPanel + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
-        };
         auto wait_empty = [&](uint32_t job) {   // no early way out: the four warps meet at a barrier for every tile
             const uint32_t use = job / 2 / kStages, st = job / 2 % kStages;
             if (use > 0) mbar_wait_warp(smem_u32(job & 1u ? &s_bar.v_empty[st] : &s_bar.k_empty[st]), (use - 1) & 1u, &s_abort);
@@ -395,19 +449,15 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         };
         if constexpr (F::kParts == 2) {
             float buf[kPerThread][8];
-            auto fetch = [&](uint32_t job, int i) {
-                const T* p;
-                const bool in = source(job, i, p);
-                if (in && a.vec) {
-                    float x[4], y[4];
-                    load_elems<float, 4>(reinterpret_cast<const float*>(p), x);
-                    load_elems<float, 4>(reinterpret_cast<const float*>(p) + 4, y);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { buf[i][e] = x[e]; buf[i][4 + e] = y[e]; }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) buf[i][e] = in ? to_float(p[e]) : 0.f;
+            auto fetch = [&](const Source& from, int i) {
+                const T* p = from.p + i * from.step;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                if (i < from.n) {
+                    x = __ldg(reinterpret_cast<const float4*>(p));
+                    y = __ldg(reinterpret_cast<const float4*>(p) + 1);
                 }
+                buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
+                buf[i][4] = y.x; buf[i][5] = y.y; buf[i][6] = y.z; buf[i][7] = y.w;
             };
             auto convert = [&](uint32_t at, int i, float up, bool any) {
                 uint32_t hi[4], lo[4];
@@ -416,14 +466,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                     if (any) split2_any(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
                     else split2(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
                 }
-                unsigned char* p = smem + at + place(i);
+                unsigned char* p = smem + at + place + i * kPlaceStep;
                 *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<uint4*>(p + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             };
+            // The largest of all loading threads' bits, by turns in three places: a warp is at most one tile ahead of another.
+            auto tile_top = [&](uint32_t top, uint32_t turn) -> uint32_t {
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) s_top[turn][warp - 4] = top;
+                sync_128();
+                return max(max(s_top[turn][0], s_top[turn][1]), max(s_top[turn][2], s_top[turn][3]));
+            };
             int exps[2] = {0, 0};   // keys', values'
             if (jobs > 0) {
+                const Source from = source(0);
 #pragma unroll
-                for (int i = 0; i < kPerThread; ++i) fetch(0, i);
+                for (int i = 0; i < kPerThread; ++i) fetch(from, i);
             }
             for (uint32_t job = 0; job < jobs; ++job) {
                 wait_empty(job);
@@ -431,39 +489,35 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 const float up = power2(which ? exps[1] : exps[0]);
                 uint32_t top = 0;
                 const bool more = job + 1 < jobs;
+                const Source next = source(more ? job + 1 : job);
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(buf[i][e]) & 0x7FFFFFFFu);
                     convert(at, i, up, false);
-                    if (more) fetch(job + 1, i);
+                    if (more) fetch(next, i);
                 }
-                // largest value of this thread: 0, or 2^-2 .. 2^15 under the power of two in use (2^-2 of some thread is enough)
+                // The tile's largest value: 0, or 2^-2 .. 2^15 under the power of two in use, or the tile is converted again with one of its own.
+                top = tile_top(top, job & 1u);
                 const int reach = (int)(top >> 23) - 127 + (which ? exps[1] : exps[0]);
-                const bool high = reach >= 15, enough = reach >= -2 && top != 0;
-                const uint32_t any_high = vote_or_128(high), any_enough = vote_or_128(enough), any_value = vote_or_128(top != 0);
-                if (any_high || (any_value && !any_enough)) {   // this tile again, with a power of two of its own
+                if (top != 0 && (reach >= 15 || reach < -2)) {
                     uint32_t big = 0;
+                    const Source from = source(job);
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i) {
-                        fetch(job, i);
+                        fetch(from, i);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
                             if (bits < 0x7F800000u) big = max(big, bits);
                         }
                     }
-                    big = __reduce_max_sync(0xffffffffu, big);
-                    if (lane == 0) s_top[warp - 4] = big;
-                    vote_or_128(0);
-                    big = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-                    vote_or_128(0);   // s_top is read
-                    const int e = exponent_for(big);
+                    const int e = exponent_for(tile_top(big, 2));
                     if (which) exps[1] = e; else exps[0] = e;
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i) {
                         convert(at, i, power2(e), true);
-                        if (more) fetch(job + 1, i);
+                        if (more) fetch(next, i);
                     }
                 }
                 if (t == 0) (which ? s_exp_v : s_exp_k)[job / 2 % 8] = which ? exps[1] : exps[0];
@@ -473,20 +527,14 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             constexpr uint32_t kAhead = 2;   // tiles whose copies are in flight
             for (uint32_t job = 0; job < jobs; ++job) {
                 wait_empty(job);
-                const uint32_t at = slot(job);
+                const uint32_t at = slot(job) + place;
+                const Source from = source(job);
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
-                    const T* p;
-                    const bool in = source(job, i, p);
-                    const uint32_t to = at + place(i);
-                    if (a.vec) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + to), "l"(in ? p : kp), "r"(in ? 16 : 0) : "memory");
-                    } else {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = in ? pack2(to_float(p[2 * e]), to_float(p[2 * e + 1]), static_cast<T*>(nullptr)) : 0u;
-                        *reinterpret_cast<uint4*>(smem + to) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    const bool in = i < from.n;
+                    const T* p = in ? from.p + i * from.step : kp;
+                    const uint32_t to = at + i * kPlaceStep;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + to), "l"(p), "r"(in ? 16 : 0) : "memory");
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (job >= kAhead) {
@@ -525,10 +573,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                     uint32_t more = 0;
 #pragma unroll
                     for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
-                        const uint32_t pa = p + (term == 1 ? 32 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
+                        const uint32_t pa = p + (term == 1 ? 16 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
 #pragma unroll
                         for (uint32_t s = 0; s < 4; ++s) {
-                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + s * 8, desc_rows(vb + s * 2048), idesc, more);
+                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + s / 2 * 32 + s % 2 * 8, desc_rows(vb + s * 2048), idesc, more);
                             more = 1;
                         }
                     }
@@ -576,23 +624,41 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
 
     if (shares > 1) {
         cluster_sync();
+        if (tid < n_rows) {   // what each part of a row counts for in the result
+            float mk[kMostShares], lk[kMostShares], top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (uint32_t k = 0; k < kMostShares; ++k) {
+                mk[k] = k < shares ? load_shared_cluster(map_to_rank(smem_u32(&s_m[tid]), k)) : -INFINITY;
+                lk[k] = k < shares ? load_shared_cluster(map_to_rank(smem_u32(&s_l[tid]), k)) : 0.f;
+                top = fmaxf(top, mk[k]);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kMostShares; ++k) {
+                mk[k] = mk[k] == -INFINITY ? 0.f : exp2_approx(mk[k] - top);
+                total += mk[k] == 0.f ? (lk[k] != lk[k] ? lk[k] : 0.f) : lk[k] * mk[k];   // a sum that is no number stays one
+            }
+            const float norm = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+            for (uint32_t k = 0; k < kMostShares; ++k)
+                if (k < shares) s_part[k][tid] = mk[k] == 0.f && norm == norm ? 0.f : mk[k] * norm;
+        }
+        __syncthreads();
         const uint32_t per_row = dim / 4;
         for (uint32_t i = share * kThreads + tid; i < n_rows * per_row; i += shares * kThreads) {
             const uint32_t r = i / per_row, c = i - r * per_row;
-            const uint32_t at_m = smem_u32(&s_m[r]), at_l = smem_u32(&s_l[r]), at_o = smem_u32(&s_o[r * (DP / 4) + (c ^ (r & (DP / 4 - 1)))]);
-            float top = -INFINITY, total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (uint32_t k = 0; k < shares; ++k) top = fmaxf(top, load_shared_cluster(map_to_rank(at_m, k)));
-            for (uint32_t k = 0; k < shares; ++k) {
-                const float mk = load_shared_cluster(map_to_rank(at_m, k)), lk = load_shared_cluster(map_to_rank(at_l, k));
-                const float f = mk == -INFINITY ? 0.f : exp2_approx(mk - top);
-                total += f == 0.f ? (lk != lk ? lk : 0.f) : lk * f;   // a sum that is no number stays one
-                if (f != 0.f) {
-                    const uint32_t at = map_to_rank(at_o, k);
+            const uint32_t at_o = smem_u32(&s_o[r * (DP / 4) + (c ^ (r & (DP / 4 - 1)))]);
+            float4 x[kMostShares];
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = fmaf(load_shared_cluster(at + 4 * e), f, v[e]);
+            for (uint32_t k = 0; k < kMostShares; ++k)
+                if (k < shares) x[k] = load_shared_cluster4(map_to_rank(at_o, k));
+#pragma unroll
+            for (uint32_t k = 0; k < kMostShares; ++k)
+                if (k < shares) {
+                    const float f = s_part[k][r];
+                    if (f != 0.f) { v[0] = fmaf(x[k].x, f, v[0]); v[1] = fmaf(x[k].y, f, v[1]); v[2] = fmaf(x[k].z, f, v[2]); v[3] = fmaf(x[k].w, f, v[3]); }
                 }
-            }
-            write_row(r, c * 4, v, total == 0.f ? 0.f : 1.f / total);
+            write_row(r, c * 4, v, 1.f);
         }
         cluster_sync();   // what the others read is read
     }
@@ -619,8 +685,8 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     uint64_t keys = a.keys;
     if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
     uint32_t shares = 1;
-    while (shares < 8 && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kKeys) shares *= 2;
-    if (items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    while (shares < kMostShares && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kKeys) shares *= 2;
+    if (rows > 0x7FFFFFFFull || items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((uint32_t)(items * shares));
     cfg.blockDim = dim3(kThreads);

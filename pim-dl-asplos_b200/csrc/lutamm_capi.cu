@@ -1036,7 +1036,8 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     if (p->keys >> 31 || p->queries >> 31) return fail(c, LUTAMM_EINVAL, "keys and queries must be below 2^31");
     if (!std::isfinite(p->scale)) return fail(c, LUTAMM_EINVAL, "scale must be finite");
     if (!p->batch || !p->queries || !p->heads) return LUTAMM_OK;
-    if ((uint64_t)p->batch * p->queries > (1ull << 40) / p->heads) return fail(c, LUTAMM_EINVAL, "batch * queries * heads must be at most 2^40");
+    if ((uint64_t)p->queries * p->heads >> 31 || (uint64_t)p->batch * p->queries > (1ull << 40) / p->heads)
+        return fail(c, LUTAMM_EINVAL, "queries * heads must be below 2^31 and batch * queries * heads at most 2^40");
     DeviceGuard g(c->device);
     int r;
     lutamm_heads k = p->k, v = p->v;
@@ -1064,7 +1065,7 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
     const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
-    const cudaError_t e = rows <= 8 ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
+    const cudaError_t e = rows <= 8 || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
                                     : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
     return dense_done(c, e, "attention", 1, flags);
 }
