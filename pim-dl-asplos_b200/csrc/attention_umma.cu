@@ -31,14 +31,19 @@ namespace {
 constexpr int kRows = 128, kKeys = 64, kThreads = 384;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
 constexpr uint32_t kMostShares = 8;
-constexpr float kBoost = 14.f;        // log2 of what weights are multiplied by
+// Tensor memory adds up towards zero: a sum of n products is short by about 3e-8 of its size a tile, 1.3e-5 at 16000 keys.  fp32's output is
+// taken into registers, where sums are rounded, every so many tiles; half the bits do not show it.
+constexpr uint32_t kChunk = 8;
+constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 template <typename T, int DP>
 struct Form {
     static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
     static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
-    static constexpr int kStages = kTile <= 8192 ? 4 : 2;
-    static constexpr int kSmem = 2 * kStages * kTile + 1024;
+    static constexpr int kSlots = 6;                                 // of the ring that keys and values take by turns
+    static constexpr int kAhead = 3;                                 // tiles on their way
+    static constexpr int kSmem = kSlots * kTile + 1024;
+    static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles in registers: see kChunk
     static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;
     static constexpr int kColumns = kUsed <= 256 ? 256 : 512;
     static constexpr int kCtas = DP <= 64 ? 2 : 1;                   // per SM
@@ -94,11 +99,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -124,18 +124,18 @@ __device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint3
 __device__ __forceinline__ uint64_t below(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 struct Bars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_full, pv_free, q_full;
+    uint64_t full[6], empty[6], s_full[2], p_full[2], pv_full, all_done, q_full;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, Form<T, DP>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tiles, uint32_t* dev_err) {
     using F = Form<T, DP>;
-    constexpr int kStages = F::kStages;
+    constexpr uint32_t kSlots = F::kSlots;
     extern __shared__ unsigned char s_raw[];
     __shared__ __align__(8) Bars s_bar;
     __shared__ uint32_t s_tmem, s_abort, s_top[3][4];
-    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most kStages + 1 tiles ahead of who reads these
+    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most three tiles ahead of who reads these
     __shared__ float s_m[kRows], s_l[kRows], s_part[kMostShares][kRows];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
@@ -169,18 +169,16 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(smem_u32(&s_bar.k_full[i]), 4);
-            mbar_init(smem_u32(&s_bar.k_empty[i]), 1);
-            mbar_init(smem_u32(&s_bar.v_full[i]), 4);
-            mbar_init(smem_u32(&s_bar.v_empty[i]), 1);
+        for (int i = 0; i < F::kSlots; ++i) {
+            mbar_init(smem_u32(&s_bar.full[i]), 4);
+            mbar_init(smem_u32(&s_bar.empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&s_bar.s_full[i]), 1);
             mbar_init(smem_u32(&s_bar.p_full[i]), 4);
         }
         mbar_init(smem_u32(&s_bar.pv_full), 1);
-        mbar_init(smem_u32(&s_bar.pv_free), 4);
+        mbar_init(smem_u32(&s_bar.all_done), 1);
         mbar_init(smem_u32(&s_bar.q_full), 4);
         fence_barrier_init();
         s_abort = 0;
@@ -191,10 +189,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     const uint32_t tmem = s_tmem;
     const uint32_t dim = a.head_dim;
 
-    auto write_row = [&](uint32_t r, uint32_t c, const float (&v)[4], float norm) {   // four elements from column c
+    auto write_row = [&](uint32_t r, uint32_t c, const float (&w)[4]) {   // four elements from column c
         const uint32_t row = r0 + r, qi = row / per_head, head = g * per_head + (row - qi * per_head);
         T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
-        const float w[4] = {v[0] * norm, v[1] * norm, v[2] * norm, v[3] * norm};
         if constexpr (sizeof(T) == 4) store_elems<T, 4>(p, w);
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(w[0], w[1], static_cast<T*>(nullptr)), pack2(w[2], w[3], static_cast<T*>(nullptr)));
     };
@@ -274,136 +271,217 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_bar.q_full));
         }
-        uint64_t o[DP / 2];   // two columns each
-        float m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int c = 0; c < DP / 2; ++c) o[c] = 0;
-
         // All rows see all of a tile that lies between these.
         const int32_t common_hi = key_bounds(a, p0, length).hi, common_lo = key_bounds(a, p1, length).lo;
-        float shrink = 1.f;   // of o, by the last tile's new maximum
-        auto add_product = [&](uint32_t j) -> bool {
-            const bool ok = mbar_wait_warp(smem_u32(&s_bar.pv_full), j & 1u, &s_abort);
-            if (!ok) return false;
-            tc_fence_after_sync();
-            float up = power2(-(int)kBoost);
-            if constexpr (F::kParts == 2) up *= power2(-s_exp_v[j % 8]);
-            const bool same = __all_sync(0xffffffffu, shrink == 1.f);
+        float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
+        const uint32_t out_at = tmem + lanes + F::kProduct;
+        // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is o, against m_o
+        uint64_t o[F::kSums ? DP / 2 : 1];
+        float m_o = -INFINITY;
+        int unit = 0;
+        if constexpr (F::kSums) {
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem + lanes + F::kProduct + c, v);
-                if (!same) {
-                    const uint64_t f = pair(shrink, shrink);
+            for (int i = 0; i < DP / 2; ++i) o[i] = 0;
+        }
+        auto add_chunk = [&]() {
+            const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against), up = power2(-unit);
+            const uint64_t f2 = pair(f, f), up2 = pair(up, up);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[c / 2 + i] = mul2(o[c / 2 + i], f);
-                }
+            for (int col = 0; col < DP; col += 16) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(out_at + col, v);
                 tmem_ld_wait();
-                const uint64_t u = pair(up, up);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[c / 2 + i] = fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), u, o[c / 2 + i]);
+                for (int i = 0; i < 8; ++i) {
+                    uint64_t& x = o[col / 2 + i];
+                    x = fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), up2, fma2(x, f2, 0ull));
+                }
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_bar.pv_free));
-            return true;
+            m_o = m;
         };
         for (uint32_t j = 0; j < tiles; ++j) {
             if (!mbar_wait_warp(smem_u32(&s_bar.s_full[j & 1u]), (j >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
             const uint32_t at = tmem + lanes + F::kScores + (j & 1u) * kKeys;
+            bool begun = j > 0;   // whether tensor memory holds an output to go on with
+            if constexpr (F::kSums) {
+                begun = j % kChunk != 0;
+                if (j > 0 && !begun) {
+                    if (!mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort)) break;
+                    tc_fence_after_sync();
+                    add_chunk();
+                }
+            }
             float c = factor;
-            if constexpr (F::kParts == 2) c *= power2(-s_exp_k[j % 8]);
+            int e = 0;
+            if constexpr (F::kParts == 2) {
+                c *= power2(-s_exp_k[j % 8]);
+                // the values' power of two is known once they are in shared memory, which the keys' turn does not wait for
+                if (!mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
+                e = s_exp_v[j % 8];
+            }
+            c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             int32_t k0, end;
             tile_keys(j, k0, end);
             uint32_t seen0 = 0xFFFFFFFFu, seen1 = 0xFFFFFFFFu;
             const bool edge = !((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks));
             if (edge) {
-                const uint64_t all = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
-                seen0 = (uint32_t)all;
-                seen1 = (uint32_t)(all >> 32);
+                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+                seen0 = (uint32_t)seen;
+                seen1 = (uint32_t)(seen >> 32);
             }
+            auto read = [&](uint32_t (&sc)[32], int half) {
+                tmem_ld_32x32b_x32(at + half * 32, sc);
+            };
             auto hide = [&](uint32_t (&sc)[32], uint32_t bits) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     if (!(bits >> i & 1u)) sc[i] = 0xFF800000u;
             };
-            // The scores are read twice, for the maximum and for the weights: 64 of them and the output are more than the registers hold.
-            float top = -INFINITY;
-            {
-                uint32_t s0[32], s1[32];
-                tmem_ld_32x32b_x32(at, s0);
-                tmem_ld_32x32b_x32(at + 32, s1);
-                tmem_ld_wait();
-                if (edge) {
-                    hide(s0, seen0);
-                    hide(s1, seen1);
-                }
-                float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto largest = [&](const uint32_t (&sc)[32]) {
+                float t[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    t4[0] = max3(t4[0], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
-                    t4[1] = max3(t4[1], __uint_as_float(s0[i + 2]), __uint_as_float(s0[i + 3]));
-                    t4[2] = max3(t4[2], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
-                    t4[3] = max3(t4[3], __uint_as_float(s1[i + 2]), __uint_as_float(s1[i + 3]));
+                    t[0] = max3(t[0], __uint_as_float(sc[i]), __uint_as_float(sc[i + 1]));
+                    t[1] = max3(t[1], __uint_as_float(sc[i + 2]), __uint_as_float(sc[i + 3]));
                 }
-                top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
+                return fmaxf(t[0], t[1]);
+            };
+            uint32_t s0[32], s1[32];
+            read(s0, 0);
+            read(s1, 1);
+            tmem_ld_wait();
+            if (edge) {
+                hide(s0, seen0);
+                hide(s1, seen1);
             }
-            const float m_new = fmaxf(m, top * c);
-            const float against = m_new == -INFINITY ? 0.f : m_new;
-            const float shrink_new = exp2_approx(m - against);
-            m = m_new;
-            const uint64_t off = pair(kBoost - against, kBoost - against), cc = pair(c, c);
-            uint64_t sum[2] = {0, 0};
-            // Weights of 32 keys where the first scores of those lay: 16 columns, and fp32's rests in the 16 behind them.
+            const float top = fmaxf(largest(s0), largest(s1)) * c;
+            // Another maximum, or another power of two of the values: the output so far is brought in line, where there is one.
+            float more = kBoost;   // log2 of what this tile's weights carry
+            if (m == -INFINITY) m = top;
+            if (!begun || m == -INFINITY) unit = e;
+            if (__any_sync(0xffffffffu, top > m + kSlack || unit != e)) {
+                const float m_new = top > m + kSlack ? top : m;
+                const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
+                if (begun) {
+                    if (!mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort)) break;
+                    tc_fence_after_sync();
+                    float f = shrink;
+                    if constexpr (F::kParts == 2) {
+                        float big = 0.f;
 #pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                uint32_t sc[32], hi[16];
-                tmem_ld_32x32b_x32(at + half * 32, sc);
-                tmem_ld_wait();
-                if (edge) hide(sc, half ? seen1 : seen0);
-                uint32_t lo[16];
+                        for (uint32_t col = 0; col < DP; col += 16) {
+                            uint32_t v[16];
+                            tmem_ld_32x32b_x16(out_at + col, v);
+                            tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
-                    const float p = exp2_approx(x.x), q = exp2_approx(x.y);
-                    sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
-                    if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
-                    else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
+                            for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
+                        }
+                        // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
+                        const int x = max(-120, min(120, e - unit));
+                        if (x <= 0 || big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2))) {
+                            f *= power2(x);
+                            unit = e;
+                        }
+                    }
+#pragma unroll 1
+                    for (uint32_t col = 0; col < DP; col += 16) {
+                        uint32_t v[16];
+                        tmem_ld_32x32b_x16(out_at + col, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st_32x32b_x16(out_at + col, v);
+                    }
+                    tmem_st_wait();
                 }
-                tmem_st_32x32b_x16(at + half * 32, hi);
-                if constexpr (F::kParts == 2) tmem_st_32x32b_x16(at + half * 32 + 16, lo);
+                l *= shrink;
+                m = m_new;
+            }
+            const float against = m == -INFINITY ? 0.f : m;
+            float back = 1.f;
+            if constexpr (F::kParts == 2) {
+                const int x = max(-120, unit - e);
+                more += (float)x;
+                back = power2(-x);
+            }
+            const uint64_t off = pair(more - against, more - against), cc = pair(c, c);
+            uint64_t sum[2] = {0, 0};
+            if constexpr (F::kSums) {
+                // Here the registers hold o, too: the scores are read once more, half by half.  Weights of 32 keys go where their scores lay,
+                // 16 columns of them and 16 of their rests.
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t sc[32], hi[16], lo[16];
+                    read(sc, half);
+                    tmem_ld_wait();
+                    if (edge) hide(sc, half ? seen1 : seen0);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
+                        const float p = exp2_approx(x.x), q = exp2_approx(x.y);
+                        sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
+                        split2(p, q, hi[i / 2], lo[i / 2]);
+                    }
+                    tmem_st_32x32b_x16(at + half * 32, hi);
+                    tmem_st_32x32b_x16(at + half * 32 + 16, lo);
+                }
+            } else {
+                uint32_t w[32];
+                auto weights = [&](const uint32_t (&sc)[32], int to) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
+                        const float p = exp2_approx(x.x), q = exp2_approx(x.y);
+                        sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
+                        w[to + i / 2] = pack2(p, q, static_cast<std::conditional_t<sizeof(T) == 4, __half, T>*>(nullptr));
+                    }
+                };
+                weights(s0, 0);
+                weights(s1, 16);
+                tmem_st_32x32b_x32(at, w);
             }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_bar.p_full[j & 1u]));
             const float2 sums = unpair(add2(sum[0], sum[1]));
-            l = fmaf(l, shrink_new, sums.x + sums.y);
-            if (j > 0 && !add_product(j - 1)) break;
-            shrink = shrink_new;
+            l = fmaf(sums.x + sums.y, back, l);
         }
-        if (tiles > 0) add_product(tiles - 1);
-        l *= power2(-(int)kBoost);
-        if (shares == 1) {
-            if (tid < n_rows) {
-                const float norm = l == 0.f ? 0.f : 1.f / l;
+        // A barrier's wait tells a phase from the one before it alone, and here the last two products may be done or under way: a barrier of its own.
+        const bool done = tiles > 0 && mbar_wait_warp(smem_u32(&s_bar.all_done), 0, &s_abort);
+        tc_fence_after_sync();
+        const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        auto put = [&](uint32_t col, float x0, float x1, float x2, float x3) {   // (a row that sees nothing may hold what others' values left)
+            const float x[4] = {norm == 0.f ? 0.f : x0 * norm, norm == 0.f ? 0.f : x1 * norm, norm == 0.f ? 0.f : x2 * norm, norm == 0.f ? 0.f : x3 * norm};
+            if (shares > 1) s_o[tid * (DP / 4) + ((col / 4) ^ (tid & (DP / 4 - 1)))] = make_float4(x[0], x[1], x[2], x[3]);   // all products are done: nothing reads the tiles
+            else if (real && col < dim) write_row(tid, col, x);
+        };
+        if constexpr (F::kSums) {
+            if (done) add_chunk();
 #pragma unroll
-                for (int c = 0; c < DP; c += 4) {
-                    const float2 x = unpair(o[c / 2]), y = unpair(o[c / 2 + 1]);
-                    const float v[4] = {x.x, x.y, y.x, y.y};
-                    if ((uint32_t)c < dim) write_row(tid, c, v, norm);
+            for (int col = 0; col < DP; col += 4) {
+                const float2 x = unpair(o[col / 2]), y = unpair(o[col / 2 + 1]);
+                put(col, x.x, x.y, y.x, y.y);
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t col = 0; col < DP; col += 16) {
+                if (col >= dim) break;
+                uint32_t v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0;
+                if (done) {
+                    tmem_ld_32x32b_x16(out_at + col, v);
+                    tmem_ld_wait();
                 }
-            }
-        } else {   // all products are done, so nothing reads the tiles any more
 #pragma unroll
-            for (int c = 0; c < DP / 4; ++c) {
-                const float2 x = unpair(o[2 * c]), y = unpair(o[2 * c + 1]);
-                s_o[tid * (DP / 4) + (c ^ (tid & (DP / 4 - 1)))] = make_float4(x.x, x.y, y.x, y.y);
+                for (int i = 0; i < 16; i += 4)
+                    put(col + i, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
             }
-            s_m[tid] = m;
-            s_l[tid] = l;
         }
+        s_m[tid] = m;
+        s_l[tid] = l;
     } else if (warp < 8) {
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
@@ -436,122 +514,102 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             s.step = job & 1u ? v_step : k_step;
             return s;
         };
-        auto slot = [&](uint32_t job) -> uint32_t { return (job & 1u ? kStages * F::kTile : 0) + (job / 2 % kStages) * F::kTile; };
-        auto wait_empty = [&](uint32_t job) {   // no early way out: the four warps meet at a barrier for every tile
-            const uint32_t use = job / 2 / kStages, st = job / 2 % kStages;
-            if (use > 0) mbar_wait_warp(smem_u32(job & 1u ? &s_bar.v_empty[st] : &s_bar.k_empty[st]), (use - 1) & 1u, &s_abort);
+        auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
+        // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
+        auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
+            if (job >= kSlots) mbar_wait_warp(smem_u32(&s_bar.empty[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
+            const Source from = source(job);
+            const uint32_t at = smem_at + slot(job);
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const bool in = i < from.n;
+                const T* p = in ? from.p + i * from.step : kp;
+#pragma unroll
+                for (int h = 0; h < F::kParts; ++h) {   // fp32: two pieces of 16 bytes, to where this thread alone reads them
+                    const uint32_t to = F::kParts == 2 ? at + (i * 2 + h) * 2048 + t * 16 : at + place + i * kPlaceStep;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? p + h * 4 : kp), "r"(in ? 16 : 0) : "memory");
+                }
+            }
         };
         auto publish = [&](uint32_t job) {
             fence_proxy_async_smem();
             __syncwarp();
-            const uint32_t st = job / 2 % kStages;
-            if (lane == 0) mbar_arrive(smem_u32(job & 1u ? &s_bar.v_full[st] : &s_bar.k_full[st]));
+            if (lane == 0) mbar_arrive(smem_u32(&s_bar.full[job % kSlots]));
         };
-        if constexpr (F::kParts == 2) {
-            float buf[kPerThread][8];
-            auto fetch = [&](const Source& from, int i) {
-                const T* p = from.p + i * from.step;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                if (i < from.n) {
-                    x = __ldg(reinterpret_cast<const float4*>(p));
-                    y = __ldg(reinterpret_cast<const float4*>(p) + 1);
-                }
-                buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
-                buf[i][4] = y.x; buf[i][5] = y.y; buf[i][6] = y.z; buf[i][7] = y.w;
-            };
-            auto convert = [&](uint32_t at, int i, float up, bool any) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (any) split2_any(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
-                    else split2(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
-                }
-                unsigned char* p = smem + at + place + i * kPlaceStep;
-                *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(p + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            };
-            // The largest of all loading threads' bits, by turns in three places: a warp is at most one tile ahead of another.
-            auto tile_top = [&](uint32_t top, uint32_t turn) -> uint32_t {
-                top = __reduce_max_sync(0xffffffffu, top);
-                if (lane == 0) s_top[turn][warp - 4] = top;
-                sync_128();
-                return max(max(s_top[turn][0], s_top[turn][1]), max(s_top[turn][2], s_top[turn][3]));
-            };
-            int exps[2] = {0, 0};   // keys', values'
-            if (jobs > 0) {
-                const Source from = source(0);
-#pragma unroll
-                for (int i = 0; i < kPerThread; ++i) fetch(from, i);
-            }
-            for (uint32_t job = 0; job < jobs; ++job) {
-                wait_empty(job);
-                const uint32_t at = slot(job), which = job & 1u;
-                const float up = power2(which ? exps[1] : exps[0]);
+        // The largest of all loading threads' bits, by turns in three places: a warp is at most one tile ahead of another.
+        auto tile_top = [&](uint32_t top, uint32_t turn) -> uint32_t {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) s_top[turn][warp - 4] = top;
+            sync_128();
+            return max(max(s_top[turn][0], s_top[turn][1]), max(s_top[turn][2], s_top[turn][3]));
+        };
+        int exp_k = 0, exp_v = 0;
+        for (uint32_t job = 0; job < F::kAhead; ++job) {
+            if (job < jobs) copy(job);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        for (uint32_t job = 0; job < jobs; ++job) {
+            if (job + F::kAhead < jobs) copy(job + F::kAhead);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(F::kAhead) : "memory");
+            if constexpr (F::kParts == 2) {   // in place, from what this thread has copied itself
+                unsigned char* at = smem + slot(job);
+                float buf[kPerThread][8];
                 uint32_t top = 0;
-                const bool more = job + 1 < jobs;
-                const Source next = source(more ? job + 1 : job);
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(at + (i * 2) * 2048 + t * 16), y = *reinterpret_cast<const float4*>(at + (i * 2 + 1) * 2048 + t * 16);
+                    buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
+                    buf[i][4] = y.x; buf[i][5] = y.y; buf[i][6] = y.z; buf[i][7] = y.w;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(buf[i][e]) & 0x7FFFFFFFu);
-                    convert(at, i, up, false);
-                    if (more) fetch(next, i);
                 }
-                // The tile's largest value: 0, or 2^-2 .. 2^15 under the power of two in use, or the tile is converted again with one of its own.
-                top = tile_top(top, job & 1u);
-                const int reach = (int)(top >> 23) - 127 + (which ? exps[1] : exps[0]);
+                top = tile_top(top, job & 1u);   // behind it everybody has read
+                // 0, or 2^-2 .. 2^15 under the power of two in use, or the tile gets one of its own.
+                int& e_now = job & 1u ? exp_v : exp_k;
+                const int reach = (int)(top >> 23) - 127 + e_now;
                 if (top != 0 && (reach >= 15 || reach < -2)) {
-                    uint32_t big = 0;
-                    const Source from = source(job);
+                    if (top >= 0x7F800000u) {   // the largest that is a number
+                        uint32_t big = 0;
 #pragma unroll
-                    for (int i = 0; i < kPerThread; ++i) {
-                        fetch(from, i);
+                        for (int i = 0; i < kPerThread; ++i)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
-                            if (bits < 0x7F800000u) big = max(big, bits);
-                        }
-                    }
-                    const int e = exponent_for(tile_top(big, 2));
-                    if (which) exps[1] = e; else exps[0] = e;
-#pragma unroll
-                    for (int i = 0; i < kPerThread; ++i) {
-                        convert(at, i, power2(e), true);
-                        if (more) fetch(next, i);
+                            for (int e = 0; e < 8; ++e) {
+                                const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
+                                if (bits < 0x7F800000u) big = max(big, bits);
+                            }
+                        big = tile_top(big, 2);
+                        const int r = (int)(big >> 23) - 127 + e_now;
+                        if (big != 0 && (r >= 15 || r < -2)) e_now = exponent_for(big);
+                    } else {
+                        e_now = exponent_for(top);
                     }
                 }
-                if (t == 0) (which ? s_exp_v : s_exp_k)[job / 2 % 8] = which ? exps[1] : exps[0];
-                publish(job);
-            }
-        } else {
-            constexpr uint32_t kAhead = 2;   // tiles whose copies are in flight
-            for (uint32_t job = 0; job < jobs; ++job) {
-                wait_empty(job);
-                const uint32_t at = slot(job) + place;
-                const Source from = source(job);
+                const float up = power2(e_now);
+                unsigned char* to = at + place;
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
-                    const bool in = i < from.n;
-                    const T* p = in ? from.p + i * from.step : kp;
-                    const uint32_t to = at + i * kPlaceStep;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + to), "l"(p), "r"(in ? 16 : 0) : "memory");
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (top >= 0x7F800000u) split2_any(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
+                        else split2(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
+                    }
+                    *reinterpret_cast<uint4*>(to + i * kPlaceStep) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(to + i * kPlaceStep + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (job >= kAhead) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-                    publish(job - kAhead);
-                }
+                if (t == 0) (job & 1u ? s_exp_v : s_exp_k)[job / 2 % 8] = e_now;
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            for (uint32_t job = jobs > kAhead ? jobs - kAhead : 0; job < jobs; ++job) publish(job);
+            publish(job);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // ---------------------------------------------------------------- the tensor core's instructions
         regs_down<F::kIssueRegs>();
         if (warp == 8 && tiles > 0) {
             const uint32_t k_steps = (dim + 15) / 16;
             auto scores = [&](uint32_t j) {   // S = Q K^T, the small products first
-                const uint32_t d = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + (j % kStages) * F::kTile;
+                const uint32_t d = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + 2 * j % kSlots * F::kTile;
                 const uint32_t idesc = idesc_f16<T>(kKeys);
                 uint32_t more = 0;
 #pragma unroll
@@ -565,31 +623,31 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 }
             };
             auto product = [&](uint32_t j) {
-                const uint32_t p = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + kStages * F::kTile + (j % kStages) * F::kTile;
+                const uint32_t p = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + (2 * j + 1) % kSlots * F::kTile;
 #pragma unroll
                 for (int panel = 0; panel < F::kPanels; ++panel) {
                     const uint32_t left = dim - panel * 64u, n = left >= 64 ? 64 : (left + 15) / 16 * 16;
                     const uint32_t idesc = idesc_f16<T>(n) | kIdescColumnMajorB;
-                    uint32_t more = 0;
+                    uint32_t more = F::kSums ? j % kChunk != 0 : j > 0;
 #pragma unroll
                     for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
                         const uint32_t pa = p + (term == 1 ? 16 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
 #pragma unroll
                         for (uint32_t s = 0; s < 4; ++s) {
-                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + s / 2 * 32 + s % 2 * 8, desc_rows(vb + s * 2048), idesc, more);
+                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), desc_rows(vb + s * 2048), idesc, more);
                             more = 1;
                         }
                     }
                 }
             };
             bool ok = mbar_wait_warp(smem_u32(&s_bar.q_full), 0, &s_abort);
-            ok = ok && mbar_wait_warp(smem_u32(&s_bar.k_full[0]), 0, &s_abort);
+            ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[0]), 0, &s_abort);
             if (ok) {
                 tc_fence_after_sync();
                 if (elect_one()) {
                     scores(0);
                     umma_commit(smem_u32(&s_bar.s_full[0]));
-                    umma_commit(smem_u32(&s_bar.k_empty[0]));
+                    umma_commit(smem_u32(&s_bar.empty[0]));
                 }
                 __syncwarp();
             }
@@ -597,25 +655,25 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 if (j + 1 < tiles) {
                     // the next tile's scores go where the weights of the tile before this one lie: its product has to be done
                     if (j > 0) ok = mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort);
-                    ok = ok && mbar_wait_warp(smem_u32(&s_bar.k_full[(j + 1) % kStages]), ((j + 1) / kStages) & 1u, &s_abort);
+                    ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 2) % kSlots]), ((2 * j + 2) / kSlots) & 1u, &s_abort);
                     if (!ok) break;
                     tc_fence_after_sync();
                     if (elect_one()) {
                         scores(j + 1);
                         umma_commit(smem_u32(&s_bar.s_full[(j + 1) & 1u]));
-                        umma_commit(smem_u32(&s_bar.k_empty[(j + 1) % kStages]));
+                        umma_commit(smem_u32(&s_bar.empty[(2 * j + 2) % kSlots]));
                     }
                     __syncwarp();
                 }
                 ok = mbar_wait_warp(smem_u32(&s_bar.p_full[j & 1u]), (j >> 1) & 1u, &s_abort);
-                ok = ok && mbar_wait_warp(smem_u32(&s_bar.v_full[j % kStages]), (j / kStages) & 1u, &s_abort);
-                if (ok && j > 0) ok = mbar_wait_warp(smem_u32(&s_bar.pv_free), (j - 1) & 1u, &s_abort);
+                ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
                     product(j);
                     umma_commit(smem_u32(&s_bar.pv_full));
-                    umma_commit(smem_u32(&s_bar.v_empty[j % kStages]));
+                    if (j + 1 == tiles) umma_commit(smem_u32(&s_bar.all_done));
+                    umma_commit(smem_u32(&s_bar.empty[(2 * j + 1) % kSlots]));
                 }
                 __syncwarp();
             }
@@ -658,7 +716,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                     const float f = s_part[k][r];
                     if (f != 0.f) { v[0] = fmaf(x[k].x, f, v[0]); v[1] = fmaf(x[k].y, f, v[1]); v[2] = fmaf(x[k].z, f, v[2]); v[3] = fmaf(x[k].w, f, v[3]); }
                 }
-            write_row(r, c * 4, v, 1.f);
+            write_row(r, c * 4, v);
         }
         cluster_sync();   // what the others read is read
     }
