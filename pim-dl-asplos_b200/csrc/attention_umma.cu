@@ -28,7 +28,7 @@
 namespace lutamm {
 namespace {
 
-constexpr int kRows = 128, kKeys = 64, kThreads = 384;
+constexpr int kRows = 128, kKeys = 64;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
 constexpr uint32_t kMostShares = 8;
 // Tensor memory adds up towards zero: a sum of n products is short by about 3e-8 of its size a tile, 1.3e-5 at 16000 keys.  fp32's output is
@@ -36,21 +36,30 @@ constexpr uint32_t kMostShares = 8;
 constexpr uint32_t kChunk = 8;
 constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
-template <typename T, int DP>
+// DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
+template <typename T, int DP, int RT>
 struct Form {
     static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
     static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
-    static constexpr int kSlots = 6;                                 // of the ring that keys and values take by turns
-    static constexpr int kAhead = 3;                                 // tiles on their way
-    static constexpr int kSmem = kSlots * kTile + 1024;
+    static constexpr int kSlots = RT == 2 ? 8 : 6;                   // of the ring that keys and values take by turns
+    static constexpr int kAhead = RT == 2 ? 2 : 3;                   // tiles that a warpgroup has on their way
+    static constexpr int kOut = RT * kRows * DP * 4;                 // bytes of the output, in fp32
+    // Where the output is put together, and the queries are turned before: behind the ring; with one tile of rows in the ring itself, which is idle
+    // then (the queries' place from the fifth slot on).
+    static constexpr int kOutAt = RT == 2 ? kSlots * kTile : 0, kQueryAt = RT == 2 ? kOutAt : 4 * kTile;
+    static constexpr int kSmem = kSlots * kTile + (RT == 2 ? kOut : 0) + 1024;
+    static_assert(kOutAt + kOut <= kSmem - 1024 && kQueryAt + RT * kRows * DP * (int)sizeof(T) <= kSmem - 1024);
     static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles in registers: see kChunk
-    static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;
-    static constexpr int kColumns = kUsed <= 256 ? 256 : 512;
-    static constexpr int kCtas = DP <= 64 ? 2 : 1;                   // per SM
-    // Registers a thread by role.  Their sum is what the three warpgroups are launched with, 3 x 80 or 3 x 168.
-    static constexpr int kRowRegs = DP <= 64 ? 152 : 232, kLoadRegs = DP <= 64 ? 64 : 136, kIssueRegs = DP <= 64 ? 24 : 136;
+    static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;   // columns of a tile of rows
+    static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
+    static_assert(RT == 1 || kUsed <= 256);
+    static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
+    // Warpgroups: RT that own rows, RT that load, one that issues.  Registers a thread of each; their sum is what the warpgroups are launched with.
+    static constexpr int kThreads = (2 * RT + 1) * 128;
+    static constexpr int kLaunchRegs = RT == 2 ? 96 : DP <= 64 ? 80 : 168;
+    static constexpr int kRowRegs = RT == 2 ? 160 : DP <= 64 ? 152 : 232, kLoadRegs = DP <= 64 ? 64 : 136, kIssueRegs = RT == 2 ? 32 : DP <= 64 ? 24 : 136;
+    static_assert(RT * (kRowRegs + kLoadRegs) + kIssueRegs == (2 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
 };
-static_assert(152 + 64 + 24 == 3 * 80 && 232 + 136 + 136 == 3 * 168);
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -74,7 +83,7 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t smem_addr) {
     return umma_desc_k_sw128(smem_addr) | (static_cast<uint64_t>(1024u >> 4) << 16);
 }
 
-__device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }   // the loading warps
+__device__ __forceinline__ void sync_128(uint32_t id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
 // The power of two that takes a largest value to 8 .. 16, up to 2^108 (results below 1e-32 have fewer bits); 0 for 0.
 __device__ __forceinline__ int exponent_for(uint32_t top_bits) { return top_bits == 0 ? 0 : min(108, 130 - (int)(top_bits >> 23)); }
@@ -123,63 +132,87 @@ __device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint3
 // ones below bit n
 __device__ __forceinline__ uint64_t below(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
-struct Bars {
-    uint64_t full[6], empty[6], s_full[2], p_full[2], pv_full, all_done, q_full;
+struct RowBars {   // of a tile of rows
+    uint64_t s_full[2], p_full[2], pv_full, all_done, q_full;
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, Form<T, DP>::kCtas)
+// Which of the CTA's tiles of keys a tile of rows sees any of: the sinks', and from .. to - 1.
+struct Seen {
+    uint32_t sink_tiles, from, to;
+    __device__ __forceinline__ bool operator()(uint32_t t) const { return t < sink_tiles || (t >= from && t < to); }
+    // the last one of t0 .. t1 - 1 that is seen, if any is
+    __device__ __forceinline__ uint32_t last(uint32_t t0, uint32_t t1) const {
+        return min(to, t1) > max(from, t0) ? min(to, t1) - 1 : min(sink_tiles, t1) > t0 ? min(sink_tiles, t1) - 1 : 0xFFFFFFFFu;
+    }
+};
+
+template <typename T, int DP, int RT>
+__global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tiles, uint32_t* dev_err) {
-    using F = Form<T, DP>;
-    constexpr uint32_t kSlots = F::kSlots;
+    using F = Form<T, DP, RT>;
+    constexpr uint32_t kSlots = F::kSlots, kThreads = F::kThreads;
     extern __shared__ unsigned char s_raw[];
-    __shared__ __align__(8) Bars s_bar;
-    __shared__ uint32_t s_tmem, s_abort, s_top[3][4];
-    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most three tiles ahead of who reads these
-    __shared__ float s_m[kRows], s_l[kRows], s_part[kMostShares][kRows];
+    __shared__ __align__(8) uint64_t s_full_bar[kSlots], s_empty_bar[kSlots];
+    __shared__ __align__(8) RowBars s_row[RT];
+    __shared__ uint32_t s_tmem, s_abort, s_top[RT][3][4];
+    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most four tiles ahead of who reads these
+    __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_part[kMostShares][RT * kRows];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
 
     const uint32_t shares = cluster_size_x(), share = cluster_rank();
     uint32_t item = blockIdx.x / shares;
-    const uint32_t rt = item % row_tiles;
+    const uint32_t ct = item % row_tiles;
     item /= row_tiles;
     const uint32_t g = item % a.kv_heads, b = item / a.kv_heads;
     const uint32_t per_head = a.heads / a.kv_heads;
-    const uint32_t rows = a.queries * per_head, r0 = rt * kRows;   // below 2^31
-    const uint32_t n_rows = min(rows - r0, (uint32_t)kRows);
+    const uint32_t rows = a.queries * per_head, r0 = ct * (RT * kRows);   // below 2^31
+    const uint32_t n_rows = min(rows - r0, (uint32_t)(RT * kRows));
     const int32_t length = key_count(a, b);
     const int64_t first = a.first ? __ldg(a.first + b) : 0;
-    const int64_t p0 = first + r0 / per_head, p1 = first + (r0 + n_rows - 1) / per_head;
-    KeySpan span = key_span(a, p0, p1, length);
+    const uint32_t dim = a.head_dim;
+    KeySpan span = key_span(a, first + r0 / per_head, first + (r0 + n_rows - 1) / per_head, length);
     if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;   // the window begins in the sinks' last tile
     const uint32_t sink_tiles = (uint32_t)(span.sinks + kKeys - 1) / kKeys;
-    const uint32_t all_tiles = sink_tiles + (uint32_t)(((int64_t)span.hi - span.lo + kKeys - 1) / kKeys);
-    const uint32_t t0 = (uint32_t)((uint64_t)all_tiles * share / shares), tiles = (uint32_t)((uint64_t)all_tiles * (share + 1) / shares) - t0;
-    auto tile_keys = [&](uint32_t j, int32_t& k0, int32_t& end) {
-        const uint32_t t = t0 + j;
+    const uint32_t all_tiles = sink_tiles + (uint32_t)(span.hi - span.lo + kKeys - 1) / kKeys;
+    const uint32_t t0 = (uint32_t)((uint64_t)all_tiles * share / shares), t1 = (uint32_t)((uint64_t)all_tiles * (share + 1) / shares), tiles = t1 - t0;
+    auto tile_keys = [&](uint32_t t, int32_t& k0, int32_t& end) {
         const bool sink = t < sink_tiles;
         k0 = sink ? (int32_t)(t * kKeys) : span.lo + (int32_t)((t - sink_tiles) * kKeys);
         end = sink ? span.sinks : span.hi;
     };
+    auto rows_see = [&](uint32_t rt) -> Seen {   // tile rt of the rows
+        Seen v{0, 0, 0};
+        if (rt * kRows >= n_rows) return v;
+        if (RT == 1) return Seen{sink_tiles, sink_tiles, all_tiles};
+        const KeySpan own = key_span(a, first + (r0 + rt * kRows) / per_head, first + (r0 + min((rt + 1) * kRows, n_rows) - 1) / per_head, length);
+        const int32_t lo = max(own.lo, span.lo), hi = min(own.hi, span.hi);
+        if (own.hi <= own.lo && own.sinks == 0) return v;
+        v.sink_tiles = sink_tiles;
+        v.from = sink_tiles + (own.sinks > 0 && span.lo == 0 ? 0u : (uint32_t)(lo - span.lo) / kKeys);   // sinks within the window's tiles
+        v.to = hi > span.lo ? sink_tiles + (uint32_t)(hi - span.lo + kKeys - 1) / kKeys : sink_tiles;
+        return v;
+    };
 
-    if (warp == 8) {
+    if (warp == 8 * RT) {
         tmem_alloc(smem_u32(&s_tmem), F::kColumns);
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < F::kSlots; ++i) {
-            mbar_init(smem_u32(&s_bar.full[i]), 4);
-            mbar_init(smem_u32(&s_bar.empty[i]), 1);
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            mbar_init(smem_u32(&s_full_bar[i]), 4);
+            mbar_init(smem_u32(&s_empty_bar[i]), RT);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&s_bar.s_full[i]), 1);
-            mbar_init(smem_u32(&s_bar.p_full[i]), 4);
+        for (int r = 0; r < RT; ++r) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(smem_u32(&s_row[r].s_full[i]), 1);
+                mbar_init(smem_u32(&s_row[r].p_full[i]), 4);
+            }
+            mbar_init(smem_u32(&s_row[r].pv_full), 1);
+            mbar_init(smem_u32(&s_row[r].all_done), 1);
+            mbar_init(smem_u32(&s_row[r].q_full), 4);
         }
-        mbar_init(smem_u32(&s_bar.pv_full), 1);
-        mbar_init(smem_u32(&s_bar.all_done), 1);
-        mbar_init(smem_u32(&s_bar.q_full), 4);
         fence_barrier_init();
         s_abort = 0;
     }
@@ -187,94 +220,95 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = s_tmem;
-    const uint32_t dim = a.head_dim;
-
-    auto write_row = [&](uint32_t r, uint32_t c, const float (&w)[4]) {   // four elements from column c
+    float4* s_o = reinterpret_cast<float4*>(smem + F::kOutAt);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
+    auto out_place = [](uint32_t r, uint32_t c4) -> uint32_t { return r * (DP / 4) + (c4 ^ (r & (DP / 4 - 1))); };
+    auto write_row = [&](uint32_t r, uint32_t c, const float4& v) {   // four elements from column c
         const uint32_t row = r0 + r, qi = row / per_head, head = g * per_head + (row - qi * per_head);
         T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
-        if constexpr (sizeof(T) == 4) store_elems<T, 4>(p, w);
-        else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(w[0], w[1], static_cast<T*>(nullptr)), pack2(w[2], w[3], static_cast<T*>(nullptr)));
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = v;
+        else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
     };
-    float4* s_o = reinterpret_cast<float4*>(smem);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
 
-    if (warp < 4) {
+    if (warp < 4 * RT) {
         // ---------------------------------------------------------------- a row a thread
         regs_up<F::kRowRegs>();
-        const uint32_t lanes = (warp * 32u) << 16;
+        const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16, warp_row = warp * 32u;
+        RowBars& bar = s_row[rt];
+        const uint32_t my_tmem = tmem + rt * 256u + lanes;
         const bool real = tid < n_rows;
-        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = row / per_head, head = g * per_head + (row - qi * per_head);
+        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = row / per_head;
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
-        float factor = fabsf(a.scale), q_up = 1.f;   // of this row's scores; of its query
+        const Seen sees = rows_see(rt);
+        float factor = fabsf(a.scale);   // of this row's scores
         {
-            const T* qp = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)qi * a.q_token + (int64_t)head * a.q_head;
-            const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+            // Queries: row by row through shared memory, 32 rows a warp, so that loads are of whole lines; then a thread has its own row.
+            constexpr int E = kPer16<T>, kPer = DP / E;   // pieces of 16 bytes a row
+            uint4* stage = reinterpret_cast<uint4*>(smem + F::kQueryAt + warp_row * (RT == 2 ? DP * 4 : DP * (int)sizeof(T)));   // where the warp's output goes
+            uint4 raw[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const uint32_t n = i * 32 + lane, r = n / kPer, c = n % kPer, q_row = r0 + warp_row + r;
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (warp_row + r < n_rows && c * E < dim) {
+                    const uint32_t i_q = q_row / per_head, head = g * per_head + (q_row - i_q * per_head);
+                    raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)i_q * a.q_token + (int64_t)head * a.q_head) + c);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const uint32_t n = i * 32 + lane, r = n / kPer, c = n % kPer;
+                stage[r * kPer + (c ^ (r & (kPer - 1)))] = raw[i];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) raw[i] = stage[lane * kPer + (i ^ (lane & (kPer - 1)))];
+            float up = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
             if (a.scale == 0.f) factor = 1.f;
-            constexpr int E = kPer16<T>;
+            if constexpr (F::kParts == 2) {   // the power of two is the row's
+                uint32_t top = 0;
+                auto look = [&](uint32_t bits) {
+                    bits &= 0x7FFFFFFFu;
+                    if (bits < 0x7F800000u) top = max(top, bits);
+                };
 #pragma unroll
-            for (int panel = 0; panel < F::kPanels; ++panel) {   // (fp32: the power of two is the row's, so its largest value comes first)
-                uint4 raw[64 / E];
+                for (int i = 0; i < kPer; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
+                const int e = exponent_for(top);
+                up *= power2(e);
+                factor *= power2(-e);
+            }
 #pragma unroll
-                for (int i = 0; i < 64 / E; ++i) {
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (real && panel * 64u + i * E < dim) raw[i] = __ldg(reinterpret_cast<const uint4*>(qp + panel * 64 + i * E));
-                }
+            for (int part = 0; part < kPer / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
                 if constexpr (F::kParts == 2) {
-                    if (panel == 0) {
-                        uint32_t top = 0;
-                        auto look = [&](uint32_t bits) {
-                            bits &= 0x7FFFFFFFu;
-                            if (bits < 0x7F800000u) top = max(top, bits);
-                        };
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                        for (int i = 0; i < 64 / E; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
-                        if constexpr (F::kPanels == 2) {
-#pragma unroll 4
-                            for (uint32_t c = 64; c < dim; c += E) {
-                                if (real) {
-                                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(qp + c));
-                                    look(w.x); look(w.y); look(w.z); look(w.w);
-                                }
-                            }
-                        }
-                        const int e = exponent_for(top);
-                        q_up = power2(e);
-                        factor *= power2(-e);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 w = raw[part * 4 + i];
+                        split2_any(__uint_as_float(w.x) * up, __uint_as_float(w.y) * up, hi[2 * i], lo[2 * i]);
+                        split2_any(__uint_as_float(w.z) * up, __uint_as_float(w.w) * up, hi[2 * i + 1], lo[2 * i + 1]);
                     }
-                }
-                const float up = sign * q_up;
+                    tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
+                    tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, lo);
+                } else {
+                    uint32_t w[16];
 #pragma unroll
-                for (int part = 0; part < 64 / E / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
-                    if constexpr (F::kParts == 2) {
-                        uint32_t hi[8], lo[8];
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t u[4] = {raw[part * 4 + i].x, raw[part * 4 + i].y, raw[part * 4 + i].z, raw[part * 4 + i].w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint4 w = raw[part * 4 + i];
-                            split2_any(__uint_as_float(w.x) * up, __uint_as_float(w.y) * up, hi[2 * i], lo[2 * i]);
-                            split2_any(__uint_as_float(w.z) * up, __uint_as_float(w.w) * up, hi[2 * i + 1], lo[2 * i + 1]);
-                        }
-                        tmem_st_32x32b_x8(tmem + lanes + F::kQuery + panel * 32 + part * 8, hi);
-                        tmem_st_32x32b_x8(tmem + lanes + F::kQuery + DP / 2 + panel * 32 + part * 8, lo);
-                    } else {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t u[4] = {raw[part * 4 + i].x, raw[part * 4 + i].y, raw[part * 4 + i].z, raw[part * 4 + i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w[4 * i + k] = a.scale > 0.f ? u[k] : a.scale < 0.f ? u[k] ^ 0x80008000u : 0u;
-                        }
-                        tmem_st_32x32b_x16(tmem + lanes + F::kQuery + panel * 32 + part * 16, w);
+                        for (int k = 0; k < 4; ++k) w[4 * i + k] = a.scale > 0.f ? u[k] : a.scale < 0.f ? u[k] ^ 0x80008000u : 0u;
                     }
+                    tmem_st_32x32b_x16(my_tmem + F::kQuery + part * 16, w);
                 }
             }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_bar.q_full));
+            if (lane == 0) mbar_arrive(smem_u32(&bar.q_full));
         }
         // All rows see all of a tile that lies between these.
-        const int32_t common_hi = key_bounds(a, p0, length).hi, common_lo = key_bounds(a, p1, length).lo;
+        const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
+        const int32_t common_hi = key_bounds(a, first + (r0 + r_first) / per_head, length).hi, common_lo = key_bounds(a, first + (r0 + max(r_last, r_first)) / per_head, length).lo;
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
-        const uint32_t out_at = tmem + lanes + F::kProduct;
+        const uint32_t out_at = my_tmem + F::kProduct;
         // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is o, against m_o
         uint64_t o[F::kSums ? DP / 2 : 1];
         float m_o = -INFINITY;
@@ -299,15 +333,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             }
             m_o = m;
         };
+        uint32_t n = 0;   // tiles so far
         for (uint32_t j = 0; j < tiles; ++j) {
-            if (!mbar_wait_warp(smem_u32(&s_bar.s_full[j & 1u]), (j >> 1) & 1u, &s_abort)) break;
+            if (!sees(t0 + j)) continue;
+            if (!mbar_wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
-            const uint32_t at = tmem + lanes + F::kScores + (j & 1u) * kKeys;
-            bool begun = j > 0;   // whether tensor memory holds an output to go on with
+            const uint32_t at = my_tmem + F::kScores + (n & 1u) * kKeys;
+            bool begun = n > 0;   // whether tensor memory holds an output to go on with
             if constexpr (F::kSums) {
-                begun = j % kChunk != 0;
-                if (j > 0 && !begun) {
-                    if (!mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort)) break;
+                begun = n % kChunk != 0;
+                if (n > 0 && !begun) {
+                    if (!mbar_wait_warp(smem_u32(&bar.pv_full), (n - 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     add_chunk();
                 }
@@ -317,12 +353,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             if constexpr (F::kParts == 2) {
                 c *= power2(-s_exp_k[j % 8]);
                 // the values' power of two is known once they are in shared memory, which the keys' turn does not wait for
-                if (!mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
+                if (!mbar_wait_warp(smem_u32(&s_full_bar[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
                 e = s_exp_v[j % 8];
             }
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             int32_t k0, end;
-            tile_keys(j, k0, end);
+            tile_keys(t0 + j, k0, end);
             uint32_t seen0 = 0xFFFFFFFFu, seen1 = 0xFFFFFFFFu;
             const bool edge = !((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks));
             if (edge) {
@@ -364,7 +400,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 const float m_new = top > m + kSlack ? top : m;
                 const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
                 if (begun) {
-                    if (!mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort)) break;
+                    if (!mbar_wait_warp(smem_u32(&bar.pv_full), (n - 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     float f = shrink;
                     if constexpr (F::kParts == 2) {
@@ -444,18 +480,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_bar.p_full[j & 1u]));
+            if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
             const float2 sums = unpair(add2(sum[0], sum[1]));
             l = fmaf(sums.x + sums.y, back, l);
+            ++n;
         }
         // A barrier's wait tells a phase from the one before it alone, and here the last two products may be done or under way: a barrier of its own.
-        const bool done = tiles > 0 && mbar_wait_warp(smem_u32(&s_bar.all_done), 0, &s_abort);
+        const bool done = n > 0 && mbar_wait_warp(smem_u32(&bar.all_done), 0, &s_abort);
         tc_fence_after_sync();
         const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         auto put = [&](uint32_t col, float x0, float x1, float x2, float x3) {   // (a row that sees nothing may hold what others' values left)
-            const float x[4] = {norm == 0.f ? 0.f : x0 * norm, norm == 0.f ? 0.f : x1 * norm, norm == 0.f ? 0.f : x2 * norm, norm == 0.f ? 0.f : x3 * norm};
-            if (shares > 1) s_o[tid * (DP / 4) + ((col / 4) ^ (tid & (DP / 4 - 1)))] = make_float4(x[0], x[1], x[2], x[3]);   // all products are done: nothing reads the tiles
-            else if (real && col < dim) write_row(tid, col, x);
+            s_o[out_place(tid, col / 4)] = norm == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x0 * norm, x1 * norm, x2 * norm, x3 * norm);
         };
         if constexpr (F::kSums) {
             if (done) add_chunk();
@@ -465,27 +500,35 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 put(col, x.x, x.y, y.x, y.y);
             }
         } else {
-#pragma unroll 1
-            for (uint32_t col = 0; col < DP; col += 16) {
-                if (col >= dim) break;
-                uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = 0;
+            for (int col = 0; col < DP; col += 32) {
+                uint32_t v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0;
                 if (done) {
-                    tmem_ld_32x32b_x16(out_at + col, v);
+                    tmem_ld_32x32b_x32(out_at + col, v);
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
+                for (int i = 0; i < 32; i += 4)
                     put(col + i, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
             }
         }
-        s_m[tid] = m;
-        s_l[tid] = l;
-    } else if (warp < 8) {
+        if (shares > 1) {
+            s_m[tid] = m;
+            s_l[tid] = l;
+        } else {   // the warp's rows, whole lines at a time
+            __syncwarp();
+            const uint32_t per_row = dim / 4, mine_rows = n_rows > warp_row ? min(32u, n_rows - warp_row) : 0u;
+            for (uint32_t i = lane; i < mine_rows * per_row; i += 32) {
+                const uint32_t r = i / per_row, c = i - r * per_row;
+                write_row(warp_row + r, c * 4, s_o[out_place(warp_row + r, c)]);
+            }
+        }
+    } else if (warp < 8 * RT) {
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
-        const uint32_t t = tid - 128;
+        const uint32_t t = tid & 127u, wg = warp / 4 - RT;   // with two warpgroups one loads keys, one values
         constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements: of one column, kStepRows rows apart
         constexpr int kPerRow = DP / 8, kStepRows = 128 / kPerRow;
         const uint32_t my_row = t / kPerRow, my_col = t % kPerRow;
@@ -496,7 +539,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         // where this thread's first group lies in a tile; the rows of its others differ by multiples of eight, which leaves the swizzle as it is
         const uint32_t place = (my_col / 8) * kPanel + my_row * 128u + (((my_col & 7u) ^ (my_row & 7u)) << 4);
         constexpr uint32_t kPlaceStep = kStepRows * 128;
-        const uint32_t jobs = 2 * tiles;   // keys of a tile, values of a tile, ...
+        // Jobs are keys of a tile, values of a tile, and so on; this warpgroup's are every RT-th from wg on.
+        const uint32_t jobs = 2 * tiles;
         // A job's source: this thread's first group, the step between its groups and how many of the groups hold keys.
         struct Source {
             const T* p;
@@ -505,7 +549,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         };
         auto source = [&](uint32_t job) -> Source {
             int32_t k0, end;
-            tile_keys(job / 2, k0, end);
+            tile_keys(t0 + job / 2, k0, end);
             const int32_t rows_left = end - k0 - (int32_t)my_row;
             Source s;
             s.n = !in_dim || rows_left <= 0 ? 0 : min(kPerThread, (rows_left + kStepRows - 1) / kStepRows);
@@ -517,7 +561,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
         // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
         auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
-            if (job >= kSlots) mbar_wait_warp(smem_u32(&s_bar.empty[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
+            if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
+            else if (RT == 1 && job >= 4) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
             const Source from = source(job);
             const uint32_t at = smem_at + slot(job);
 #pragma unroll
@@ -534,22 +579,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         auto publish = [&](uint32_t job) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_bar.full[job % kSlots]));
+            if (lane == 0) mbar_arrive(smem_u32(&s_full_bar[job % kSlots]));
         };
         // The largest of all loading threads' bits, by turns in three places: a warp is at most one tile ahead of another.
         auto tile_top = [&](uint32_t top, uint32_t turn) -> uint32_t {
             top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) s_top[turn][warp - 4] = top;
-            sync_128();
-            return max(max(s_top[turn][0], s_top[turn][1]), max(s_top[turn][2], s_top[turn][3]));
+            if (lane == 0) s_top[wg][turn][warp & 3u] = top;
+            sync_128(1 + wg);
+            return max(max(s_top[wg][turn][0], s_top[wg][turn][1]), max(s_top[wg][turn][2], s_top[wg][turn][3]));
         };
         int exp_k = 0, exp_v = 0;
-        for (uint32_t job = 0; job < F::kAhead; ++job) {
-            if (job < jobs) copy(job);
+        for (uint32_t i = 0; i < F::kAhead; ++i) {
+            if (wg + i * RT < jobs) copy(wg + i * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        for (uint32_t job = 0; job < jobs; ++job) {
-            if (job + F::kAhead < jobs) copy(job + F::kAhead);
+        for (uint32_t job = wg; job < jobs; job += RT) {
+            if (job + F::kAhead * RT < jobs) copy(job + F::kAhead * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(F::kAhead) : "memory");
             if constexpr (F::kParts == 2) {   // in place, from what this thread has copied itself
@@ -564,7 +609,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(buf[i][e]) & 0x7FFFFFFFu);
                 }
-                top = tile_top(top, job & 1u);   // behind it everybody has read
+                top = tile_top(top, job / RT & 1u);   // behind it everybody has read
                 // 0, or 2^-2 .. 2^15 under the power of two in use, or the tile gets one of its own.
                 int& e_now = job & 1u ? exp_v : exp_k;
                 const int reach = (int)(top >> 23) - 127 + e_now;
@@ -604,17 +649,20 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-        // ---------------------------------------------------------------- the tensor core's instructions
+        // ---------------------------------------------------------------- the tensor core's instructions, a warp for each tile of rows
         regs_down<F::kIssueRegs>();
-        if (warp == 8 && tiles > 0) {
-            const uint32_t k_steps = (dim + 15) / 16;
-            auto scores = [&](uint32_t j) {   // S = Q K^T, the small products first
-                const uint32_t d = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + 2 * j % kSlots * F::kTile;
+        const uint32_t rt = warp - 8 * RT;
+        if (rt < RT) {
+            RowBars& bar = s_row[rt];
+            const Seen sees = rows_see(rt);
+            const uint32_t my_tmem = tmem + rt * 256u, k_steps = (dim + 15) / 16;
+            auto scores = [&](uint32_t j, uint32_t n) {   // S = Q K^T, the small products first
+                const uint32_t d = my_tmem + F::kScores + (n & 1u) * kKeys, at = smem_at + 2 * j % kSlots * F::kTile;
                 const uint32_t idesc = idesc_f16<T>(kKeys);
                 uint32_t more = 0;
 #pragma unroll
                 for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
-                    const uint32_t qa = tmem + F::kQuery + (term == 1 ? DP / 2 : 0);
+                    const uint32_t qa = my_tmem + F::kQuery + (term == 1 ? DP / 2 : 0);
                     const uint32_t kb = at + (term == 0 ? F::kPanels * kPanel : 0);
                     for (uint32_t s = 0; s < k_steps; ++s) {
                         umma_f16_ts(d, qa + s * 8, umma_desc_k_sw128(kb + (s / 4) * kPanel + (s % 4) * 32), idesc, more);
@@ -622,60 +670,66 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                     }
                 }
             };
-            auto product = [&](uint32_t j) {
-                const uint32_t p = tmem + F::kScores + (j & 1u) * kKeys, at = smem_at + (2 * j + 1) % kSlots * F::kTile;
+            auto product = [&](uint32_t j, uint32_t n) {
+                const uint32_t p = my_tmem + F::kScores + (n & 1u) * kKeys, at = smem_at + (2 * j + 1) % kSlots * F::kTile;
 #pragma unroll
                 for (int panel = 0; panel < F::kPanels; ++panel) {
-                    const uint32_t left = dim - panel * 64u, n = left >= 64 ? 64 : (left + 15) / 16 * 16;
-                    const uint32_t idesc = idesc_f16<T>(n) | kIdescColumnMajorB;
-                    uint32_t more = F::kSums ? j % kChunk != 0 : j > 0;
+                    const uint32_t left = dim - panel * 64u, cols = left >= 64 ? 64 : (left + 15) / 16 * 16;
+                    const uint32_t idesc = idesc_f16<T>(cols) | kIdescColumnMajorB;
+                    uint32_t more = F::kSums ? n % kChunk != 0 : n > 0;
 #pragma unroll
                     for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
                         const uint32_t pa = p + (term == 1 ? 16 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
 #pragma unroll
                         for (uint32_t s = 0; s < 4; ++s) {
-                            umma_f16_ts(tmem + F::kProduct + panel * 64, pa + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), desc_rows(vb + s * 2048), idesc, more);
+                            umma_f16_ts(my_tmem + F::kProduct + panel * 64, pa + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), desc_rows(vb + s * 2048), idesc, more);
                             more = 1;
                         }
                     }
                 }
             };
-            bool ok = mbar_wait_warp(smem_u32(&s_bar.q_full), 0, &s_abort);
-            ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[0]), 0, &s_abort);
-            if (ok) {
+            auto wait_full = [&](uint32_t job) { return mbar_wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
+            uint32_t n_s = 0, n_p = 0;   // scores and products so far, of the tiles that these rows see
+            auto issue_scores = [&](uint32_t j) -> bool {
+                // they go where the weights of the last tile but one lie: its product has to be done
+                if (n_s > 1 && !mbar_wait_warp(smem_u32(&bar.pv_full), (n_s - 2) & 1u, &s_abort)) return false;
+                if (!wait_full(2 * j)) return false;
                 tc_fence_after_sync();
                 if (elect_one()) {
-                    scores(0);
-                    umma_commit(smem_u32(&s_bar.s_full[0]));
-                    umma_commit(smem_u32(&s_bar.empty[0]));
+                    scores(j, n_s);
+                    umma_commit(smem_u32(&bar.s_full[n_s & 1u]));
+                    umma_commit(smem_u32(&s_empty_bar[2 * j % kSlots]));
                 }
                 __syncwarp();
-            }
+                ++n_s;
+                return true;
+            };
+            const uint32_t last = sees.last(t0, t1);
+            bool ok = mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort), ahead = false;
             for (uint32_t j = 0; ok && j < tiles; ++j) {
-                if (j + 1 < tiles) {
-                    // the next tile's scores go where the weights of the tile before this one lie: its product has to be done
-                    if (j > 0) ok = mbar_wait_warp(smem_u32(&s_bar.pv_full), (j - 1) & 1u, &s_abort);
-                    ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 2) % kSlots]), ((2 * j + 2) / kSlots) & 1u, &s_abort);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    if (elect_one()) {
-                        scores(j + 1);
-                        umma_commit(smem_u32(&s_bar.s_full[(j + 1) & 1u]));
-                        umma_commit(smem_u32(&s_bar.empty[(2 * j + 2) % kSlots]));
+                if (!sees(t0 + j)) {   // handed back unread
+                    ok = wait_full(2 * j) && wait_full(2 * j + 1);
+                    if (ok && lane == 0) {
+                        mbar_arrive(smem_u32(&s_empty_bar[2 * j % kSlots]));
+                        mbar_arrive(smem_u32(&s_empty_bar[(2 * j + 1) % kSlots]));
                     }
-                    __syncwarp();
+                    continue;
                 }
-                ok = mbar_wait_warp(smem_u32(&s_bar.p_full[j & 1u]), (j >> 1) & 1u, &s_abort);
-                ok = ok && mbar_wait_warp(smem_u32(&s_bar.full[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort);
+                if (!ahead) ok = issue_scores(j);
+                ahead = j + 1 < tiles && sees(t0 + j + 1);
+                if (ok && ahead) ok = issue_scores(j + 1);   // while this tile's weights are formed
+                ok = ok && mbar_wait_warp(smem_u32(&bar.p_full[n_p & 1u]), (n_p >> 1) & 1u, &s_abort);
+                ok = ok && wait_full(2 * j + 1);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
-                    product(j);
-                    umma_commit(smem_u32(&s_bar.pv_full));
-                    if (j + 1 == tiles) umma_commit(smem_u32(&s_bar.all_done));
-                    umma_commit(smem_u32(&s_bar.empty[(2 * j + 1) % kSlots]));
+                    product(j, n_p);
+                    umma_commit(smem_u32(&bar.pv_full));
+                    if (t0 + j == last) umma_commit(smem_u32(&bar.all_done));
+                    umma_commit(smem_u32(&s_empty_bar[(2 * j + 1) % kSlots]));
                 }
                 __syncwarp();
+                ++n_p;
             }
         }
     }
@@ -703,10 +757,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         __syncthreads();
         const uint32_t per_row = dim / 4;
         for (uint32_t i = share * kThreads + tid; i < n_rows * per_row; i += shares * kThreads) {
-            const uint32_t r = i / per_row, c = i - r * per_row;
-            const uint32_t at_o = smem_u32(&s_o[r * (DP / 4) + (c ^ (r & (DP / 4 - 1)))]);
-            float4 x[kMostShares];
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t r = i / per_row, c = i - r * per_row, at_o = smem_u32(&s_o[out_place(r, c)]);
+            float4 x[kMostShares], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (uint32_t k = 0; k < kMostShares; ++k)
                 if (k < shares) x[k] = load_shared_cluster4(map_to_rank(at_o, k));
@@ -714,7 +766,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             for (uint32_t k = 0; k < kMostShares; ++k)
                 if (k < shares) {
                     const float f = s_part[k][r];
-                    if (f != 0.f) { v[0] = fmaf(x[k].x, f, v[0]); v[1] = fmaf(x[k].y, f, v[1]); v[2] = fmaf(x[k].z, f, v[2]); v[3] = fmaf(x[k].w, f, v[3]); }
+                    if (f != 0.f) { v.x = fmaf(x[k].x, f, v.x); v.y = fmaf(x[k].y, f, v.y); v.z = fmaf(x[k].z, f, v.z); v.w = fmaf(x[k].w, f, v.w); }
                 }
             write_row(r, c * 4, v);
         }
@@ -723,31 +775,31 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == 8 && s_abort) {   // what is in flight gets time to end before its columns are handed back
+    if (warp == 8 * RT && s_abort) {   // what is in flight gets time to end before its columns are handed back
         const long long from = clock64();
         while (clock64() - from < 200000) {}
         if (lane == 0) report_error(dev_err, 7);
     }
-    if (warp == 8) tmem_dealloc(tmem, F::kColumns);
+    if (warp == 8 * RT) tmem_dealloc(tmem, F::kColumns);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int RT>
 cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
-    using F = Form<T, DP>;
+    using F = Form<T, DP, RT>;
     static SmemOptIn memo;
-    cudaError_t e = allow_smem(memo, attention_umma_kernel<T, DP>, F::kSmem);
+    cudaError_t e = allow_smem(memo, attention_umma_kernel<T, DP, RT>, F::kSmem);
     if (e != cudaSuccess) return e;
-    const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads), tiles = (rows + kRows - 1) / kRows;
+    const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads), tiles = (rows + RT * kRows - 1) / (RT * kRows);
     const uint64_t items = (uint64_t)a.batch * a.kv_heads * tiles;
     // Keys that a tile of rows sees at most.
     uint64_t keys = a.keys;
-    if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
+    if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + RT * kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
     uint32_t shares = 1;
     while (shares < kMostShares && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kKeys) shares *= 2;
     if (rows > 0x7FFFFFFFull || items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((uint32_t)(items * shares));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(F::kThreads);
     cfg.dynamicSmemBytes = F::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -757,12 +809,19 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP>, a, (uint32_t)tiles, dev_err);
+    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP, RT>, a, (uint32_t)tiles, dev_err);
 }
 
 template <typename T>
 cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
-    return a.head_dim <= 64 ? run<T, 64>(a, sm_count, dev_err, s) : run<T, 128>(a, sm_count, dev_err, s);
+    if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
+    const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads);
+    // fp32's keys and values are converted once for 256 rows (ViT's batch 148 us with 128, 116 with 256); 16-bit types, which are only copied, do
+    // better with two CTAs of 128 rows on an SM (8192 tokens in bf16 101 us, 116 with 256).
+    if constexpr (sizeof(T) == 4) {
+        if (rows > kRows) return run<T, 64, 2>(a, sm_count, dev_err, s);
+    }
+    return run<T, 64, 1>(a, sm_count, dev_err, s);
 }
 
 }  // namespace
