@@ -32,7 +32,25 @@ __device__ __forceinline__ void load_row(const T* p, bool vec, uint32_t c, uint3
     }
 }
 
-template <typename T, int LPK, int RB>
+template <typename T>
+__device__ __forceinline__ uint4 load_16(const T* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+template <typename T, int E>
+__device__ __forceinline__ void widen(const uint4& w, float (&v)[E]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(u[i]);
+        } else {
+            const float2 f = unpack2(u[i], static_cast<T*>(nullptr));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
+
+// VEC: all tensors start on 16 bytes throughout.
+template <typename T, int LPK, int RB, bool VEC>
 __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs a, uint32_t row_groups) {
     constexpr int E = kPer16<T>, kGroups = 32 / LPK, kStreams = kWarps * kGroups, kStep = LPK / RB;
     static_assert(RB <= LPK);
@@ -63,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs 
             const uint64_t row = r0 + r;
             const uint64_t i = row / per_head;
             const uint32_t h = g * per_head + (uint32_t)(row - i * per_head);
-            load_row<T, E>(static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)i * a.q_token + (int64_t)h * a.q_head, a.vec, c, a.head_dim, q[r]);
+            load_row<T, E>(static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)i * a.q_token + (int64_t)h * a.q_head, VEC, c, a.head_dim, q[r]);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) q[r][e] = 0.f;
@@ -82,6 +100,22 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs 
         for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
 
     const uint32_t stream = warp * kGroups + group;
+    // The next four keys and values are on their way while these are worked on, as raw bytes.
+    uint4 k_raw[kUnroll], v_raw[kUnroll];
+    auto key_at = [&](uint32_t t) -> uint32_t { return t < (uint32_t)span.sinks ? t : (uint32_t)span.lo + (t - (uint32_t)span.sinks); };
+    auto fetch = [&](uint32_t base) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t t = base + u * kStreams + stream;
+            k_raw[u] = v_raw[u] = make_uint4(0, 0, 0, 0);
+            if (t < t1 && c < a.head_dim) {
+                const int64_t key = key_at(t);
+                k_raw[u] = load_16(kp + key * a.k_token + c);
+                v_raw[u] = load_16(vp + key * a.v_token + c);
+            }
+        }
+    };
+    if (VEC && t0 < t1) fetch(t0);
     for (uint32_t base = t0; base < t1; base += kUnroll * kStreams) {   // (t1 - t0 and this stay below 2^31 + 2^9)
         float kf[kUnroll][E], vf[kUnroll][E], s[kUnroll];
         uint32_t key[kUnroll];
@@ -90,15 +124,19 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs 
         for (int u = 0; u < kUnroll; ++u) {
             const uint32_t t = base + u * kStreams + stream;
             in[u] = t < t1;
-            key[u] = in[u] ? (t < (uint32_t)span.sinks ? t : (uint32_t)span.lo + (t - (uint32_t)span.sinks)) : 0u;
-            if (in[u]) {
-                load_row<T, E>(kp + (int64_t)key[u] * a.k_token, a.vec, c, a.head_dim, kf[u]);
-                load_row<T, E>(vp + (int64_t)key[u] * a.v_token, a.vec, c, a.head_dim, vf[u]);
+            key[u] = in[u] ? key_at(t) : 0u;
+            if constexpr (VEC) {
+                widen<T, E>(k_raw[u], kf[u]);
+                widen<T, E>(v_raw[u], vf[u]);
+            } else if (in[u]) {
+                load_row<T, E>(kp + (int64_t)key[u] * a.k_token, false, c, a.head_dim, kf[u]);
+                load_row<T, E>(vp + (int64_t)key[u] * a.v_token, false, c, a.head_dim, vf[u]);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) kf[u][e] = vf[u][e] = 0.f;
             }
         }
+        if (VEC && base + kUnroll * kStreams < t1) fetch(base + kUnroll * kStreams);
         float top = m;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
@@ -233,8 +271,13 @@ cudaError_t run(const AttentionArgs& a, int sm_count, cudaStream_t s) {
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads), groups = (rows + RB - 1) / RB;
     const uint64_t items = (uint64_t)a.batch * a.kv_heads * groups;
     uint32_t shares = 1;
-    while (shares < 8 && items * shares < 4ull * sm_count && a.keys / (2 * shares) >= 64) shares *= 2;
+    while (shares < 16 && items * shares < 4ull * sm_count && a.keys / (2 * shares) >= 64) shares *= 2;
     if (items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    auto kernel = a.vec ? attention_rows_kernel<T, LPK, RB, true> : attention_rows_kernel<T, LPK, RB, false>;
+    if (shares > 8) {   // clusters of 16 are to be asked for
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((uint32_t)(items * shares));
     cfg.blockDim = dim3(kThreads);
@@ -246,7 +289,7 @@ cudaError_t run(const AttentionArgs& a, int sm_count, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_rows_kernel<T, LPK, RB>, a, (uint32_t)groups);
+    return cudaLaunchKernelEx(&cfg, kernel, a, (uint32_t)groups);
 }
 
 template <typename T, int LPK>
