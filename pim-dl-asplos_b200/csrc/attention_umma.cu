@@ -41,12 +41,12 @@ template <typename T, int DP, int RT>
 struct Form {
     static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
     static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
-    static constexpr int kSlots = RT == 2 ? 8 : 6;                   // of the ring that keys and values take by turns
-    static constexpr int kAhead = RT == 2 ? 2 : 3;                   // tiles that a warpgroup has on their way
+    static constexpr int kSlots = RT == 2 ? 8 : sizeof(T) == 4 ? 6 : 12;   // of the ring that keys and values take by turns
+    static constexpr int kAhead = RT == 2 ? 2 : sizeof(T) == 4 ? 3 : 8;    // tiles that a warpgroup has on their way
     static constexpr int kOut = RT * kRows * DP * 4;                 // bytes of the output, in fp32
     // Where the output is put together, and the queries are turned before: behind the ring; with one tile of rows in the ring itself, which is idle
-    // then (the queries' place from the fifth slot on).
-    static constexpr int kOutAt = RT == 2 ? kSlots * kTile : 0, kQueryAt = RT == 2 ? kOutAt : 4 * kTile;
+    // then (the queries' place is the last two slots).
+    static constexpr int kOutAt = RT == 2 ? kSlots * kTile : 0, kQueryAt = RT == 2 ? kOutAt : (kSlots - 2) * kTile;
     static constexpr int kSmem = kSlots * kTile + (RT == 2 ? kOut : 0) + 1024;
     static_assert(kOutAt + kOut <= kSmem - 1024 && kQueryAt + RT * kRows * DP * (int)sizeof(T) <= kSmem - 1024);
     static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles in registers: see kChunk
@@ -106,6 +106,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -173,7 +178,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     const int64_t first = a.first ? __ldg(a.first + b) : 0;
     const uint32_t dim = a.head_dim;
     KeySpan span = key_span(a, first + r0 / per_head, first + (r0 + n_rows - 1) / per_head, length);
-    if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;   // the window begins in the sinks' last tile
+    // Where the window begins in the sinks' last tile, the tiles run on from the first key; keys that no row sees are left out of them.
+    const int32_t gap_from = span.sinks, gap_to = span.lo;
+    if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;
     const uint32_t sink_tiles = (uint32_t)(span.sinks + kKeys - 1) / kKeys;
     const uint32_t all_tiles = sink_tiles + (uint32_t)(span.hi - span.lo + kKeys - 1) / kKeys;
     const uint32_t t0 = (uint32_t)((uint64_t)all_tiles * share / shares), t1 = (uint32_t)((uint64_t)all_tiles * (share + 1) / shares), tiles = t1 - t0;
@@ -546,6 +553,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             const T* p;
             int64_t step;
             int n;
+            int32_t key;
         };
         auto source = [&](uint32_t job) -> Source {
             int32_t k0, end;
@@ -556,18 +564,20 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             const int64_t key = (int64_t)k0 + my_row;
             s.p = job & 1u ? vp + key * a.v_token : kp + key * a.k_token;
             s.step = job & 1u ? v_step : k_step;
+            s.key = k0 + (int32_t)my_row;
             return s;
         };
         auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
         // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
         auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
             if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
-            else if (RT == 1 && job >= 4) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
+            else if (RT == 1 && job >= kSlots - 2) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
             const Source from = source(job);
             const uint32_t at = smem_at + slot(job);
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const bool in = i < from.n;
+                const int32_t key = from.key + i * kStepRows;
+                const bool in = i < from.n && (key < gap_from || key >= gap_to);
                 const T* p = in ? from.p + i * from.step : kp;
 #pragma unroll
                 for (int h = 0; h < F::kParts; ++h) {   // fp32: two pieces of 16 bytes, to where this thread alone reads them
@@ -600,49 +610,49 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             if constexpr (F::kParts == 2) {   // in place, from what this thread has copied itself
                 unsigned char* at = smem + slot(job);
                 float buf[kPerThread][8];
-                uint32_t top = 0;
+                float big = 0.f;   // (what is no number is passed over here, and is itself in both parts)
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
                     const float4 x = *reinterpret_cast<const float4*>(at + (i * 2) * 2048 + t * 16), y = *reinterpret_cast<const float4*>(at + (i * 2 + 1) * 2048 + t * 16);
                     buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
                     buf[i][4] = y.x; buf[i][5] = y.y; buf[i][6] = y.z; buf[i][7] = y.w;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(buf[i][e]) & 0x7FFFFFFFu);
+                    for (int e = 0; e < 8; e += 2) big = max3(big, fabsf(buf[i][e]), fabsf(buf[i][e + 1]));
                 }
-                top = tile_top(top, job / RT & 1u);   // behind it everybody has read
+                uint32_t top = tile_top(__float_as_uint(big), job / RT & 1u);   // behind it everybody has read
                 // 0, or 2^-2 .. 2^15 under the power of two in use, or the tile gets one of its own.
                 int& e_now = job & 1u ? exp_v : exp_k;
+                const bool infinite = top >= 0x7F800000u;
+                if (infinite) {   // the largest that is a number
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int i = 0; i < kPerThread; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
+                            if (bits < 0x7F800000u) most = max(most, bits);
+                        }
+                    top = tile_top(most, 2);
+                }
                 const int reach = (int)(top >> 23) - 127 + e_now;
-                if (top != 0 && (reach >= 15 || reach < -2)) {
-                    if (top >= 0x7F800000u) {   // the largest that is a number
-                        uint32_t big = 0;
-#pragma unroll
-                        for (int i = 0; i < kPerThread; ++i)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
-                                if (bits < 0x7F800000u) big = max(big, bits);
-                            }
-                        big = tile_top(big, 2);
-                        const int r = (int)(big >> 23) - 127 + e_now;
-                        if (big != 0 && (r >= 15 || r < -2)) e_now = exponent_for(big);
-                    } else {
-                        e_now = exponent_for(top);
-                    }
-                }
-                const float up = power2(e_now);
+                if (top != 0 && (reach >= 15 || reach < -2)) e_now = exponent_for(top);
+                const uint64_t up = pair(power2(e_now), power2(e_now));
                 unsigned char* to = at + place;
+                auto convert = [&](auto split) {
 #pragma unroll
-                for (int i = 0; i < kPerThread; ++i) {
-                    uint32_t hi[4], lo[4];
+                    for (int i = 0; i < kPerThread; ++i) {
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (top >= 0x7F800000u) split2_any(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
-                        else split2(buf[i][2 * e] * up, buf[i][2 * e + 1] * up, hi[e], lo[e]);
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 x = unpair(mul2(pair(buf[i][2 * e], buf[i][2 * e + 1]), up));
+                            split(x.x, x.y, hi[e], lo[e]);
+                        }
+                        *reinterpret_cast<uint4*>(to + i * kPlaceStep) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(to + i * kPlaceStep + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    *reinterpret_cast<uint4*>(to + i * kPlaceStep) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(to + i * kPlaceStep + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
+                };
+                if (infinite) convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2_any(x, y, hi, lo); });
+                else convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, hi, lo); });
                 if (t == 0) (job & 1u ? s_exp_v : s_exp_k)[job / 2 % 8] = e_now;
             }
             publish(job);

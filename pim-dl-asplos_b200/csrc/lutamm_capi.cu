@@ -1065,7 +1065,9 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
     const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
-    const cudaError_t e = rows <= 8 || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
+    // The tensor cores need many rows to be worth fp32's conversion (12 rows of 8 x 8192 keys, heads of 128: 695 us there, 568 here), and 16-bit types
+    // almost none (2 rows, heads of 64: 78 and 81 us; 8 rows 79 and 160).  What does not start on 16 bytes goes element by element here.
+    const cudaError_t e = rows <= (size == 4 ? 16 : 2) || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
                                     : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
     return dense_done(c, e, "attention", 1, flags);
 }
