@@ -151,9 +151,20 @@ struct Seen {
     }
 };
 
+// n / d for n below 2^31: the quotient's 32 bits above the binary point of n * mul / 2^(31 + shift).
+struct Divisor {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return d == 1 ? n : (uint32_t)(((uint64_t)n * mul) >> shift); }
+};
+Divisor divisor(uint32_t d) {
+    uint32_t bits = 0;
+    while ((1ull << bits) < d) ++bits;
+    return Divisor{d, (uint32_t)(d == 1 ? 0 : (1ull << (31 + bits)) / d + 1), 31 + bits};
+}
+
 template <typename T, int DP, int RT>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
-attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tiles, uint32_t* dev_err) {
+attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
     using F = Form<T, DP, RT>;
     constexpr uint32_t kSlots = F::kSlots, kThreads = F::kThreads;
     extern __shared__ unsigned char s_raw[];
@@ -167,17 +178,16 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
 
     const uint32_t shares = cluster_size_x(), share = cluster_rank();
-    uint32_t item = blockIdx.x / shares;
-    const uint32_t ct = item % row_tiles;
-    item /= row_tiles;
-    const uint32_t g = item % a.kv_heads, b = item / a.kv_heads;
-    const uint32_t per_head = a.heads / a.kv_heads;
-    const uint32_t rows = a.queries * per_head, r0 = ct * (RT * kRows);   // below 2^31
+    uint32_t item = shares == 1 ? blockIdx.x : blockIdx.x / shares;
+    const uint32_t ct = item - row_tiles(item) * row_tiles.d;
+    item = row_tiles(item);
+    const uint32_t b = kv_heads(item), g = item - b * kv_heads.d;
+    const uint32_t rows = a.queries * per_head.d, r0 = ct * (RT * kRows);   // below 2^31
     const uint32_t n_rows = min(rows - r0, (uint32_t)(RT * kRows));
     const int32_t length = key_count(a, b);
     const int64_t first = a.first ? __ldg(a.first + b) : 0;
     const uint32_t dim = a.head_dim;
-    KeySpan span = key_span(a, first + r0 / per_head, first + (r0 + n_rows - 1) / per_head, length);
+    KeySpan span = key_span(a, first + per_head(r0), first + per_head(r0 + n_rows - 1), length);
     // Where the window begins in the sinks' last tile, the tiles run on from the first key; keys that no row sees are left out of them.
     const int32_t gap_from = span.sinks, gap_to = span.lo;
     if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;
@@ -193,7 +203,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         Seen v{0, 0, 0};
         if (rt * kRows >= n_rows) return v;
         if (RT == 1) return Seen{sink_tiles, sink_tiles, all_tiles};
-        const KeySpan own = key_span(a, first + (r0 + rt * kRows) / per_head, first + (r0 + min((rt + 1) * kRows, n_rows) - 1) / per_head, length);
+        const KeySpan own = key_span(a, first + per_head(r0 + rt * kRows), first + per_head(r0 + min((rt + 1) * kRows, n_rows) - 1), length);
         const int32_t lo = max(own.lo, span.lo), hi = min(own.hi, span.hi);
         if (own.hi <= own.lo && own.sinks == 0) return v;
         v.sink_tiles = sink_tiles;
@@ -202,26 +212,97 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         return v;
     };
 
-    if (warp == 8 * RT) {
+    // ---- what loads keys and values: warpgroup wg of them (with two, one loads keys, one values)
+    const uint32_t t = tid & 127u, wg = warp / 4 - RT;
+    constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements: of one column, kStepRows rows apart
+    constexpr int kPerRow = DP / 8, kStepRows = 128 / kPerRow;
+    const uint32_t my_row = t / kPerRow, my_col = t % kPerRow;
+    const bool in_dim = my_col * 8 < dim;
+    const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head + (in_dim ? my_col * 8 : 0);
+    const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head + (in_dim ? my_col * 8 : 0);
+    const int64_t k_step = a.k_token * kStepRows, v_step = a.v_token * kStepRows;
+    // where this thread's first group lies in a tile; the rows of its others differ by multiples of eight, which leaves the swizzle as it is
+    const uint32_t place = (my_col / 8) * kPanel + my_row * 128u + (((my_col & 7u) ^ (my_row & 7u)) << 4);
+    constexpr uint32_t kPlaceStep = kStepRows * 128;
+    // Jobs are keys of a tile, values of a tile, and so on; this warpgroup's are every RT-th from wg on.
+    const uint32_t jobs = 2 * tiles;
+    // A job's source: this thread's first group, the step between its groups and how many of the groups hold keys.
+    struct Source {
+        const T* p;
+        int64_t step;
+        int n;
+        int32_t key;
+    };
+    auto source = [&](uint32_t job) -> Source {
+        int32_t k0, end;
+        tile_keys(t0 + job / 2, k0, end);
+        const int32_t rows_left = end - k0 - (int32_t)my_row;
+        Source s;
+        s.n = !in_dim || rows_left <= 0 ? 0 : min(kPerThread, (rows_left + kStepRows - 1) / kStepRows);
+        const int64_t key = (int64_t)k0 + my_row;
+        s.p = job & 1u ? vp + key * a.v_token : kp + key * a.k_token;
+        s.step = job & 1u ? v_step : k_step;
+        s.key = k0 + (int32_t)my_row;
+        return s;
+    };
+    auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
+    // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
+    auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
+        if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
+        else if (RT == 1 && job >= kSlots - 2) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
+        const Source from = source(job);
+        const uint32_t at = smem_at + slot(job);
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            const int32_t key = from.key + i * kStepRows;
+            const bool in = i < from.n && (key < gap_from || key >= gap_to);
+            const T* p = in ? from.p + i * from.step : kp;
+#pragma unroll
+            for (int h = 0; h < F::kParts; ++h) {   // fp32: two pieces of 16 bytes, to where this thread alone reads them
+                const uint32_t to = F::kParts == 2 ? at + (i * 2 + h) * 2048 + t * 16 : at + place + i * kPlaceStep;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? p + h * 4 : kp), "r"(in ? 16 : 0) : "memory");
+            }
+        }
+    };
+
+    // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
+    // lines; then a thread has its own row.
+    constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
+    const uint32_t warp_row = warp * 32u, q_stage = F::kQueryAt + warp_row * (RT == 2 ? DP * 4 : DP * (int)sizeof(T));   // (with two, where the warp's output goes)
+    if (warp < 4 * RT) {
+        const uint32_t c = lane % kPerQ;
+        const bool in_row = c * kPer16<T> < dim;
+        const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)(g * per_head.d) * a.q_head + (in_row ? c * kPer16<T> : 0);
+#pragma unroll 4
+        for (uint32_t r = lane / kPerQ; r < 32; r += 32 / kPerQ) {
+            const bool in = in_row && warp_row + r < n_rows;
+            const uint32_t row = r0 + (in ? warp_row + r : 0u), qi = per_head(row);
+            const T* p = qb + (int64_t)qi * a.q_token + (int64_t)(row - qi * per_head.d) * a.q_head;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + q_stage + (r * kPerQ + (c ^ (r & (kPerQ - 1)))) * 16), "l"(p), "r"(in ? 16 : 0) : "memory");
+        }
+    } else if (warp < 8 * RT) {
+        for (uint32_t i = 0; i < F::kAhead; ++i) {
+            if (wg + i * RT < jobs) copy(wg + i * RT);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    } else if (warp == 8 * RT) {
         tmem_alloc(smem_u32(&s_tmem), F::kColumns);
         tmem_relinquish();
-    }
-    if (tid == 0) {
-        for (uint32_t i = 0; i < kSlots; ++i) {
-            mbar_init(smem_u32(&s_full_bar[i]), 4);
-            mbar_init(smem_u32(&s_empty_bar[i]), RT);
-        }
-        for (int r = 0; r < RT; ++r) {
+    } else if (warp == 8 * RT + 1) {
+        if (lane < kSlots) mbar_init(smem_u32(&s_full_bar[lane]), 4);
+        if (lane < kSlots) mbar_init(smem_u32(&s_empty_bar[lane]), RT);
+        if (lane < RT) {
+            RowBars& bar = s_row[lane];
             for (int i = 0; i < 2; ++i) {
-                mbar_init(smem_u32(&s_row[r].s_full[i]), 1);
-                mbar_init(smem_u32(&s_row[r].p_full[i]), 4);
+                mbar_init(smem_u32(&bar.s_full[i]), 1);
+                mbar_init(smem_u32(&bar.p_full[i]), 4);
             }
-            mbar_init(smem_u32(&s_row[r].pv_full), 1);
-            mbar_init(smem_u32(&s_row[r].all_done), 1);
-            mbar_init(smem_u32(&s_row[r].q_full), 4);
+            mbar_init(smem_u32(&bar.pv_full), 1);
+            mbar_init(smem_u32(&bar.all_done), 1);
+            mbar_init(smem_u32(&bar.q_full), 4);
         }
         fence_barrier_init();
-        s_abort = 0;
+        if (lane == 0) s_abort = 0;
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -230,7 +311,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     float4* s_o = reinterpret_cast<float4*>(smem + F::kOutAt);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
     auto out_place = [](uint32_t r, uint32_t c4) -> uint32_t { return r * (DP / 4) + (c4 ^ (r & (DP / 4 - 1))); };
     auto write_row = [&](uint32_t r, uint32_t c, const float4& v) {   // four elements from column c
-        const uint32_t row = r0 + r, qi = row / per_head, head = g * per_head + (row - qi * per_head);
+        const uint32_t row = r0 + r, qi = per_head(row), head = g * per_head.d + (row - qi * per_head.d);
         T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = v;
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
@@ -239,36 +320,20 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
     if (warp < 4 * RT) {
         // ---------------------------------------------------------------- a row a thread
         regs_up<F::kRowRegs>();
-        const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16, warp_row = warp * 32u;
+        const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16;
         RowBars& bar = s_row[rt];
         const uint32_t my_tmem = tmem + rt * 256u + lanes;
         const bool real = tid < n_rows;
-        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = row / per_head;
+        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = per_head(row);
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
         float factor = fabsf(a.scale);   // of this row's scores
         {
-            // Queries: row by row through shared memory, 32 rows a warp, so that loads are of whole lines; then a thread has its own row.
-            constexpr int E = kPer16<T>, kPer = DP / E;   // pieces of 16 bytes a row
-            uint4* stage = reinterpret_cast<uint4*>(smem + F::kQueryAt + warp_row * (RT == 2 ? DP * 4 : DP * (int)sizeof(T)));   // where the warp's output goes
-            uint4 raw[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const uint32_t n = i * 32 + lane, r = n / kPer, c = n % kPer, q_row = r0 + warp_row + r;
-                raw[i] = make_uint4(0, 0, 0, 0);
-                if (warp_row + r < n_rows && c * E < dim) {
-                    const uint32_t i_q = q_row / per_head, head = g * per_head + (q_row - i_q * per_head);
-                    raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)i_q * a.q_token + (int64_t)head * a.q_head) + c);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const uint32_t n = i * 32 + lane, r = n / kPer, c = n % kPer;
-                stage[r * kPer + (c ^ (r & (kPer - 1)))] = raw[i];
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
+            uint4 raw[kPerQ];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) raw[i] = stage[lane * kPer + (i ^ (lane & (kPer - 1)))];
+            for (int i = 0; i < kPerQ; ++i) raw[i] = *reinterpret_cast<const uint4*>(smem + q_stage + (lane * kPerQ + (i ^ (lane & (kPerQ - 1)))) * 16);
             float up = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
             if (a.scale == 0.f) factor = 1.f;
             if constexpr (F::kParts == 2) {   // the power of two is the row's
@@ -278,13 +343,13 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                     if (bits < 0x7F800000u) top = max(top, bits);
                 };
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
+                for (int i = 0; i < kPerQ; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
                 const int e = exponent_for(top);
                 up *= power2(e);
                 factor *= power2(-e);
             }
 #pragma unroll
-            for (int part = 0; part < kPer / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
+            for (int part = 0; part < kPerQ / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
                 if constexpr (F::kParts == 2) {
                     uint32_t hi[8], lo[8];
 #pragma unroll
@@ -313,7 +378,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
         }
         // All rows see all of a tile that lies between these.
         const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
-        const int32_t common_hi = key_bounds(a, first + (r0 + r_first) / per_head, length).hi, common_lo = key_bounds(a, first + (r0 + max(r_last, r_first)) / per_head, length).lo;
+        const int32_t common_hi = key_bounds(a, first + per_head(r0 + r_first), length).hi, common_lo = key_bounds(a, first + per_head(r0 + max(r_last, r_first)), length).lo;
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
         const uint32_t out_at = my_tmem + F::kProduct;
         // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is o, against m_o
@@ -526,66 +591,15 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             s_l[tid] = l;
         } else {   // the warp's rows, whole lines at a time
             __syncwarp();
-            const uint32_t per_row = dim / 4, mine_rows = n_rows > warp_row ? min(32u, n_rows - warp_row) : 0u;
-            for (uint32_t i = lane; i < mine_rows * per_row; i += 32) {
-                const uint32_t r = i / per_row, c = i - r * per_row;
-                write_row(warp_row + r, c * 4, s_o[out_place(warp_row + r, c)]);
-            }
+            constexpr uint32_t kPerO = DP / 4;
+            const uint32_t c = lane % kPerO;
+#pragma unroll 4
+            for (uint32_t r = lane / kPerO; r < 32; r += 32 / kPerO)
+                if (warp_row + r < n_rows && c * 4 < dim) write_row(warp_row + r, c * 4, s_o[out_place(warp_row + r, c)]);
         }
     } else if (warp < 8 * RT) {
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
-        const uint32_t t = tid & 127u, wg = warp / 4 - RT;   // with two warpgroups one loads keys, one values
-        constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements: of one column, kStepRows rows apart
-        constexpr int kPerRow = DP / 8, kStepRows = 128 / kPerRow;
-        const uint32_t my_row = t / kPerRow, my_col = t % kPerRow;
-        const bool in_dim = my_col * 8 < dim;
-        const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head + (in_dim ? my_col * 8 : 0);
-        const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head + (in_dim ? my_col * 8 : 0);
-        const int64_t k_step = a.k_token * kStepRows, v_step = a.v_token * kStepRows;
-        // where this thread's first group lies in a tile; the rows of its others differ by multiples of eight, which leaves the swizzle as it is
-        const uint32_t place = (my_col / 8) * kPanel + my_row * 128u + (((my_col & 7u) ^ (my_row & 7u)) << 4);
-        constexpr uint32_t kPlaceStep = kStepRows * 128;
-        // Jobs are keys of a tile, values of a tile, and so on; this warpgroup's are every RT-th from wg on.
-        const uint32_t jobs = 2 * tiles;
-        // A job's source: this thread's first group, the step between its groups and how many of the groups hold keys.
-        struct Source {
-            const T* p;
-            int64_t step;
-            int n;
-            int32_t key;
-        };
-        auto source = [&](uint32_t job) -> Source {
-            int32_t k0, end;
-            tile_keys(t0 + job / 2, k0, end);
-            const int32_t rows_left = end - k0 - (int32_t)my_row;
-            Source s;
-            s.n = !in_dim || rows_left <= 0 ? 0 : min(kPerThread, (rows_left + kStepRows - 1) / kStepRows);
-            const int64_t key = (int64_t)k0 + my_row;
-            s.p = job & 1u ? vp + key * a.v_token : kp + key * a.k_token;
-            s.step = job & 1u ? v_step : k_step;
-            s.key = k0 + (int32_t)my_row;
-            return s;
-        };
-        auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
-        // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
-        auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
-            if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
-            else if (RT == 1 && job >= kSlots - 2) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
-            const Source from = source(job);
-            const uint32_t at = smem_at + slot(job);
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) {
-                const int32_t key = from.key + i * kStepRows;
-                const bool in = i < from.n && (key < gap_from || key >= gap_to);
-                const T* p = in ? from.p + i * from.step : kp;
-#pragma unroll
-                for (int h = 0; h < F::kParts; ++h) {   // fp32: two pieces of 16 bytes, to where this thread alone reads them
-                    const uint32_t to = F::kParts == 2 ? at + (i * 2 + h) * 2048 + t * 16 : at + place + i * kPlaceStep;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? p + h * 4 : kp), "r"(in ? 16 : 0) : "memory");
-                }
-            }
-        };
         auto publish = [&](uint32_t job) {
             fence_proxy_async_smem();
             __syncwarp();
@@ -599,10 +613,6 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
             return max(max(s_top[wg][turn][0], s_top[wg][turn][1]), max(s_top[wg][turn][2], s_top[wg][turn][3]));
         };
         int exp_k = 0, exp_v = 0;
-        for (uint32_t i = 0; i < F::kAhead; ++i) {
-            if (wg + i * RT < jobs) copy(wg + i * RT);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
         for (uint32_t job = wg; job < jobs; job += RT) {
             if (job + F::kAhead * RT < jobs) copy(job + F::kAhead * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -765,9 +775,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, uint32_t row_tile
                 if (k < shares) s_part[k][tid] = mk[k] == 0.f && norm == norm ? 0.f : mk[k] * norm;
         }
         __syncthreads();
-        const uint32_t per_row = dim / 4;
-        for (uint32_t i = share * kThreads + tid; i < n_rows * per_row; i += shares * kThreads) {
-            const uint32_t r = i / per_row, c = i - r * per_row, at_o = smem_u32(&s_o[out_place(r, c)]);
+        for (uint32_t i = share * kThreads + tid; i < n_rows * (DP / 4); i += shares * kThreads) {
+            const uint32_t r = i / (DP / 4), c = i % (DP / 4), at_o = smem_u32(&s_o[out_place(r, c)]);
+            if (c * 4 >= dim) continue;
             float4 x[kMostShares], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (uint32_t k = 0; k < kMostShares; ++k)
@@ -819,7 +829,7 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP, RT>, a, (uint32_t)tiles, dev_err);
+    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP, RT>, a, divisor((uint32_t)tiles), divisor(a.kv_heads), divisor(a.heads / a.kv_heads), dev_err);
 }
 
 template <typename T>
