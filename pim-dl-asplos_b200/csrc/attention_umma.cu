@@ -31,9 +31,10 @@ namespace {
 constexpr int kRows = 128, kKeys = 64;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
 constexpr uint32_t kMostShares = 8;
-// Tensor memory adds up towards zero: a sum of n products is short by about 3e-8 of its size a tile, 1.3e-5 at 16000 keys.  fp32's output is
-// taken into registers, where sums are rounded, every so many tiles; half the bits do not show it.
-constexpr uint32_t kChunk = 8;
+// Tensor memory adds up towards zero: each of a tile's twelve products takes half a unit of the sum off, 3.5e-7 of it a tile.  fp32's output is taken out
+// and summed with rounding every other tile: 4000 keys of values around 0 (around 1) come out 5.0e-7 (4.8e-7) off, plain fp32 4.8e-7 (1.2e-7); every
+// four tiles 9.2e-7 (1.2e-6), every eight 1.8e-6 (2.8e-6), never 1.8e-6 (1.3e-5 at 16000 keys).  Half the bits do not show it.
+constexpr uint32_t kChunk = 2;
 constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 // DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
@@ -41,15 +42,11 @@ template <typename T, int DP, int RT>
 struct Form {
     static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
     static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
-    static constexpr int kSlots = RT == 2 ? 8 : sizeof(T) == 4 ? 6 : 12;   // of the ring that keys and values take by turns
-    static constexpr int kAhead = RT == 2 ? 2 : sizeof(T) == 4 ? 3 : 8;    // tiles that a warpgroup has on their way
-    static constexpr int kOut = RT * kRows * DP * 4;                 // bytes of the output, in fp32
-    // Where the output is put together, and the queries are turned before: behind the ring; with one tile of rows in the ring itself, which is idle
-    // then (the queries' place is the last two slots).
-    static constexpr int kOutAt = RT == 2 ? kSlots * kTile : 0, kQueryAt = RT == 2 ? kOutAt : (kSlots - 2) * kTile;
-    static constexpr int kSmem = kSlots * kTile + (RT == 2 ? kOut : 0) + 1024;
-    static_assert(kOutAt + kOut <= kSmem - 1024 && kQueryAt + RT * kRows * DP * (int)sizeof(T) <= kSmem - 1024);
-    static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles in registers: see kChunk
+    static constexpr int kSlots = RT == 1 && sizeof(T) == 4 ? 4 : 8;       // of the ring that keys and values take by turns
+    static constexpr int kAhead = RT == 2 ? 2 : sizeof(T) == 4 ? 2 : 4;    // tiles that a warpgroup has on their way
+    static constexpr int kOut = RT * kRows * DP * 4;                 // bytes of the output, in fp32: queries come, and results leave, through there
+    static constexpr int kSmem = kSlots * kTile + kOut + 1024;
+    static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles outside tensor memory: see kChunk
     static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;   // columns of a tile of rows
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
     static_assert(RT == 1 || kUsed <= 256);
@@ -214,61 +211,42 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 
     // ---- what loads keys and values: warpgroup wg of them (with two, one loads keys, one values)
     const uint32_t t = tid & 127u, wg = warp / 4 - RT;
-    constexpr int kPerThread = kKeys * DP / 8 / 128;   // groups of eight elements: of one column, kStepRows rows apart
-    constexpr int kPerRow = DP / 8, kStepRows = 128 / kPerRow;
-    const uint32_t my_row = t / kPerRow, my_col = t % kPerRow;
-    const bool in_dim = my_col * 8 < dim;
-    const T* kp = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head + (in_dim ? my_col * 8 : 0);
-    const T* vp = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head + (in_dim ? my_col * 8 : 0);
-    const int64_t k_step = a.k_token * kStepRows, v_step = a.v_token * kStepRows;
-    // where this thread's first group lies in a tile; the rows of its others differ by multiples of eight, which leaves the swizzle as it is
-    const uint32_t place = (my_col / 8) * kPanel + my_row * 128u + (((my_col & 7u) ^ (my_row & 7u)) << 4);
-    constexpr uint32_t kPlaceStep = kStepRows * 128;
+    // A thread copies pieces of 16 bytes: of one column, kStepRows rows apart, so that neighbours copy whole rows.
+    constexpr int kElems = kPer16<T>, kPerRow = DP / kElems, kStepRows = 128 / kPerRow, kPerThread = kKeys / kStepRows;
+    const uint32_t my_row = t / kPerRow, my_col = t % kPerRow * kElems;
+    const bool in_dim = my_col < dim;
+    // Where this thread's first piece lies in a tile (of fp32: 8 bytes of it); the rows of its others differ by multiples of eight, which leaves the
+    // swizzle as it is, or of four, which turns a bit of it every time.
+    const uint32_t place = my_col / 64 * kPanel + my_row * 128u + ((my_col / 8 % 8 ^ (my_row & 7u)) << 4) + my_col % 8 * 2;
+    auto place_of = [&](int i) -> uint32_t { return (kStepRows == 4 && (i & 1) ? place ^ 64u : place) + i * kStepRows * 128; };
+    static_assert(kStepRows == 4 || kStepRows % 8 == 0);
     // Jobs are keys of a tile, values of a tile, and so on; this warpgroup's are every RT-th from wg on.
     const uint32_t jobs = 2 * tiles;
-    // A job's source: this thread's first group, the step between its groups and how many of the groups hold keys.
-    struct Source {
-        const T* p;
-        int64_t step;
-        int n;
-        int32_t key;
-    };
-    auto source = [&](uint32_t job) -> Source {
-        int32_t k0, end;
-        tile_keys(t0 + job / 2, k0, end);
-        const int32_t rows_left = end - k0 - (int32_t)my_row;
-        Source s;
-        s.n = !in_dim || rows_left <= 0 ? 0 : min(kPerThread, (rows_left + kStepRows - 1) / kStepRows);
-        const int64_t key = (int64_t)k0 + my_row;
-        s.p = job & 1u ? vp + key * a.v_token : kp + key * a.k_token;
-        s.step = job & 1u ? v_step : k_step;
-        s.key = k0 + (int32_t)my_row;
-        return s;
-    };
-    auto slot = [&](uint32_t job) -> uint32_t { return job % kSlots * F::kTile; };
     // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
     auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
         if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
-        else if (RT == 1 && job >= kSlots - 2) mbar_wait_warp(smem_u32(&s_row[0].q_full), 0, &s_abort);   // the queries passed through there
-        const Source from = source(job);
-        const uint32_t at = smem_at + slot(job);
+        int32_t k0, end;
+        tile_keys(t0 + job / 2, k0, end);
+        const bool values = job & 1u;
+        const int64_t token = values ? a.v_token : a.k_token;
+        const T* base = values ? static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head
+                               : static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
+        const int32_t key0 = k0 + (int32_t)my_row;
+        const T* from = base + (int64_t)key0 * token + my_col;
+        const uint32_t at = smem_at + job % kSlots * F::kTile;
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            const int32_t key = from.key + i * kStepRows;
-            const bool in = i < from.n && (key < gap_from || key >= gap_to);
-            const T* p = in ? from.p + i * from.step : kp;
-#pragma unroll
-            for (int h = 0; h < F::kParts; ++h) {   // fp32: two pieces of 16 bytes, to where this thread alone reads them
-                const uint32_t to = F::kParts == 2 ? at + (i * 2 + h) * 2048 + t * 16 : at + place + i * kPlaceStep;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? p + h * 4 : kp), "r"(in ? 16 : 0) : "memory");
-            }
+            const int32_t key = key0 + i * kStepRows;
+            const bool in = in_dim && key < end && (key < gap_from || key >= gap_to);
+            const uint32_t to = at + (F::kParts == 2 ? i * 2048 + t * 16 : place_of(i));   // (fp32: to where this thread alone reads it)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? from + i * kStepRows * token : base), "r"(in ? 16 : 0) : "memory");
         }
     };
 
     // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
     // lines; then a thread has its own row.
     constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
-    const uint32_t warp_row = warp * 32u, q_stage = F::kQueryAt + warp_row * (RT == 2 ? DP * 4 : DP * (int)sizeof(T));   // (with two, where the warp's output goes)
+    const uint32_t warp_row = warp * 32u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
     if (warp < 4 * RT) {
         const uint32_t c = lane % kPerQ;
         const bool in_row = c * kPer16<T> < dim;
@@ -308,7 +286,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = s_tmem;
-    float4* s_o = reinterpret_cast<float4*>(smem + F::kOutAt);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
+    float4* s_o = reinterpret_cast<float4*>(smem + kSlots * F::kTile);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
     auto out_place = [](uint32_t r, uint32_t c4) -> uint32_t { return r * (DP / 4) + (c4 ^ (r & (DP / 4 - 1))); };
     auto write_row = [&](uint32_t r, uint32_t c, const float4& v) {   // four elements from column c
         const uint32_t row = r0 + r, qi = per_head(row), head = g * per_head.d + (row - qi * per_head.d);
@@ -381,29 +359,35 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const int32_t common_hi = key_bounds(a, first + per_head(r0 + r_first), length).hi, common_lo = key_bounds(a, first + per_head(r0 + max(r_last, r_first)), length).lo;
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
         const uint32_t out_at = my_tmem + F::kProduct;
-        // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is o, against m_o
-        uint64_t o[F::kSums ? DP / 2 : 1];
+        // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is in shared memory, against m_o
         float m_o = -INFINITY;
         int unit = 0;
-        if constexpr (F::kSums) {
-#pragma unroll
-            for (int i = 0; i < DP / 2; ++i) o[i] = 0;
-        }
-        auto add_chunk = [&]() {
-            const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against), up = power2(-unit);
-            const uint64_t f2 = pair(f, f), up2 = pair(up, up);
-#pragma unroll
-            for (int col = 0; col < DP; col += 16) {
+        bool o_any = false;
+        // ... both together, times norm
+        auto add_chunk = [&](bool chunk, float norm) {
+            const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm, up = power2(-unit) * norm;
+#pragma unroll 2
+            for (uint32_t col = 0; col < DP; col += 16) {
                 uint32_t v[16];
-                tmem_ld_32x32b_x16(out_at + col, v);
-                tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint64_t& x = o[col / 2 + i];
-                    x = fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), up2, fma2(x, f2, 0ull));
+                for (int i = 0; i < 16; ++i) v[i] = 0;
+                if (chunk) {
+                    tmem_ld_32x32b_x16(out_at + col, v);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    float4& at = s_o[out_place(tid, (col + i) / 4)];
+                    float4 x = make_float4(__uint_as_float(v[i]) * up, __uint_as_float(v[i + 1]) * up, __uint_as_float(v[i + 2]) * up, __uint_as_float(v[i + 3]) * up);
+                    if (F::kSums && o_any) {
+                        const float4 y = at;
+                        x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+                    }
+                    at = norm == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : x;   // (a row that sees nothing may hold what others' values left)
                 }
             }
             m_o = m;
+            o_any = true;
         };
         uint32_t n = 0;   // tiles so far
         for (uint32_t j = 0; j < tiles; ++j) {
@@ -417,7 +401,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 if (n > 0 && !begun) {
                     if (!mbar_wait_warp(smem_u32(&bar.pv_full), (n - 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
-                    add_chunk();
+                    add_chunk(true, 1.f);
                 }
             }
             float c = factor;
@@ -515,40 +499,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             }
             const uint64_t off = pair(more - against, more - against), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
-            if constexpr (F::kSums) {
-                // Here the registers hold o, too: the scores are read once more, half by half.  Weights of 32 keys go where their scores lay,
-                // 16 columns of them and 16 of their rests.
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t sc[32], hi[16], lo[16];
-                    read(sc, half);
-                    tmem_ld_wait();
-                    if (edge) hide(sc, half ? seen1 : seen0);
+            // Weights of 32 keys go where their scores lay: 16 columns, and of fp32 16 of their rests.
+            auto weights = [&](const uint32_t (&sc)[32], uint32_t to) {
+                uint32_t hi[16], lo[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
-                        const float p = exp2_approx(x.x), q = exp2_approx(x.y);
-                        sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
-                        split2(p, q, hi[i / 2], lo[i / 2]);
-                    }
-                    tmem_st_32x32b_x16(at + half * 32, hi);
-                    tmem_st_32x32b_x16(at + half * 32 + 16, lo);
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
+                    const float p = exp2_approx(x.x), q = exp2_approx(x.y);
+                    sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
+                    if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
+                    else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
                 }
-            } else {
-                uint32_t w[32];
-                auto weights = [&](const uint32_t (&sc)[32], int to) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
-                        const float p = exp2_approx(x.x), q = exp2_approx(x.y);
-                        sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
-                        w[to + i / 2] = pack2(p, q, static_cast<std::conditional_t<sizeof(T) == 4, __half, T>*>(nullptr));
-                    }
-                };
-                weights(s0, 0);
-                weights(s1, 16);
-                tmem_st_32x32b_x32(at, w);
-            }
+                tmem_st_32x32b_x16(to, hi);
+                if constexpr (F::kParts == 2) tmem_st_32x32b_x16(to + 16, lo);
+            };
+            weights(s0, at);
+            weights(s1, at + (F::kParts == 2 ? 32 : 16));
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -561,31 +527,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const bool done = n > 0 && mbar_wait_warp(smem_u32(&bar.all_done), 0, &s_abort);
         tc_fence_after_sync();
         const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        auto put = [&](uint32_t col, float x0, float x1, float x2, float x3) {   // (a row that sees nothing may hold what others' values left)
-            s_o[out_place(tid, col / 4)] = norm == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x0 * norm, x1 * norm, x2 * norm, x3 * norm);
-        };
-        if constexpr (F::kSums) {
-            if (done) add_chunk();
-#pragma unroll
-            for (int col = 0; col < DP; col += 4) {
-                const float2 x = unpair(o[col / 2]), y = unpair(o[col / 2 + 1]);
-                put(col, x.x, x.y, y.x, y.y);
-            }
-        } else {
-#pragma unroll
-            for (int col = 0; col < DP; col += 32) {
-                uint32_t v[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = 0;
-                if (done) {
-                    tmem_ld_32x32b_x32(out_at + col, v);
-                    tmem_ld_wait();
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    put(col + i, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-            }
-        }
+        add_chunk(done, norm);
         if (shares > 1) {
             s_m[tid] = m;
             s_l[tid] = l;
@@ -618,16 +560,14 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(F::kAhead) : "memory");
             if constexpr (F::kParts == 2) {   // in place, from what this thread has copied itself
-                unsigned char* at = smem + slot(job);
-                float buf[kPerThread][8];
+                unsigned char* at = smem + job % kSlots * F::kTile;
+                float buf[kPerThread][4];
                 float big = 0.f;   // (what is no number is passed over here, and is itself in both parts)
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(at + (i * 2) * 2048 + t * 16), y = *reinterpret_cast<const float4*>(at + (i * 2 + 1) * 2048 + t * 16);
+                    const float4 x = *reinterpret_cast<const float4*>(at + i * 2048 + t * 16);
                     buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
-                    buf[i][4] = y.x; buf[i][5] = y.y; buf[i][6] = y.z; buf[i][7] = y.w;
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) big = max3(big, fabsf(buf[i][e]), fabsf(buf[i][e + 1]));
+                    big = max3(big, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
                 }
                 uint32_t top = tile_top(__float_as_uint(big), job / RT & 1u);   // behind it everybody has read
                 // 0, or 2^-2 .. 2^15 under the power of two in use, or the tile gets one of its own.
@@ -638,7 +578,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
+                        for (int e = 0; e < 4; ++e) {
                             const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
                             if (bits < 0x7F800000u) most = max(most, bits);
                         }
@@ -647,18 +587,18 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 const int reach = (int)(top >> 23) - 127 + e_now;
                 if (top != 0 && (reach >= 15 || reach < -2)) e_now = exponent_for(top);
                 const uint64_t up = pair(power2(e_now), power2(e_now));
-                unsigned char* to = at + place;
                 auto convert = [&](auto split) {
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i) {
-                        uint32_t hi[4], lo[4];
+                        uint32_t hi[2], lo[2];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < 2; ++e) {
                             const float2 x = unpair(mul2(pair(buf[i][2 * e], buf[i][2 * e + 1]), up));
                             split(x.x, x.y, hi[e], lo[e]);
                         }
-                        *reinterpret_cast<uint4*>(to + i * kPlaceStep) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(to + i * kPlaceStep + F::kPanels * kPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        unsigned char* to = at + place_of(i);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(to + F::kPanels * kPanel) = make_uint2(lo[0], lo[1]);
                     }
                 };
                 if (infinite) convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2_any(x, y, hi, lo); });
@@ -711,8 +651,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             auto wait_full = [&](uint32_t job) { return mbar_wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
             uint32_t n_s = 0, n_p = 0;   // scores and products so far, of the tiles that these rows see
             auto issue_scores = [&](uint32_t j) -> bool {
-                // they go where the weights of the last tile but one lie: its product has to be done
-                if (n_s > 1 && !mbar_wait_warp(smem_u32(&bar.pv_full), (n_s - 2) & 1u, &s_abort)) return false;
+                // They go where the weights of the last tile but one lie, so its product has to be done.  Waited for is the last product issued, that one or
+                // the one behind it: of an older phase the barrier could not tell whether it is over.
+                if (n_p > 0 && !mbar_wait_warp(smem_u32(&bar.pv_full), (n_p - 1) & 1u, &s_abort)) return false;
                 if (!wait_full(2 * j)) return false;
                 tc_fence_after_sync();
                 if (elect_one()) {
