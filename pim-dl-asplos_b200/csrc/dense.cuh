@@ -70,6 +70,32 @@ __device__ __forceinline__ void store_elems(T* p, const float (&v)[E]) {
     }
 }
 
+// E elements as they lie in memory.
+template <typename T, int E>
+struct Piece {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void widen(float (&v)[E]) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(u[i]);
+            } else {
+                const float2 f = unpack2(u[i], static_cast<T*>(nullptr));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+template <typename T>
+struct Piece<T, 1> {
+    T w;
+    __device__ __forceinline__ void load(const T* p) { w = *p; }
+    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = to_float(w); }
+};
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

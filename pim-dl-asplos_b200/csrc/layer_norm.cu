@@ -11,6 +11,7 @@
 #include "dense.cuh"
 #include "kernels.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace lutamm {
@@ -180,20 +181,30 @@ __global__ void __launch_bounds__(kBlock<TPR>) norm_grad_kernel(NormGradArgs a) 
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < E; ++i) dw[k][i] = db[k][i] = 0.f;
-    for (uint64_t row = (uint64_t)blockIdx.x * kRows + sub; row < a.rows; row += (uint64_t)gridDim.x * kRows) {
+    // The next row's loads are on their way while this one is worked on.
+    Piece<T, E> x_raw[NV], d_raw[NV];
+    auto fetch = [&](uint64_t row) {
         const T* x = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride;
         const T* dy = static_cast<const T*>(a.dout) + (int64_t)row * a.dout_stride;
-        float xh[NV][E], d[NV][E];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t g = t + k * TPR;
-#pragma unroll
-            for (int i = 0; i < E; ++i) xh[k][i] = d[k][i] = 0.f;
             if (g < groups) {
-                load_elems<T, E>(x + g * E, xh[k]);
-                load_elems<T, E>(dy + g * E, d[k]);
+                x_raw[k].load(x + g * E);
+                d_raw[k].load(dy + g * E);
             }
         }
+    };
+    const uint64_t first = (uint64_t)blockIdx.x * kRows + sub, step = (uint64_t)gridDim.x * kRows;
+    if (first < a.rows) fetch(first);
+    for (uint64_t row = first; row < a.rows; row += step) {
+        float xh[NV][E], d[NV][E];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            x_raw[k].widen(xh[k]);
+            d_raw[k].widen(d[k]);
+        }
+        if (row + step < a.rows) fetch(row + step);
         const float mean = __ldg(a.stats + 2 * row), rstd = __ldg(a.stats + 2 * row + 1);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -312,23 +323,23 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(NormGradArgs a) {
     a.partial[(size_t)blockIdx.y * 2 * a.width + a.width + c] = db;
 }
 
-// partial[parts][2][width] -> dw, db: 32 columns a CTA, eight threads to a column, their sums joined in order.
-__global__ void __launch_bounds__(256) norm_join_kernel(const float* partial, uint32_t parts, uint32_t width, float* dweight, float* dbias) {
-    __shared__ float s[8][32];
+// partial[parts][2][width] -> dw, db: 32 columns a CTA, 32 threads to a column, their sums joined in order.
+__global__ void __launch_bounds__(1024) norm_join_kernel(const float* partial, uint32_t parts, uint32_t width, float* dweight, float* dbias) {
+    __shared__ float s[32][33];
     const uint32_t lane = threadIdx.x & 31u, k = threadIdx.x >> 5;
     const uint64_t c = (uint64_t)blockIdx.x * 32 + lane, columns = 2 * (uint64_t)width;
     float sum = 0.f;
     if (c < columns) {
 #pragma unroll 8
-        for (uint32_t p = k; p < parts; p += 8) sum += partial[(size_t)p * columns + c];
+        for (uint32_t p = k; p < parts; p += 32) sum += partial[(size_t)p * columns + c];
     }
     s[k][lane] = sum;
     __syncthreads();
-    if (k == 0 && c < columns) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) sum += s[i][lane];
-        float* out = c < width ? dweight : dbias;
-        if (out) out[c < width ? c : c - width] = sum;
+    sum = warp_sum(s[lane][k]);   // column k of the CTA's
+    const uint64_t mine = (uint64_t)blockIdx.x * 32 + k;
+    if (lane == 0 && mine < columns) {
+        float* out = mine < width ? dweight : dbias;
+        if (out) out[mine < width ? mine : mine - width] = sum;
     }
 }
 
@@ -361,30 +372,32 @@ cudaError_t run_norm(const NormArgs& a, cudaStream_t s) {
 
 template <typename T, int TPR, int NV, int E>
 cudaError_t run_grad(const NormGradArgs& a, uint32_t ctas, cudaStream_t s) {
-    const int bytes = TPR == 32 ? (int)(2 * a.width * sizeof(float)) : 0;   // at most 8 KB: a warp holds 1024 elements
+    const int bytes = TPR == 32 ? (int)(2 * a.width * sizeof(float)) : 0;   // at most 2 KB: a warp holds 256 elements
     norm_grad_kernel<T, TPR, NV, E><<<ctas, kBlock<TPR>, bytes, s>>>(a);
     return cudaGetLastError();
 }
 
+// Threads of a row, by its width: eight to sixteen elements a thread, so that the sums of several CTAs' columns fit an SM's registers.
+inline int grad_threads(uint32_t width) { return width <= 256 ? 32 : width <= 2048 ? 128 : 512; }
+
 template <typename T, int E>
 cudaError_t run_norm_grad(const NormGradArgs& a, uint32_t ctas, cudaStream_t s) {
-    const uint32_t groups = a.width / E;
-    constexpr int kMost = 16 / E;   // groups that make 16 elements a thread
-    if (a.width <= 128) return run_grad<T, 32, (128 / 32 + E - 1) / E, E>(a, ctas, s);
-    if (groups <= 32 * kMost) return run_grad<T, 32, kMost, E>(a, ctas, s);
-    if constexpr (E > 1) {
-        if (groups <= 32 * 2 * kMost) return run_grad<T, 32, 2 * kMost, E>(a, ctas, s);
-    }
-    if (groups <= 128 * kMost) return run_grad<T, 128, kMost, E>(a, ctas, s);
-    return run_grad<T, 512, kMost, E>(a, ctas, s);
+    constexpr int k4 = (4 + E - 1) / E, k8 = 8 / E, k16 = 16 / E;   // groups that make so many elements a thread
+    if (a.width <= 32 * 4 && E <= 4) return run_grad<T, 32, k4, E>(a, ctas, s);
+    if (a.width <= 32 * 8) return run_grad<T, 32, k8, E>(a, ctas, s);
+    if (a.width <= 128 * 8) return run_grad<T, 128, k8, E>(a, ctas, s);
+    if (a.width <= 128 * 16) return run_grad<T, 128, k16, E>(a, ctas, s);
+    if (a.width <= 512 * 8) return run_grad<T, 512, k8, E>(a, ctas, s);
+    return run_grad<T, 512, k16, E>(a, ctas, s);
 }
 
-// The parts that the sums towards dw and db come in: CTAs, or row blocks of the columns' kernel.
+// The parts that the sums towards dw and db come in: CTAs, or row blocks of the columns' kernel.  Four rows a CTA at least, which halves what the
+// second launch reads.
 uint32_t grad_parts(uint32_t rows, uint32_t width, int sm_count) {
-    const uint32_t per = width > kMostElems ? 1 : width <= 1024 ? 8 : 1;   // rows a CTA takes at a time
-    const uint32_t sets = (rows + per - 1) / per;
-    const uint32_t most = (uint32_t)sm_count * (width > kMostElems ? 1 : width <= 1024 ? 2 : width <= 2048 ? 6 : 2);
-    return sets < most ? (sets ? sets : 1) : most;
+    if (width > kMostElems) return std::max(1u, std::min(rows, (uint32_t)sm_count));
+    const int threads = grad_threads(width);
+    const uint32_t per = 4 * (threads == 32 ? 8 : 1), sets = (rows + per - 1) / per;
+    return std::max(1u, std::min(sets, (uint32_t)sm_count * (threads == 512 ? 2 : 4)));
 }
 
 template <typename T>
@@ -407,7 +420,7 @@ cudaError_t run_typed_grad(const NormGradArgs& a, int sm_count, cudaStream_t s) 
         e = vec ? run_norm_grad<T, kPer16<T>>(a, parts, s) : run_norm_grad<T, 1>(a, parts, s);
     }
     if (e != cudaSuccess || !a.partial) return e;
-    norm_join_kernel<<<(uint32_t)((2 * (uint64_t)a.width + 31) / 32), 256, 0, s>>>(a.partial, parts, a.width, a.dweight, a.dbias);
+    norm_join_kernel<<<(uint32_t)((2 * (uint64_t)a.width + 31) / 32), 1024, 0, s>>>(a.partial, parts, a.width, a.dweight, a.dbias);
     return cudaGetLastError();
 }
 
