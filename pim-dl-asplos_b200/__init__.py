@@ -316,6 +316,8 @@ class LutAmmContext:
             raise LutAmmError(rc, self._L.lutamm_last_error(None).decode())
         self._h = h
         self._amm_address = ctypes.cast(self._L.lutamm_amm, ctypes.c_void_p).value
+        self._dense_address = {n: ctypes.cast(getattr(self._L, "lutamm_" + n), ctypes.c_void_p).value
+                               for n in ("layer_norm", "layer_norm_backward", "rotary", "attention")}
         self.device = device
         self.stream: int | None = None   # the caller's stream, None while the context runs on its own
         self.layers: dict[int, _LayerInfo] = {}
@@ -429,11 +431,23 @@ class LutAmmContext:
         self._check(self._L.lutamm_pim_lut(self._h, layer_id, _ptr(input_index), _ptr(output_tensor), M, flags))
 
     # -- the layer's dense operators (device tensors; include/lutamm.h has the formulas)
+    def _fast_dense(self, name: str, *args) -> bool:
+        """The call through csrc/python/fastcall.c, where that takes these arguments."""
+        if _fast is None or not self._h:
+            return False
+        rc = getattr(_fast, name)(self._dense_address[name], self._h.value, *args)
+        if rc is NotImplemented:
+            return False
+        self._check(rc)
+        return True
+
     def layer_norm(self, x, weight, bias, out, eps: float = 1e-6, residual=None, stats=None, flags: int = 0):
         """out = residual + layer norm of x over the last axis (layer_norm() of the reference, transformer_layer.cpp:50-90, and the
         addition behind it).  x, residual, out [rows, width] float32, float16 or bfloat16, rows of any stride; weight and bias
         float32 [width] or None; stats float32 [rows, 2] takes mean and 1 / sqrt(var + eps) for layer_norm_backward.  out may
         be x or residual."""
+        if self._fast_dense("layer_norm", x, weight, bias, out, eps, residual, stats, flags):
+            return
         import torch
         rows, width = x.shape
         f32 = torch.float32
@@ -448,6 +462,8 @@ class LutAmmContext:
         """Gradients of layer_norm: dx like x, dweight and dbias float32 [width], each only where a tensor is given (that of the
         residual is dout).  stats as layer_norm left them.  workspace: a uint8 tensor of layer_norm_backward_workspace() bytes
         in place of the context's own, for captured calls that may run beside others of this context."""
+        if workspace is None and self._fast_dense("layer_norm_backward", dout, x, weight, stats, dx, dweight, dbias, flags):
+            return
         import torch
         rows, width = x.shape
         f32 = torch.float32
@@ -470,17 +486,22 @@ class LutAmmContext:
         or bfloat16, of any strides (the query and key heads of a fused projection are one view); out may be x.  positions
         int32 [tokens, axes], or [batch, tokens, axes]; inv_freq float32 [sum(sections)]; sections the pairs of each axis.
         Pairs are (i, i + pairs) of a head, or (2i, 2i + 1) if interleaved.  inverse turns back: the gradient."""
+        if self._fast_dense("rotary", x, positions, inv_freq, sections, out, interleaved, inverse, flags):
+            return
         import torch
-        if x.dim() == 3:
+        batched, own_positions = x.dim() == 4, positions.dim() == 3
+        if not batched:
             x, out = x.unsqueeze(0), out.unsqueeze(0)
-        if positions.dim() == 2:
+        if not own_positions:
             positions = positions.expand(x.shape[0], -1, -1)
         axes = len(sections)
         if x.dim() != 4 or not 1 <= axes <= MAX_AXES or min(sections) < 0:
             raise ValueError(f"x has three or four axes, sections 1 to {MAX_AXES} counts")
         p = RotaryParams(_dtype_of(x), *x.shape, axes, tuple(sections), bool(interleaved), bool(inverse), _heads("x", x, x.dtype, x.shape),
                          _heads("out", out, x.dtype, x.shape), _operand("positions", positions, torch.int32, (*x.shape[:2], axes)),
-                         positions.stride(0), positions.stride(1), _packed("inv_freq", inv_freq, torch.float32, (sum(sections),)))
+                         positions.stride(0) if own_positions else 0, positions.stride(1), _packed("inv_freq", inv_freq, torch.float32, (sum(sections),)))
+        if not batched:
+            p.x.batch_stride = p.out.batch_stride = 0
         self._check(self._L.lutamm_rotary(self._h, ctypes.byref(p), flags))
 
     def attention(self, q, k, v, out, scale: float | None = None, window=(-1, -1), sinks: int = 0, lengths=None, first=None, flags: int = 0):
@@ -490,6 +511,8 @@ class LutAmmContext:
         sequence b is at position first[b] + i (first: int32 [batch] on the device, None: 0) and sees the keys from window[0]
         in front of it to window[1] behind it (negative: no bound), and of those in front also the first `sinks`, up to
         lengths[b] (int32 [batch] on the device, None: all).  A query that sees none gives zeros."""
+        if self._fast_dense("attention", q, k, v, out, scale, window, sinks, lengths, first, flags):
+            return
         import torch
         B, Q, H, D = q.shape
         K, G = k.shape[1:3]

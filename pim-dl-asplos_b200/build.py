@@ -91,12 +91,12 @@ def build_host(force: bool = False) -> None:
 
 
 def build_fastcall(force: bool = False) -> None:
-    """The operator call as a CPython extension (the ctypes binding serves where Python's headers are missing)."""
+    """The operator calls as a CPython extension (the ctypes binding serves where Python's headers are missing)."""
     src, inc = os.path.join(CSRC, "python", "fastcall.c"), sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(inc, "Python.h")):
         return
-    if force or _stale(FASTCALL, [src]):
-        subprocess.run(["gcc", "-O2", "-Wall", "-fPIC", "-shared", "-I", inc, "-o", FASTCALL, src], check=True)
+    if force or _stale(FASTCALL, [src, os.path.join(HERE, "..", "include", "lutamm.h")]):
+        subprocess.run(["gcc", "-O2", "-Wall", "-fPIC", "-shared", "-I", inc, "-o", FASTCALL, src, "-lm"], check=True)
 
 
 def build_all(force: bool = False, verbose: bool = False) -> None:
