@@ -394,6 +394,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if (!sees(t0 + j)) continue;
             if (!mbar_wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
+            if (warp_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
+                if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
+                ++n;
+                continue;
+            }
             const uint32_t at = my_tmem + F::kScores + (n & 1u) * kKeys;
             bool begun = n > 0;   // whether tensor memory holds an output to go on with
             if constexpr (F::kSums) {
@@ -755,8 +760,12 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     // Keys that a tile of rows sees at most.
     uint64_t keys = a.keys;
     if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + RT * kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
+    // As many shares as the SMs hold, by twos (clusters of three do not all find room: 48 items in thirds 42 us, in halves 29), of at least four tiles,
+    // or two of fp32: joining them takes as long as those (256 tokens of 12 heads in bf16 in quarters 11.8 us, whole 9.8; 512 in fp32 in quarters 17.7,
+    // in halves 21.6).
+    constexpr uint32_t kShareTiles = sizeof(T) == 4 ? 2 : 4;
     uint32_t shares = 1;
-    while (shares < kMostShares && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kKeys) shares *= 2;
+    while (shares < kMostShares && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kShareTiles * kKeys) shares *= 2;
     if (rows > 0x7FFFFFFFull || items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((uint32_t)(items * shares));
