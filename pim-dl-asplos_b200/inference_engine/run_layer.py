@@ -2,6 +2,7 @@
 
     python run_layer.py --transformer_config_file configs/bert_base_layer.yaml
                         [--need_compile] [--need_breakdown --breakdown_type {0,1,2}] [--tune]
+                        [--dense_kernels [--window N --sinks N]]
 
 Runs 5 warm-up and 10 timed rounds of one layer (test_transformer_layer.cpp:35-36) on random
 weights and prints "inference time", the line the reference's experiment scripts look for,
@@ -39,6 +40,10 @@ def parse_args():
                         'a checkpoint that holds query/key/value instead of a fused qkv operator selects this by itself')
     p.add_argument('--separate_gelu', action='store_true', default=False,
                    help='run GELU as its own pass after FFN1, as the reference does, instead of in the FFN1 epilogue')
+    p.add_argument('--dense_kernels', action='store_true', default=False,
+                   help="run attention and the norms in this library's own kernels instead of PyTorch's")
+    p.add_argument('--window', type=int, default=-1, help='with --dense_kernels: keys seen on either side of a query (negative: all)')
+    p.add_argument('--sinks', type=int, default=0, help='with --dense_kernels and --window: first tokens that stay visible')
     return p.parse_args()
 
 
@@ -84,7 +89,8 @@ def run(args, whole_model: bool):
                 w[name] = (cen, lut, bias, cfg["scale"][key], cfg["lut_bias"][key])
             weights.append(w)
     print("attention projections:", "separate Q / K / V operators" if "qkv" not in weights[0] else "one fused QKV operator")
-    model = L.LutTransformer(ctx, weights, S, B, H, plans=cfg["plans"], fused_gelu=not getattr(args, "separate_gelu", False))
+    model = L.LutTransformer(ctx, weights, S, B, H, plans=cfg["plans"], fused_gelu=not getattr(args, "separate_gelu", False),
+                          dense=L.Dense(window=(args.window, args.window), sinks=args.sinks) if getattr(args, "dense_kernels", False) else None)
     if args.tune:
         plans = model.layers[0].tune()
         for lay in model.layers[1:]:

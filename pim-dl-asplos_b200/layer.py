@@ -14,7 +14,10 @@ and transformer_inference() (transformer_model.cpp:13-49) of the reference:
 
 The four linears run in the CUDA library through the C ABI; attention, LayerNorm and the
 residual adds are plain PyTorch on the same stream (they stay dense fp32, as in the
-reference, where they run in ggml on the host).  The GELU after FFN1 - a separate in-place
+reference, where they run in ggml on the host), or, with a `Dense`, the library's own operators in fp32 as well:
+rotary positions on Q and K in place, attention with a window and padded sequences, LayerNorm with the residual behind it in
+one pass.  The two differ in the last bits, and where a bit decides which centroid is nearest, a linear takes another
+table row; so the default stays what it was.  The GELU after FFN1 - a separate in-place
 pass in the reference (:503) - is applied inside the FFN1 operator's epilogue
 (`fused_gelu`, lutamm_set_activation), which saves one read and one write of [n, ffn_dim].  All the loops of the reference that move
 data between the DPU-tiled layout and row-major (:97-208, :449-471, :520-542, :574-596)
@@ -25,6 +28,8 @@ is not part of the reference tree, so the layer's output is not pinned bit for b
 results inside it are.
 """
 from __future__ import annotations
+
+from dataclasses import dataclass
 
 import numpy as np
 
@@ -123,11 +128,26 @@ def checkpoint_layer_count(npz) -> int:
     return max(ids) + 1 if ids else 0
 
 
+@dataclass
+class Dense:
+    """The layer's dense operators in the library: attention sees keys from window[0] in front of a query to window[1] behind it (negative: no
+    bound) and of those in front also the first `sinks` (the class token, say), up to lengths[b] (int32 [batch] on the device: padded
+    sequences).  positions (int32 [seq, axes] or [batch, seq, axes]), inv_freq (float32 [pairs]) and sections (pairs of each axis)
+    turn queries and keys first; without positions they stay as they are."""
+    window: tuple = (-1, -1)
+    sinks: int = 0
+    lengths: object = None
+    positions: object = None
+    inv_freq: object = None
+    sections: tuple = ()
+    interleaved: bool = False
+
+
 class LutTransformerLayer:
-    """One encoder layer; `forward` takes and returns a device tensor [n, token_dim]."""
+    """One encoder layer; `forward` takes and returns a device tensor [n, token_dim].  dense: a Dense, None for PyTorch's operators."""
 
     def __init__(self, ctx: LutAmmContext, weights: dict, seq_len: int, batch_size: int, head_num: int,
-                 first_layer_id: int = 0, plans: dict | None = None, fused_gelu: bool = True):
+                 first_layer_id: int = 0, plans: dict | None = None, fused_gelu: bool = True, dense: Dense | None = None):
         import torch
         self.ctx, self.torch = ctx, torch
         self.seq_len, self.batch, self.heads = seq_len, batch_size, head_num
@@ -158,6 +178,9 @@ class LutTransformerLayer:
                 self.buf[name] = torch.empty(self.n, self.token_dim, **f32)
         else:
             self.buf["qkv"] = torch.empty(self.n, 3 * self.token_dim, **f32)
+        self.dense = dense
+        if dense is not None:
+            self.buf["att"], self.buf["h"] = torch.empty(self.n, self.token_dim, **f32), torch.empty(self.n, self.token_dim, **f32)
         self.amm_ms = 0.0
         self._graph = None          # (key, graph, input copy, h, f, launches) of the captured forward
         self._seen, self._seen_key = 0, None
@@ -180,7 +203,7 @@ class LutTransformerLayer:
                     x_in.copy_(x)
                     graph.replay()
                     self.ctx.replayed_launches += launches
-                    return h + f
+                    return self._finish(h, f)
                 # two ordinary calls under the same key first: they size every buffer, and a caller that keeps
                 # changing something is left alone
                 self._graph = None
@@ -188,8 +211,15 @@ class LutTransformerLayer:
                 self._seen_key = key
                 if self._seen > 2:
                     self._capture(x, key)
-        h, f = self._body(x)
-        return h + f
+        return self._finish(*self._body(x))
+
+    def _finish(self, h, f):
+        """The layer's last addition, into a tensor of the call's own: y = h + f, with a Dense y = h + LayerNorm_2(f)."""
+        if getattr(self, "dense", None) is None:
+            return h + f
+        y = self.torch.empty_like(h)
+        self.ctx.layer_norm(f, *self.ln["ln2"], y, eps=1e-6, residual=h, flags=FLAG_ASYNC)
+        return y
 
     def _graph_key(self, x):
         """What a captured forward depends on beyond the values in x; None where it does not apply."""
@@ -232,8 +262,33 @@ class LutTransformerLayer:
         if self.ctx.generation == key[1]:
             self._graph = (key, graph, x_in, h, f, launches)
 
+    def _dense_body(self, x):
+        """The layer up to its second norm, all in the library."""
+        B, S, H, D = self.batch, self.seq_len, self.heads, self.token_dim
+        hd, d, ctx = D // H, self.dense, self.ctx
+        if self.separate_qkv:
+            q, k, v = (self._amm(name, x).view(B, S, H, hd) for name in ("q", "k", "v"))
+            turned = (q, k)
+        else:
+            qkv = self._amm("qkv", x).view(B, S, 3 * H, hd)
+            q, k, v = qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:]
+            turned = (qkv[:, :, :2 * H],)
+        if d.positions is not None:
+            for t in turned:
+                ctx.rotary(t, d.positions, d.inv_freq, d.sections, t, interleaved=d.interleaved, flags=FLAG_ASYNC)
+        att = self.buf["att"]
+        ctx.attention(q, k, v, att.view(B, S, H, hd), window=tuple(d.window), sinks=d.sinks, lengths=d.lengths, flags=FLAG_ASYNC)
+        h = self.buf["h"]
+        ctx.layer_norm(self._amm("o", att), *self.ln["ln1"], h, eps=1e-6, residual=x, flags=FLAG_ASYNC)
+        f = self._amm("ffn1", h)
+        if not self.fused_gelu:
+            f = self.torch.nn.functional.gelu(f, approximate="tanh")
+        return h, self._amm("ffn2", f)
+
     def _body(self, x):
         """The layer up to its last addition: y = h + f."""
+        if getattr(self, "dense", None) is not None:
+            return self._dense_body(x)
         torch, F = self.torch, self.torch.nn.functional
         B, S, H, D = self.batch, self.seq_len, self.heads, self.token_dim
         hd = D // H
@@ -255,9 +310,9 @@ class LutTransformerLayer:
 class LutTransformer:
     """layer_num encoder layers back to back (transformer_model.cpp:13-49)."""
 
-    def __init__(self, ctx, layer_weights: list, seq_len, batch_size, head_num, plans=None, fused_gelu=True):
+    def __init__(self, ctx, layer_weights: list, seq_len, batch_size, head_num, plans=None, fused_gelu=True, dense=None):
         self.layers = [LutTransformerLayer(ctx, w, seq_len, batch_size, head_num, first_layer_id=8 * i, plans=plans,
-                                           fused_gelu=fused_gelu)
+                                           fused_gelu=fused_gelu, dense=dense)
                        for i, w in enumerate(layer_weights)]
 
     def forward(self, x):
