@@ -51,11 +51,13 @@ struct Form {
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
     static_assert(RT == 1 || kUsed <= 256);
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
-    // Warpgroups: RT that own rows, RT that load, one that issues.  Registers a thread of each; their sum is what the warpgroups are launched with.
-    static constexpr int kThreads = (2 * RT + 1) * 128;
-    static constexpr int kLaunchRegs = RT == 2 ? 96 : DP <= 64 ? 80 : 168;
-    static constexpr int kRowRegs = RT == 2 ? 160 : DP <= 64 ? 152 : 232, kLoadRegs = DP <= 64 ? 64 : 136, kIssueRegs = RT == 2 ? 32 : DP <= 64 ? 24 : 136;
-    static_assert(RT * (kRowRegs + kLoadRegs) + kIssueRegs == (2 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
+    // Warpgroups: two for each tile of rows, one with the first 32 keys of a tile and one with the others, one for each that loads, one that issues.
+    // Registers a thread of each; their sum is what the warpgroups are launched with.
+    static constexpr int kThreads = (3 * RT + 1) * 128;
+    static constexpr int kLaunchRegs = RT == 2 ? 72 : DP <= 64 ? 64 : 128;
+    static constexpr int kRowRegs = DP > 64 ? 152 : RT == 2 || sizeof(T) == 4 ? 80 : 88, kLoadRegs = DP > 64 ? 128 : RT == 2 ? 72 : sizeof(T) == 4 ? 56 : 40;
+    static constexpr int kIssueRegs = DP > 64 ? 80 : 40;
+    static_assert(RT * (2 * kRowRegs + kLoadRegs) + kIssueRegs == (3 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
 };
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -135,17 +137,13 @@ __device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint3
 __device__ __forceinline__ uint64_t below(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 struct RowBars {   // of a tile of rows
-    uint64_t s_full[2], p_full[2], pv_full, all_done, q_full;
+    uint64_t s_full[2], p_full[2], done[2], q_full, halves[4];   // scores, weights and products of every other tile; queries; a row's two warps
 };
 
 // Which of the CTA's tiles of keys a tile of rows sees any of: the sinks', and from .. to - 1.
 struct Seen {
     uint32_t sink_tiles, from, to;
     __device__ __forceinline__ bool operator()(uint32_t t) const { return t < sink_tiles || (t >= from && t < to); }
-    // the last one of t0 .. t1 - 1 that is seen, if any is
-    __device__ __forceinline__ uint32_t last(uint32_t t0, uint32_t t1) const {
-        return min(to, t1) > max(from, t0) ? min(to, t1) - 1 : min(sink_tiles, t1) > t0 ? min(sink_tiles, t1) - 1 : 0xFFFFFFFFu;
-    }
 };
 
 // n / d for n below 2^31: the quotient's 32 bits above the binary point of n * mul / 2^(31 + shift).
@@ -169,6 +167,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     __shared__ __align__(8) RowBars s_row[RT];
     __shared__ uint32_t s_tmem, s_abort, s_top[RT][3][4];
     __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most four tiles ahead of who reads these
+    __shared__ float s_half[2][2][RT * kRows], s_factor[RT * kRows];   // what the two warps of a row tell one another
     __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_part[kMostShares][RT * kRows];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
@@ -210,7 +209,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     };
 
     // ---- what loads keys and values: warpgroup wg of them (with two, one loads keys, one values)
-    const uint32_t t = tid & 127u, wg = warp / 4 - RT;
+    const uint32_t t = tid & 127u, wg = warp / 4 - 2 * RT;
     // A thread copies pieces of 16 bytes: of one column, kStepRows rows apart, so that neighbours copy whole rows.
     constexpr int kElems = kPer16<T>, kPerRow = DP / kElems, kStepRows = 128 / kPerRow, kPerThread = kKeys / kStepRows;
     const uint32_t my_row = t / kPerRow, my_col = t % kPerRow * kElems;
@@ -246,8 +245,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
     // lines; then a thread has its own row.
     constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
-    const uint32_t warp_row = warp * 32u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
-    if (warp < 4 * RT) {
+    const uint32_t warp_row = warp / 8 * kRows + (warp & 3u) * 32u, half = warp / 4 & 1u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
+    if (warp < 8 * RT) {
+      if (half == 0) {
         const uint32_t c = lane % kPerQ;
         const bool in_row = c * kPer16<T> < dim;
         const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)(g * per_head.d) * a.q_head + (in_row ? c * kPer16<T> : 0);
@@ -258,25 +258,26 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             const T* p = qb + (int64_t)qi * a.q_token + (int64_t)(row - qi * per_head.d) * a.q_head;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + q_stage + (r * kPerQ + (c ^ (r & (kPerQ - 1)))) * 16), "l"(p), "r"(in ? 16 : 0) : "memory");
         }
-    } else if (warp < 8 * RT) {
+      }
+    } else if (warp < 12 * RT) {
         for (uint32_t i = 0; i < F::kAhead; ++i) {
             if (wg + i * RT < jobs) copy(wg + i * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-    } else if (warp == 8 * RT) {
+    } else if (warp == 12 * RT) {
         tmem_alloc(smem_u32(&s_tmem), F::kColumns);
         tmem_relinquish();
-    } else if (warp == 8 * RT + 1) {
+    } else if (warp == 12 * RT + 1) {
         if (lane < kSlots) mbar_init(smem_u32(&s_full_bar[lane]), 4);
         if (lane < kSlots) mbar_init(smem_u32(&s_empty_bar[lane]), RT);
         if (lane < RT) {
             RowBars& bar = s_row[lane];
             for (int i = 0; i < 2; ++i) {
                 mbar_init(smem_u32(&bar.s_full[i]), 1);
-                mbar_init(smem_u32(&bar.p_full[i]), 4);
+                mbar_init(smem_u32(&bar.p_full[i]), 8);
+                mbar_init(smem_u32(&bar.done[i]), 1);
             }
-            mbar_init(smem_u32(&bar.pv_full), 1);
-            mbar_init(smem_u32(&bar.all_done), 1);
+            for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar.halves[i]), 2);
             mbar_init(smem_u32(&bar.q_full), 4);
         }
         fence_barrier_init();
@@ -295,18 +296,30 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
     };
 
-    if (warp < 4 * RT) {
-        // ---------------------------------------------------------------- a row a thread
+    if (warp < 8 * RT) {
+        // ---------------------------------------------------------------- a row for two threads, in two warps: half the keys of a tile each
         regs_up<F::kRowRegs>();
-        const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16;
+        const uint32_t rt = warp / 8, lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
         RowBars& bar = s_row[rt];
         const uint32_t my_tmem = tmem + rt * 256u + lanes;
-        const bool real = tid < n_rows;
-        const uint32_t row = r0 + (real ? tid : n_rows - 1), qi = per_head(row);
+        const uint32_t row = r0 + min(r, n_rows - 1), qi = per_head(row);
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
+        // The two warps of a row exchange a number of each row: what the other one has for this row.  False where the other one does not come.
+        uint32_t exchanges = 0;
+        auto exchange = [&](float v, float& theirs) -> bool {
+            s_half[exchanges & 1u][half][r] = v;
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bar.halves[warp & 3u]));
+            const bool ok = mbar_wait_warp(smem_u32(&bar.halves[warp & 3u]), exchanges & 1u, &s_abort);
+            tc_fence_after_sync();
+            theirs = s_half[exchanges & 1u][half ^ 1u][r];
+            ++exchanges;
+            return ok;
+        };
         float factor = fabsf(a.scale);   // of this row's scores
-        {
+        if (half == 0) {
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
             uint4 raw[kPerQ];
@@ -350,10 +363,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 }
             }
             tmem_st_wait();
+            if constexpr (F::kParts == 2) s_factor[r] = factor;
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.q_full));
+        } else if (F::kParts == 2) {
+            if (mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort)) factor = s_factor[r];
+        } else if (a.scale == 0.f) {
+            factor = 1.f;
         }
+        constexpr uint32_t kCols = DP / 2;   // of the output, a warp's
+        const uint32_t col0 = half * kCols;
         // All rows see all of a tile that lies between these.
         const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
         const int32_t common_hi = key_bounds(a, first + per_head(r0 + r_first), length).hi, common_lo = key_bounds(a, first + per_head(r0 + max(r_last, r_first)), length).lo;
@@ -367,7 +387,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         auto add_chunk = [&](bool chunk, float norm) {
             const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm, up = power2(-unit) * norm;
 #pragma unroll 2
-            for (uint32_t col = 0; col < DP; col += 16) {
+            for (uint32_t col = col0; col < col0 + kCols; col += 16) {
                 uint32_t v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] = 0;
@@ -377,7 +397,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 }
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    float4& at = s_o[out_place(tid, (col + i) / 4)];
+                    float4& at = s_o[out_place(r, (col + i) / 4)];
                     float4 x = make_float4(__uint_as_float(v[i]) * up, __uint_as_float(v[i + 1]) * up, __uint_as_float(v[i + 2]) * up, __uint_as_float(v[i + 3]) * up);
                     if (F::kSums && o_any) {
                         const float4 y = at;
@@ -404,7 +424,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if constexpr (F::kSums) {
                 begun = n % kChunk != 0;
                 if (n > 0 && !begun) {
-                    if (!mbar_wait_warp(smem_u32(&bar.pv_full), (n - 1) & 1u, &s_abort)) break;
+                    if (!mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     add_chunk(true, 1.f);
                 }
@@ -420,39 +440,29 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             int32_t k0, end;
             tile_keys(t0 + j, k0, end);
-            uint32_t seen0 = 0xFFFFFFFFu, seen1 = 0xFFFFFFFFu;
-            const bool edge = !((int64_t)k0 + kKeys <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + kKeys <= (int64_t)a.sinks));
-            if (edge) {
-                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
-                seen0 = (uint32_t)seen;
-                seen1 = (uint32_t)(seen >> 32);
-            }
-            auto read = [&](uint32_t (&sc)[32], int half) {
-                tmem_ld_32x32b_x32(at + half * 32, sc);
-            };
-            auto hide = [&](uint32_t (&sc)[32], uint32_t bits) {
+            uint32_t sc[32];
+            tmem_ld_32x32b_x32(at + half * 32, sc);
+            tmem_ld_wait();
+            k0 += half * 32;
+            if (!((int64_t)k0 + 32 <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + 32 <= (int64_t)a.sinks))) {
+                const uint32_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (!(bits >> i & 1u)) sc[i] = 0xFF800000u;
-            };
-            auto largest = [&](const uint32_t (&sc)[32]) {
-                float t[2] = {-INFINITY, -INFINITY};
+                    if (!(seen >> i & 1u)) sc[i] = 0xFF800000u;
+            }
+            float top;
+            {
+                float x = -INFINITY, y = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    t[0] = max3(t[0], __uint_as_float(sc[i]), __uint_as_float(sc[i + 1]));
-                    t[1] = max3(t[1], __uint_as_float(sc[i + 2]), __uint_as_float(sc[i + 3]));
+                    x = max3(x, __uint_as_float(sc[i]), __uint_as_float(sc[i + 1]));
+                    y = max3(y, __uint_as_float(sc[i + 2]), __uint_as_float(sc[i + 3]));
                 }
-                return fmaxf(t[0], t[1]);
-            };
-            uint32_t s0[32], s1[32];
-            read(s0, 0);
-            read(s1, 1);
-            tmem_ld_wait();
-            if (edge) {
-                hide(s0, seen0);
-                hide(s1, seen1);
+                top = fmaxf(x, y) * c;
+                float other;
+                if (!exchange(top, other)) break;
+                top = fmaxf(top, other);
             }
-            const float top = fmaxf(largest(s0), largest(s1)) * c;
             // Another maximum, or another power of two of the values: the output so far is brought in line, where there is one.
             float more = kBoost;   // log2 of what this tile's weights carry
             if (m == -INFINITY) m = top;
@@ -461,19 +471,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 const float m_new = top > m + kSlack ? top : m;
                 const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
                 if (begun) {
-                    if (!mbar_wait_warp(smem_u32(&bar.pv_full), (n - 1) & 1u, &s_abort)) break;
+                    if (!mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     float f = shrink;
                     if constexpr (F::kParts == 2) {
                         float big = 0.f;
 #pragma unroll 1
-                        for (uint32_t col = 0; col < DP; col += 16) {
+                        for (uint32_t col = col0; col < col0 + kCols; col += 16) {
                             uint32_t v[16];
                             tmem_ld_32x32b_x16(out_at + col, v);
                             tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
                         }
+                        float other;
+                        if (!exchange(big, other)) break;
+                        big = fmaxf(big, other);
                         // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
                         const int x = max(-120, min(120, e - unit));
                         if (x <= 0 || big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2))) {
@@ -482,7 +495,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         }
                     }
 #pragma unroll 1
-                    for (uint32_t col = 0; col < DP; col += 16) {
+                    for (uint32_t col = col0; col < col0 + kCols; col += 16) {
                         uint32_t v[16];
                         tmem_ld_32x32b_x16(out_at + col, v);
                         tmem_ld_wait();
@@ -504,22 +517,23 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             }
             const uint64_t off = pair(more - against, more - against), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
-            // Weights of 32 keys go where their scores lay: 16 columns, and of fp32 16 of their rests.
-            auto weights = [&](const uint32_t (&sc)[32], uint32_t to) {
-                uint32_t hi[16], lo[16];
+            // Weights: of 16-bit types 16 columns where the first half's scores lay, which both warps have read; of fp32 16 and as many of their rests
+            // where their own scores lay.
+            const uint32_t to = at + half * (F::kParts == 2 ? 32 : 16);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[i]), __uint_as_float(sc[i + 1])), cc, off));
+            for (int part = 0; part < 2; ++part) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[part * 16 + i]), __uint_as_float(sc[part * 16 + i + 1])), cc, off));
                     const float p = exp2_approx(x.x), q = exp2_approx(x.y);
                     sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
                     if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
                     else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
                 }
-                tmem_st_32x32b_x16(to, hi);
-                if constexpr (F::kParts == 2) tmem_st_32x32b_x16(to + 16, lo);
-            };
-            weights(s0, at);
-            weights(s1, at + (F::kParts == 2 ? 32 : 16));
+                tmem_st_32x32b_x8(to + part * 8, hi);
+                if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16 + part * 8, lo);
+            }
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -528,23 +542,27 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             l = fmaf(sums.x + sums.y, back, l);
             ++n;
         }
-        // A barrier's wait tells a phase from the one before it alone, and here the last two products may be done or under way: a barrier of its own.
-        const bool done = n > 0 && mbar_wait_warp(smem_u32(&bar.all_done), 0, &s_abort);
+        const bool done = n > 0 && mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
+        float other_l = 0.f;
+        exchange(l, other_l);
+        l += other_l;
         const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         add_chunk(done, norm);
         if (shares > 1) {
-            s_m[tid] = m;
-            s_l[tid] = l;
-        } else {   // the warp's rows, whole lines at a time
+            if (half == 0) {
+                s_m[r] = m;
+                s_l[r] = l;
+            }
+        } else {   // the warp's columns of its rows, whole lines (of fp32) at a time
             __syncwarp();
-            constexpr uint32_t kPerO = DP / 4;
-            const uint32_t c = lane % kPerO;
+            constexpr uint32_t kPerO = kCols / 4;
+            const uint32_t c4 = half * kPerO + lane % kPerO;
 #pragma unroll 4
-            for (uint32_t r = lane / kPerO; r < 32; r += 32 / kPerO)
-                if (warp_row + r < n_rows && c * 4 < dim) write_row(warp_row + r, c * 4, s_o[out_place(warp_row + r, c)]);
+            for (uint32_t i = lane / kPerO; i < 32; i += 32 / kPerO)
+                if (warp_row + i < n_rows && c4 * 4 < dim) write_row(warp_row + i, c4 * 4, s_o[out_place(warp_row + i, c4)]);
         }
-    } else if (warp < 8 * RT) {
+    } else if (warp < 12 * RT) {
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
         auto publish = [&](uint32_t job) {
@@ -614,88 +632,91 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-        // ---------------------------------------------------------------- the tensor core's instructions, a warp for each tile of rows
+        // ---------------------------------------------------------------- the tensor core's instructions
+        // A warp for the scores of each tile of rows, another for its products: what a tile costs such a warp - looking at barriers, issuing, committing -
+        // is as long as the tensor core's work, and the two need not wait for one another.  All waits but the queries' are for the barriers of every other
+        // tile, whose next phase cannot end before this one has been seen.
         regs_down<F::kIssueRegs>();
-        const uint32_t rt = warp - 8 * RT;
-        if (rt < RT) {
-            RowBars& bar = s_row[rt];
-            const Seen sees = rows_see(rt);
-            const uint32_t my_tmem = tmem + rt * 256u, k_steps = (dim + 15) / 16;
-            auto scores = [&](uint32_t j, uint32_t n) {   // S = Q K^T, the small products first
-                const uint32_t d = my_tmem + F::kScores + (n & 1u) * kKeys, at = smem_at + 2 * j % kSlots * F::kTile;
-                const uint32_t idesc = idesc_f16<T>(kKeys);
-                uint32_t more = 0;
-#pragma unroll
-                for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
-                    const uint32_t qa = my_tmem + F::kQuery + (term == 1 ? DP / 2 : 0);
-                    const uint32_t kb = at + (term == 0 ? F::kPanels * kPanel : 0);
-                    for (uint32_t s = 0; s < k_steps; ++s) {
-                        umma_f16_ts(d, qa + s * 8, umma_desc_k_sw128(kb + (s / 4) * kPanel + (s % 4) * 32), idesc, more);
-                        more = 1;
-                    }
+        const uint32_t rt = (warp - 12 * RT) % RT, role = (warp - 12 * RT) / RT;
+        RowBars& bar = s_row[rt];
+        const Seen sees = rows_see(rt);
+        const uint32_t my_tmem = tmem + rt * 256u;
+        auto wait_full = [&](uint32_t job) { return mbar_wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
+        auto hand_back = [&](uint32_t job) {   // unread
+            const bool ok = wait_full(job);
+            if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty_bar[job % kSlots]));
+            return ok;
+        };
+        uint32_t n = 0;   // tiles that these rows see, so far
+        if (role == 0) {
+            const uint32_t k_steps = (dim + 15) / 16, idesc = idesc_f16<T>(kKeys);
+            bool ok = mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort);
+            for (uint32_t j = 0; ok && j < tiles; ++j) {
+                if (!sees(t0 + j)) {
+                    ok = hand_back(2 * j);
+                    continue;
                 }
-            };
-            auto product = [&](uint32_t j, uint32_t n) {
-                const uint32_t p = my_tmem + F::kScores + (n & 1u) * kKeys, at = smem_at + (2 * j + 1) % kSlots * F::kTile;
-#pragma unroll
-                for (int panel = 0; panel < F::kPanels; ++panel) {
-                    const uint32_t left = dim - panel * 64u, cols = left >= 64 ? 64 : (left + 15) / 16 * 16;
-                    const uint32_t idesc = idesc_f16<T>(cols) | kIdescColumnMajorB;
-                    uint32_t more = F::kSums ? n % kChunk != 0 : n > 0;
-#pragma unroll
-                    for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
-                        const uint32_t pa = p + (term == 1 ? 16 : 0), vb = at + (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel;
-#pragma unroll
-                        for (uint32_t s = 0; s < 4; ++s) {
-                            umma_f16_ts(my_tmem + F::kProduct + panel * 64, pa + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), desc_rows(vb + s * 2048), idesc, more);
-                            more = 1;
-                        }
-                    }
-                }
-            };
-            auto wait_full = [&](uint32_t job) { return mbar_wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
-            uint32_t n_s = 0, n_p = 0;   // scores and products so far, of the tiles that these rows see
-            auto issue_scores = [&](uint32_t j) -> bool {
-                // They go where the weights of the last tile but one lie, so its product has to be done.  Waited for is the last product issued, that one or
-                // the one behind it: of an older phase the barrier could not tell whether it is over.
-                if (n_p > 0 && !mbar_wait_warp(smem_u32(&bar.pv_full), (n_p - 1) & 1u, &s_abort)) return false;
-                if (!wait_full(2 * j)) return false;
+                // S = Q K^T goes where the weights of the tile before the last lie: its product has to be done
+                if (n > 1) ok = mbar_wait_warp(smem_u32(&bar.done[n & 1u]), ((n >> 1) - 1) & 1u, &s_abort);
+                ok = ok && wait_full(2 * j);
+                if (!ok) break;
                 tc_fence_after_sync();
-                if (elect_one()) {
-                    scores(j, n_s);
-                    umma_commit(smem_u32(&bar.s_full[n_s & 1u]));
+                if (elect_one()) {   // the small products first
+                    const uint32_t d = my_tmem + F::kScores + (n & 1u) * kKeys;
+                    const uint64_t keys = umma_desc_k_sw128(smem_at + 2 * j % kSlots * F::kTile);
+                    auto issue = [&](uint32_t steps) {
+#pragma unroll
+                        for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+#pragma unroll
+                            for (uint32_t s = 0; s < DP / 16; ++s) {
+                                if (s >= steps) break;
+                                const uint32_t at = (term == 0 ? F::kPanels * kPanel : 0) + s / 4 * kPanel + s % 4 * 32;
+                                umma_f16_ts(d, my_tmem + F::kQuery + (term == 1 ? DP / 2 : 0) + s * 8, keys + (at >> 4), idesc, term != (F::kParts == 2 ? 0 : 2) || s > 0);
+                            }
+                        }
+                    };
+                    if (k_steps == DP / 16) issue(DP / 16);
+                    else issue(k_steps);
+                    umma_commit(smem_u32(&bar.s_full[n & 1u]));
                     umma_commit(smem_u32(&s_empty_bar[2 * j % kSlots]));
                 }
                 __syncwarp();
-                ++n_s;
-                return true;
-            };
-            const uint32_t last = sees.last(t0, t1);
-            bool ok = mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort), ahead = false;
+                ++n;
+            }
+        } else if (role == 1) {
+            uint32_t idescs[F::kPanels];
+#pragma unroll
+            for (int panel = 0; panel < F::kPanels; ++panel) idescs[panel] = idesc_f16<T>((min(dim - panel * 64u, 64u) + 15) / 16 * 16) | kIdescColumnMajorB;
+            bool ok = true;
             for (uint32_t j = 0; ok && j < tiles; ++j) {
-                if (!sees(t0 + j)) {   // handed back unread
-                    ok = wait_full(2 * j) && wait_full(2 * j + 1);
-                    if (ok && lane == 0) {
-                        mbar_arrive(smem_u32(&s_empty_bar[2 * j % kSlots]));
-                        mbar_arrive(smem_u32(&s_empty_bar[(2 * j + 1) % kSlots]));
-                    }
+                if (!sees(t0 + j)) {
+                    ok = hand_back(2 * j + 1);
                     continue;
                 }
-                if (!ahead) ok = issue_scores(j);
-                ahead = j + 1 < tiles && sees(t0 + j + 1);
-                if (ok && ahead) ok = issue_scores(j + 1);   // while this tile's weights are formed
-                ok = ok && mbar_wait_warp(smem_u32(&bar.p_full[n_p & 1u]), (n_p >> 1) & 1u, &s_abort);
-                ok = ok && wait_full(2 * j + 1);
+                ok = wait_full(2 * j + 1) && mbar_wait_warp(smem_u32(&bar.p_full[n & 1u]), (n >> 1) & 1u, &s_abort);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
-                    product(j, n_p);
-                    umma_commit(smem_u32(&bar.pv_full));
-                    if (t0 + j == last) umma_commit(smem_u32(&bar.all_done));
+                    const uint32_t p = my_tmem + F::kScores + (n & 1u) * kKeys;
+                    const uint64_t values = desc_rows(smem_at + (2 * j + 1) % kSlots * F::kTile);
+                    const uint32_t go_on = F::kSums ? n % kChunk != 0 : n > 0;
+#pragma unroll
+                    for (int panel = 0; panel < F::kPanels; ++panel) {
+#pragma unroll
+                        for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+#pragma unroll
+                            for (uint32_t s = 0; s < 4; ++s) {
+                                const uint32_t at = (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel + s * 2048;
+                                umma_f16_ts(my_tmem + F::kProduct + panel * 64, p + (term == 1 ? 16 : 0) + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), values + (at >> 4),
+                                            idescs[panel], term != (F::kParts == 2 ? 0 : 2) || s > 0 ? 1u : go_on);
+                            }
+                        }
+                    }
+                    umma_commit(smem_u32(&bar.done[n & 1u]));
                     umma_commit(smem_u32(&s_empty_bar[(2 * j + 1) % kSlots]));
                 }
                 __syncwarp();
-                ++n_p;
+                ++n;
             }
         }
     }
@@ -741,12 +762,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == 8 * RT && s_abort) {   // what is in flight gets time to end before its columns are handed back
+    if (warp == 12 * RT && s_abort) {   // what is in flight gets time to end before its columns are handed back
         const long long from = clock64();
         while (clock64() - from < 200000) {}
         if (lane == 0) report_error(dev_err, 7);
     }
-    if (warp == 8 * RT) tmem_dealloc(tmem, F::kColumns);
+    if (warp == 12 * RT) tmem_dealloc(tmem, F::kColumns);
 }
 
 template <typename T, int DP, int RT>
