@@ -86,6 +86,23 @@ __device__ __forceinline__ void sync_128(uint32_t id) { asm volatile("barrier.ct
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
 // The power of two that takes a largest value to 8 .. 16, up to 2^108 (results below 1e-32 have fewer bits); 0 for 0.
 __device__ __forceinline__ int exponent_for(uint32_t top_bits) { return top_bits == 0 ? 0 : min(108, 130 - (int)(top_bits >> 23)); }
+// A warp's bounded wait, with one answer.  The hint lets the hardware hold a waiting warp for up to two microseconds a look: without it the fifteen warps
+// of a CTA that wait for one another took a third of all instructions.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word) {
+    uint32_t ok = 0;
+    for (uint32_t it = 0; it < 1u << 18; ++it) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if (*abort_word) return false;
+    }
+    *abort_word = 1u;
+    return false;
+}
+
 // Two fp32 operations an instruction.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -223,22 +240,29 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     const uint32_t jobs = 2 * tiles;
     // No early way out of the loops: the four warps meet at a barrier for every tile of fp32.
     auto copy = [&](uint32_t job) {   // this thread's part of a tile, on its way to the job's slot once that is free
-        if (job >= kSlots) mbar_wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
+        if (job >= kSlots) wait_warp(smem_u32(&s_empty_bar[job % kSlots]), (job / kSlots - 1) & 1u, &s_abort);
         int32_t k0, end;
         tile_keys(t0 + job / 2, k0, end);
         const bool values = job & 1u;
         const int64_t token = values ? a.v_token : a.k_token;
         const T* base = values ? static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head
                                : static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
-        const int32_t key0 = k0 + (int32_t)my_row;
-        const T* from = base + (int64_t)key0 * token + my_col;
+        const T* from = base + (int64_t)(k0 + (int32_t)my_row) * token + (in_dim ? my_col : 0);
+        const int64_t step = token * kStepRows;
         const uint32_t at = smem_at + job % kSlots * F::kTile;
+        auto to = [&](int i) -> uint32_t { return at + (F::kParts == 2 ? i * 2048 + t * 16 : place_of(i)); };   // (fp32: to where this thread alone reads it)
+        if ((uint32_t)k0 + kKeys <= (uint32_t)end && (k0 >= gap_to || (uint32_t)k0 + kKeys <= (uint32_t)gap_from)) {
+            const uint32_t size = in_dim ? 16u : 0u;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const int32_t key = key0 + i * kStepRows;
-            const bool in = in_dim && key < end && (key < gap_from || key >= gap_to);
-            const uint32_t to = at + (F::kParts == 2 ? i * 2048 + t * 16 : place_of(i));   // (fp32: to where this thread alone reads it)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? from + i * kStepRows * token : base), "r"(in ? 16 : 0) : "memory");
+            for (int i = 0; i < kPerThread; ++i, from += step)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to(i)), "l"(from), "r"(size) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i, from += step) {
+                const int32_t key = k0 + (int32_t)my_row + i * kStepRows;
+                const bool in = in_dim && key < end && (key < gap_from || key >= gap_to);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to(i)), "l"(in ? from : base), "r"(in ? 16 : 0) : "memory");
+            }
         }
     };
 
@@ -312,7 +336,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.halves[warp & 3u]));
-            const bool ok = mbar_wait_warp(smem_u32(&bar.halves[warp & 3u]), exchanges & 1u, &s_abort);
+            const bool ok = wait_warp(smem_u32(&bar.halves[warp & 3u]), exchanges & 1u, &s_abort);
             tc_fence_after_sync();
             theirs = s_half[exchanges & 1u][half ^ 1u][r];
             ++exchanges;
@@ -368,7 +392,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.q_full));
         } else if (F::kParts == 2) {
-            if (mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort)) factor = s_factor[r];
+            if (wait_warp(smem_u32(&bar.q_full), 0, &s_abort)) factor = s_factor[r];
         } else if (a.scale == 0.f) {
             factor = 1.f;
         }
@@ -377,6 +401,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         // All rows see all of a tile that lies between these.
         const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
         const int32_t common_hi = key_bounds(a, first + per_head(r0 + r_first), length).hi, common_lo = key_bounds(a, first + per_head(r0 + max(r_last, r_first)), length).lo;
+        // ... the tiles full_from .. full_to - 1
+        const uint32_t full_from = sink_tiles + (uint32_t)max(0, (common_lo - span.lo + kKeys - 1) / kKeys);
+        const uint32_t full_to = sink_tiles + (uint32_t)max(0, (min(span.hi, common_hi) - span.lo) / kKeys);
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
         const uint32_t out_at = my_tmem + F::kProduct;
         // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is in shared memory, against m_o
@@ -411,8 +438,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         };
         uint32_t n = 0;   // tiles so far
         for (uint32_t j = 0; j < tiles; ++j) {
-            if (!sees(t0 + j)) continue;
-            if (!mbar_wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
+            if (RT == 2 && !sees(t0 + j)) continue;
+            if (!wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
             if (warp_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
                 if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
@@ -424,7 +451,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if constexpr (F::kSums) {
                 begun = n % kChunk != 0;
                 if (n > 0 && !begun) {
-                    if (!mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
+                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     add_chunk(true, 1.f);
                 }
@@ -434,17 +461,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if constexpr (F::kParts == 2) {
                 c *= power2(-s_exp_k[j % 8]);
                 // the values' power of two is known once they are in shared memory, which the keys' turn does not wait for
-                if (!mbar_wait_warp(smem_u32(&s_full_bar[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
+                if (!wait_warp(smem_u32(&s_full_bar[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
                 e = s_exp_v[j % 8];
             }
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
-            int32_t k0, end;
-            tile_keys(t0 + j, k0, end);
             uint32_t sc[32];
             tmem_ld_32x32b_x32(at + half * 32, sc);
             tmem_ld_wait();
-            k0 += half * 32;
-            if (!((int64_t)k0 + 32 <= min(end, common_hi) && (k0 >= common_lo || (int64_t)k0 + 32 <= (int64_t)a.sinks))) {
+            if (t0 + j < full_from || t0 + j >= full_to) {
+                int32_t k0, end;
+                tile_keys(t0 + j, k0, end);
+                k0 += half * 32;
                 const uint32_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -471,7 +498,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 const float m_new = top > m + kSlack ? top : m;
                 const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
                 if (begun) {
-                    if (!mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
+                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
                     tc_fence_after_sync();
                     float f = shrink;
                     if constexpr (F::kParts == 2) {
@@ -542,7 +569,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             l = fmaf(sums.x + sums.y, back, l);
             ++n;
         }
-        const bool done = n > 0 && mbar_wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
+        const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
         float other_l = 0.f;
         exchange(l, other_l);
@@ -641,7 +668,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         RowBars& bar = s_row[rt];
         const Seen sees = rows_see(rt);
         const uint32_t my_tmem = tmem + rt * 256u;
-        auto wait_full = [&](uint32_t job) { return mbar_wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
+        auto wait_full = [&](uint32_t job) { return wait_warp(smem_u32(&s_full_bar[job % kSlots]), (job / kSlots) & 1u, &s_abort); };
         auto hand_back = [&](uint32_t job) {   // unread
             const bool ok = wait_full(job);
             if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty_bar[job % kSlots]));
@@ -650,14 +677,14 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         uint32_t n = 0;   // tiles that these rows see, so far
         if (role == 0) {
             const uint32_t k_steps = (dim + 15) / 16, idesc = idesc_f16<T>(kKeys);
-            bool ok = mbar_wait_warp(smem_u32(&bar.q_full), 0, &s_abort);
+            bool ok = wait_warp(smem_u32(&bar.q_full), 0, &s_abort);
             for (uint32_t j = 0; ok && j < tiles; ++j) {
                 if (!sees(t0 + j)) {
                     ok = hand_back(2 * j);
                     continue;
                 }
                 // S = Q K^T goes where the weights of the tile before the last lie: its product has to be done
-                if (n > 1) ok = mbar_wait_warp(smem_u32(&bar.done[n & 1u]), ((n >> 1) - 1) & 1u, &s_abort);
+                if (n > 1) ok = wait_warp(smem_u32(&bar.done[n & 1u]), ((n >> 1) - 1) & 1u, &s_abort);
                 ok = ok && wait_full(2 * j);
                 if (!ok) break;
                 tc_fence_after_sync();
@@ -693,7 +720,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     ok = hand_back(2 * j + 1);
                     continue;
                 }
-                ok = wait_full(2 * j + 1) && mbar_wait_warp(smem_u32(&bar.p_full[n & 1u]), (n >> 1) & 1u, &s_abort);
+                ok = wait_full(2 * j + 1) && wait_warp(smem_u32(&bar.p_full[n & 1u]), (n >> 1) & 1u, &s_abort);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
