@@ -51,13 +51,17 @@ struct Form {
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
     static_assert(RT == 1 || kUsed <= 256);
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
-    // Warpgroups: two for each tile of rows, one with the first 32 keys of a tile and one with the others, one for each that loads, one that issues.
-    // Registers a thread of each; their sum is what the warpgroups are launched with.
-    static constexpr int kThreads = (3 * RT + 1) * 128;
-    static constexpr int kLaunchRegs = RT == 2 ? 72 : DP <= 64 ? 64 : 128;
-    static constexpr int kRowRegs = DP > 64 ? 152 : RT == 2 || sizeof(T) == 4 ? 80 : 88, kLoadRegs = DP > 64 ? 128 : RT == 2 ? 72 : sizeof(T) == 4 ? 56 : 40;
-    static constexpr int kIssueRegs = DP > 64 ? 80 : 40;
-    static_assert(RT * (2 * kRowRegs + kLoadRegs) + kIssueRegs == (3 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
+    // Threads of a row: of fp32 two, in two warps, each with half the keys of a tile; of 16-bit types, whose weights take less, one (8192 tokens in bf16 with two
+    // 106 us).  Warpgroups: one for each of them and each tile of rows, one for each tile of rows that loads, one that issues.  Registers a thread of each; their
+    // sum is what the warpgroups are launched with.
+    static constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kRowWarps = 4 * RT * kHalves, kLoadWarps = 4 * RT, kIssueAt = kRowWarps + kLoadWarps;
+    static constexpr int kThreads = (kIssueAt + 4) * 32;
+    static constexpr int kLaunchRegs = kHalves == 1 ? (DP > 64 ? 168 : 80) : RT == 2 ? 72 : DP <= 64 ? 64 : 128;
+    static constexpr int kRowRegs = kHalves == 1 ? (DP > 64 ? 232 : 152) : DP > 64 ? 152 : 80;
+    static constexpr int kLoadRegs = kHalves == 1 ? (DP > 64 ? 136 : 64) : DP > 64 ? 128 : RT == 2 ? 72 : 56;
+    static constexpr int kIssueRegs = kHalves == 1 ? (DP > 64 ? 136 : 24) : DP > 64 ? 80 : 40;
+    static_assert(RT * (kHalves * kRowRegs + kLoadRegs) + kIssueRegs == (RT * (kHalves + 1) + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
 };
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -226,7 +230,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     };
 
     // ---- what loads keys and values: warpgroup wg of them (with two, one loads keys, one values)
-    const uint32_t t = tid & 127u, wg = warp / 4 - 2 * RT;
+    const uint32_t t = tid & 127u, wg = warp / 4 - RT * F::kHalves;
     // A thread copies pieces of 16 bytes: of one column, kStepRows rows apart, so that neighbours copy whole rows.
     constexpr int kElems = kPer16<T>, kPerRow = DP / kElems, kStepRows = 128 / kPerRow, kPerThread = kKeys / kStepRows;
     const uint32_t my_row = t / kPerRow, my_col = t % kPerRow * kElems;
@@ -269,8 +273,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
     // lines; then a thread has its own row.
     constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
-    const uint32_t warp_row = warp / 8 * kRows + (warp & 3u) * 32u, half = warp / 4 & 1u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
-    if (warp < 8 * RT) {
+    constexpr uint32_t kHalves = F::kHalves;
+    const uint32_t warp_row = warp / (4 * kHalves) * kRows + (warp & 3u) * 32u, half = kHalves == 2 ? warp / 4 & 1u : 0u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
+    if (warp < F::kRowWarps) {
       if (half == 0) {
         const uint32_t c = lane % kPerQ;
         const bool in_row = c * kPer16<T> < dim;
@@ -283,22 +288,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + q_stage + (r * kPerQ + (c ^ (r & (kPerQ - 1)))) * 16), "l"(p), "r"(in ? 16 : 0) : "memory");
         }
       }
-    } else if (warp < 12 * RT) {
+    } else if (warp < F::kIssueAt) {
         for (uint32_t i = 0; i < F::kAhead; ++i) {
             if (wg + i * RT < jobs) copy(wg + i * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-    } else if (warp == 12 * RT) {
+    } else if (warp == F::kIssueAt) {
         tmem_alloc(smem_u32(&s_tmem), F::kColumns);
         tmem_relinquish();
-    } else if (warp == 12 * RT + 1) {
+    } else if (warp == F::kIssueAt + 1) {
         if (lane < kSlots) mbar_init(smem_u32(&s_full_bar[lane]), 4);
         if (lane < kSlots) mbar_init(smem_u32(&s_empty_bar[lane]), RT);
         if (lane < RT) {
             RowBars& bar = s_row[lane];
             for (int i = 0; i < 2; ++i) {
                 mbar_init(smem_u32(&bar.s_full[i]), 1);
-                mbar_init(smem_u32(&bar.p_full[i]), 8);
+                mbar_init(smem_u32(&bar.p_full[i]), 4 * kHalves);
                 mbar_init(smem_u32(&bar.done[i]), 1);
             }
             for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar.halves[i]), 2);
@@ -320,10 +325,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
     };
 
-    if (warp < 8 * RT) {
-        // ---------------------------------------------------------------- a row for two threads, in two warps: half the keys of a tile each
+    if (warp < F::kRowWarps) {
+        // ---------------------------------------------------------------- a row a thread, or for two in two warps, half the keys of a tile each
         regs_up<F::kRowRegs>();
-        const uint32_t rt = warp / 8, lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
+        const uint32_t rt = warp / (4 * kHalves), lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
         RowBars& bar = s_row[rt];
         const uint32_t my_tmem = tmem + rt * 256u + lanes;
         const uint32_t row = r0 + min(r, n_rows - 1), qi = per_head(row);
@@ -396,7 +401,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         } else if (a.scale == 0.f) {
             factor = 1.f;
         }
-        constexpr uint32_t kCols = DP / 2;   // of the output, a warp's
+        constexpr uint32_t kCols = DP / kHalves;   // of the output, a warp's
         const uint32_t col0 = half * kCols;
         // All rows see all of a tile that lies between these.
         const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
@@ -465,30 +470,39 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 e = s_exp_v[j % 8];
             }
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
-            uint32_t sc[32];
-            tmem_ld_32x32b_x32(at + half * 32, sc);
+            constexpr int kMine = 2 / (int)kHalves;   // groups of 32 keys
+            uint32_t sc[kMine][32];
+#pragma unroll
+            for (int g = 0; g < kMine; ++g) tmem_ld_32x32b_x32(at + (half + g) * 32, sc[g]);
             tmem_ld_wait();
             if (t0 + j < full_from || t0 + j >= full_to) {
                 int32_t k0, end;
                 tile_keys(t0 + j, k0, end);
-                k0 += half * 32;
-                const uint32_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (!(seen >> i & 1u)) sc[i] = 0xFF800000u;
+                for (int g = 0; g < kMine; ++g) {
+                    const uint32_t bits = (uint32_t)(seen >> 32 * (half + g));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(bits >> i & 1u)) sc[g][i] = 0xFF800000u;
+                }
             }
             float top;
             {
                 float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    x = max3(x, __uint_as_float(sc[i]), __uint_as_float(sc[i + 1]));
-                    y = max3(y, __uint_as_float(sc[i + 2]), __uint_as_float(sc[i + 3]));
-                }
+                for (int g = 0; g < kMine; ++g)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        x = max3(x, __uint_as_float(sc[g][i]), __uint_as_float(sc[g][i + 1]));
+                        y = max3(y, __uint_as_float(sc[g][i + 2]), __uint_as_float(sc[g][i + 3]));
+                    }
                 top = fmaxf(x, y) * c;
-                float other;
-                if (!exchange(top, other)) break;
-                top = fmaxf(top, other);
+                if constexpr (kHalves == 2) {
+                    float other;
+                    if (!exchange(top, other)) break;
+                    top = fmaxf(top, other);
+                }
             }
             // Another maximum, or another power of two of the values: the output so far is brought in line, where there is one.
             float more = kBoost;   // log2 of what this tile's weights carry
@@ -511,9 +525,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                             for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
                         }
-                        float other;
-                        if (!exchange(big, other)) break;
-                        big = fmaxf(big, other);
+                        if constexpr (kHalves == 2) {
+                            float other;
+                            if (!exchange(big, other)) break;
+                            big = fmaxf(big, other);
+                        }
                         // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
                         const int x = max(-120, min(120, e - unit));
                         if (x <= 0 || big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2))) {
@@ -544,22 +560,24 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             }
             const uint64_t off = pair(more - against, more - against), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
-            // Weights: of 16-bit types 16 columns where the first half's scores lay, which both warps have read; of fp32 16 and as many of their rests
-            // where their own scores lay.
-            const uint32_t to = at + half * (F::kParts == 2 ? 32 : 16);
+            // Weights of 32 keys: of 16-bit types 16 columns, of fp32, where their own scores lay, 16 and as many of their rests.
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                uint32_t hi[8], lo[8];
+            for (int g = 0; g < kMine; ++g) {
+                const uint32_t to = at + (half + g) * (F::kParts == 2 ? 32 : 16);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float2 x = unpair(fma2(pair(__uint_as_float(sc[part * 16 + i]), __uint_as_float(sc[part * 16 + i + 1])), cc, off));
-                    const float p = exp2_approx(x.x), q = exp2_approx(x.y);
-                    sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
-                    if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
-                    else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 x = unpair(fma2(pair(__uint_as_float(sc[g][part * 16 + i]), __uint_as_float(sc[g][part * 16 + i + 1])), cc, off));
+                        const float p = exp2_approx(x.x), q = exp2_approx(x.y);
+                        sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
+                        if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
+                        else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
+                    }
+                    tmem_st_32x32b_x8(to + part * 8, hi);
+                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16 + part * 8, lo);
                 }
-                tmem_st_32x32b_x8(to + part * 8, hi);
-                if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16 + part * 8, lo);
             }
             tmem_st_wait();
             tc_fence_before_sync();
@@ -571,9 +589,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
-        float other_l = 0.f;
-        exchange(l, other_l);
-        l += other_l;
+        if constexpr (kHalves == 2) {
+            float other = 0.f;
+            exchange(l, other);
+            l += other;
+        }
         const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         add_chunk(done, norm);
         if (shares > 1) {
@@ -589,7 +609,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             for (uint32_t i = lane / kPerO; i < 32; i += 32 / kPerO)
                 if (warp_row + i < n_rows && c4 * 4 < dim) write_row(warp_row + i, c4 * 4, s_o[out_place(warp_row + i, c4)]);
         }
-    } else if (warp < 12 * RT) {
+    } else if (warp < F::kIssueAt) {
         // ---------------------------------------------------------------- keys and values into shared memory
         regs_down<F::kLoadRegs>();
         auto publish = [&](uint32_t job) {
@@ -664,7 +684,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         // is as long as the tensor core's work, and the two need not wait for one another.  All waits but the queries' are for the barriers of every other
         // tile, whose next phase cannot end before this one has been seen.
         regs_down<F::kIssueRegs>();
-        const uint32_t rt = (warp - 12 * RT) % RT, role = (warp - 12 * RT) / RT;
+        const uint32_t rt = (warp - F::kIssueAt) % RT, role = (warp - F::kIssueAt) / RT;
         RowBars& bar = s_row[rt];
         const Seen sees = rows_see(rt);
         const uint32_t my_tmem = tmem + rt * 256u;
@@ -789,12 +809,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == 12 * RT && s_abort) {   // what is in flight gets time to end before its columns are handed back
+    if (warp == F::kIssueAt && s_abort) {   // what is in flight gets time to end before its columns are handed back
         const long long from = clock64();
         while (clock64() - from < 200000) {}
         if (lane == 0) report_error(dev_err, 7);
     }
-    if (warp == 12 * RT) tmem_dealloc(tmem, F::kColumns);
+    if (warp == F::kIssueAt) tmem_dealloc(tmem, F::kColumns);
 }
 
 template <typename T, int DP, int RT>
