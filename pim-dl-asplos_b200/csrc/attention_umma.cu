@@ -1,24 +1,25 @@
 // Attention for many rows, on the tensor cores:  out = softmax(scale q k^T) v  over the keys that a query sees (attention.cuh).
 //
-// A CTA takes 128 rows - query tokens times the query heads that share a key head - of one sequence through the keys that any of
-// them sees, 64 keys a tile: first the tiles of the sinks, then those of the window; tiles in between are never loaded.  With S = Q K^T
-// (tcgen05.mma, queries in tensor memory, keys in shared memory) in tensor memory, a thread owns a row: it reads the 64 scores,
-// keeps the running maximum m and sum l, and writes p = exp2(s - m) back over S, where the next product P V reads it as its operand;
-// the sum of the tiles' products, rescaled by exp2(m_old - m_new), stays in the thread's registers.  What is exchanged between
-// threads is two barriers a tile.  While a tile's weights are formed, the tensor core works on the next tile's scores and the last
-// tile's product: S is double, and two CTAs share an SM where head_dim is at most 64.
+// A CTA takes 128 rows - query tokens times the query heads that share a key head - or, of fp32, twice 128, of one sequence through the keys that
+// any of them sees, 64 keys a tile: first the tiles of the sinks, then those of the window; tiles in between are never loaded.  Scores S = Q K^T
+// (tcgen05.mma, queries in tensor memory, keys in shared memory) go to tensor memory, where a thread owns a row: it reads the 64 scores, takes the
+// largest, and writes weights p = exp2(s - m) back over S, where the next product P V reads them as its operand; their sum l stays with the thread.  The
+// output stays in tensor memory, too.  It is brought in line, multiplied by exp2(m_old - m), only where a row's maximum has grown by 2^8: until then
+// weights are formed against the old m.  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
-// Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.
-// fp32 operands are split into two f16 numbers, x = hi + lo to 22 bits, and hi hi + hi lo + lo hi is summed; the product of the rests, 2^-22
-// of the whole, is left out.  f16 ends at 65504 and thins out below 2^-14, so operands carry a power of two: queries one per row, keys
-// and values one per tile, kept from tile to tile for as long as the tile's largest value lies in 1/4 .. 32768 under it; the loading
-// warps look at that while they convert, and convert a tile once more where it does not.  Weights carry 2^14, the sum l with
-// them.  Maxima, sums and outputs are fp32.
+// Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.  fp32 operands are split into
+// two f16 numbers, x = hi + lo to 22 bits, and hi hi + hi lo + lo hi is summed; the product of the rests, 2^-22 of the whole, is left out.  f16 ends at
+// 65504 and thins out below 2^-14, so operands carry a power of two: queries one per row, keys and values one per tile, kept from tile to tile for as long
+// as the tile's largest value lies in 1/4 .. 32768 under it.  Weights carry 2^6 and up to 2^8 more, the sum l with them.  Maxima, sums and outputs
+// are fp32; the rescaling of the output in tensor memory, and the sum over tiles that fp32 takes out of it (kChunk), round once each.
 //
-// The loading warps read global memory with plain 16-byte loads: no tensor maps, and rows behind the last key become zeros.  Tensors that
-// do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.
-// Where there are few CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no
-// scratch memory and one order of summation.
+// Loading warps copy 16 bytes a piece (cp.async): no tensor maps to be made by the host, and rows behind the last key become zeros.  fp32 is
+// converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
+// CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no scratch memory and one order of summation.
+//
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 98 us, 350 TFLOP/s; of 2900 warp instructions a
+// tile 680 form its weights.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 32 us, 540 TFLOP/s.  fp32,
+// three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 96 us, of which a CTA spends half before its first and behind its last tile.
 #include "attention.cuh"
 #include "ptx.cuh"
 
@@ -51,17 +52,12 @@ struct Form {
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
     static_assert(RT == 1 || kUsed <= 256);
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
-    // Threads of a row: of fp32 two, in two warps, each with half the keys of a tile; of 16-bit types, whose weights take less, one (8192 tokens in bf16 with two
-    // 106 us).  Warpgroups: one for each of them and each tile of rows, one for each tile of rows that loads, one that issues.  Registers a thread of each; their
-    // sum is what the warpgroups are launched with.
-    static constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int kRowWarps = 4 * RT * kHalves, kLoadWarps = 4 * RT, kIssueAt = kRowWarps + kLoadWarps;
-    static constexpr int kThreads = (kIssueAt + 4) * 32;
-    static constexpr int kLaunchRegs = kHalves == 1 ? (DP > 64 ? 168 : 80) : RT == 2 ? 72 : DP <= 64 ? 64 : 128;
-    static constexpr int kRowRegs = kHalves == 1 ? (DP > 64 ? 232 : 152) : DP > 64 ? 152 : 80;
-    static constexpr int kLoadRegs = kHalves == 1 ? (DP > 64 ? 136 : 64) : DP > 64 ? 128 : RT == 2 ? 72 : 56;
-    static constexpr int kIssueRegs = kHalves == 1 ? (DP > 64 ? 136 : 24) : DP > 64 ? 80 : 40;
-    static_assert(RT * (kHalves * kRowRegs + kLoadRegs) + kIssueRegs == (RT * (kHalves + 1) + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
+    // Warpgroups: one for each tile of rows, a row a thread, one for each tile of rows that loads, one that issues.  Registers a thread of each; their sum is
+    // what the warpgroups are launched with.
+    static constexpr int kRowWarps = 4 * RT, kIssueAt = 8 * RT, kThreads = (2 * RT + 1) * 128;
+    static constexpr int kLaunchRegs = DP > 64 ? 168 : RT == 2 ? 96 : 80, kRowRegs = DP > 64 ? 232 : 152, kLoadRegs = DP > 64 ? 136 : RT == 2 ? 72 : 64;
+    static constexpr int kIssueRegs = DP > 64 ? 136 : RT == 2 ? 32 : 24;
+    static_assert(RT * (kRowRegs + kLoadRegs) + kIssueRegs == (2 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
 };
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -158,7 +154,7 @@ __device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint3
 __device__ __forceinline__ uint64_t below(int64_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 struct RowBars {   // of a tile of rows
-    uint64_t s_full[2], p_full[2], done[2], q_full, halves[4];   // scores, weights and products of every other tile; queries; a row's two warps
+    uint64_t s_full[2], p_full[2], done[2], q_full;   // scores, weights and products of every other tile; queries
 };
 
 // Which of the CTA's tiles of keys a tile of rows sees any of: the sinks', and from .. to - 1.
@@ -188,7 +184,6 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     __shared__ __align__(8) RowBars s_row[RT];
     __shared__ uint32_t s_tmem, s_abort, s_top[RT][3][4];
     __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most four tiles ahead of who reads these
-    __shared__ float s_half[2][2][RT * kRows], s_factor[RT * kRows];   // what the two warps of a row tell one another
     __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_part[kMostShares][RT * kRows];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
@@ -230,7 +225,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     };
 
     // ---- what loads keys and values: warpgroup wg of them (with two, one loads keys, one values)
-    const uint32_t t = tid & 127u, wg = warp / 4 - RT * F::kHalves;
+    const uint32_t t = tid & 127u, wg = warp / 4 - RT;
     // A thread copies pieces of 16 bytes: of one column, kStepRows rows apart, so that neighbours copy whole rows.
     constexpr int kElems = kPer16<T>, kPerRow = DP / kElems, kStepRows = 128 / kPerRow, kPerThread = kKeys / kStepRows;
     const uint32_t my_row = t / kPerRow, my_col = t % kPerRow * kElems;
@@ -273,10 +268,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
     // lines; then a thread has its own row.
     constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
-    constexpr uint32_t kHalves = F::kHalves;
-    const uint32_t warp_row = warp / (4 * kHalves) * kRows + (warp & 3u) * 32u, half = kHalves == 2 ? warp / 4 & 1u : 0u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
+    const uint32_t warp_row = warp * 32u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
     if (warp < F::kRowWarps) {
-      if (half == 0) {
         const uint32_t c = lane % kPerQ;
         const bool in_row = c * kPer16<T> < dim;
         const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)(g * per_head.d) * a.q_head + (in_row ? c * kPer16<T> : 0);
@@ -287,7 +280,6 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             const T* p = qb + (int64_t)qi * a.q_token + (int64_t)(row - qi * per_head.d) * a.q_head;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + q_stage + (r * kPerQ + (c ^ (r & (kPerQ - 1)))) * 16), "l"(p), "r"(in ? 16 : 0) : "memory");
         }
-      }
     } else if (warp < F::kIssueAt) {
         for (uint32_t i = 0; i < F::kAhead; ++i) {
             if (wg + i * RT < jobs) copy(wg + i * RT);
@@ -303,10 +295,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             RowBars& bar = s_row[lane];
             for (int i = 0; i < 2; ++i) {
                 mbar_init(smem_u32(&bar.s_full[i]), 1);
-                mbar_init(smem_u32(&bar.p_full[i]), 4 * kHalves);
+                mbar_init(smem_u32(&bar.p_full[i]), 4);
                 mbar_init(smem_u32(&bar.done[i]), 1);
             }
-            for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar.halves[i]), 2);
             mbar_init(smem_u32(&bar.q_full), 4);
         }
         fence_barrier_init();
@@ -326,29 +317,16 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     };
 
     if (warp < F::kRowWarps) {
-        // ---------------------------------------------------------------- a row a thread, or for two in two warps, half the keys of a tile each
+        // ---------------------------------------------------------------- a row a thread
         regs_up<F::kRowRegs>();
-        const uint32_t rt = warp / (4 * kHalves), lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
+        const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
         RowBars& bar = s_row[rt];
         const uint32_t my_tmem = tmem + rt * 256u + lanes;
         const uint32_t row = r0 + min(r, n_rows - 1), qi = per_head(row);
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
-        // The two warps of a row exchange a number of each row: what the other one has for this row.  False where the other one does not come.
-        uint32_t exchanges = 0;
-        auto exchange = [&](float v, float& theirs) -> bool {
-            s_half[exchanges & 1u][half][r] = v;
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bar.halves[warp & 3u]));
-            const bool ok = wait_warp(smem_u32(&bar.halves[warp & 3u]), exchanges & 1u, &s_abort);
-            tc_fence_after_sync();
-            theirs = s_half[exchanges & 1u][half ^ 1u][r];
-            ++exchanges;
-            return ok;
-        };
         float factor = fabsf(a.scale);   // of this row's scores
-        if (half == 0) {
+        {
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
             uint4 raw[kPerQ];
@@ -392,17 +370,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 }
             }
             tmem_st_wait();
-            if constexpr (F::kParts == 2) s_factor[r] = factor;
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.q_full));
-        } else if (F::kParts == 2) {
-            if (wait_warp(smem_u32(&bar.q_full), 0, &s_abort)) factor = s_factor[r];
-        } else if (a.scale == 0.f) {
-            factor = 1.f;
         }
-        constexpr uint32_t kCols = DP / kHalves;   // of the output, a warp's
-        const uint32_t col0 = half * kCols;
         // All rows see all of a tile that lies between these.
         const uint32_t r_first = min(rt * kRows, n_rows - 1), r_last = min((rt + 1) * kRows, n_rows) - 1;
         const int32_t common_hi = key_bounds(a, first + per_head(r0 + r_first), length).hi, common_lo = key_bounds(a, first + per_head(r0 + max(r_last, r_first)), length).lo;
@@ -419,7 +390,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         auto add_chunk = [&](bool chunk, float norm) {
             const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm, up = power2(-unit) * norm;
 #pragma unroll 2
-            for (uint32_t col = col0; col < col0 + kCols; col += 16) {
+            for (uint32_t col = 0; col < DP; col += 16) {
                 uint32_t v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] = 0;
@@ -470,18 +441,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 e = s_exp_v[j % 8];
             }
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
-            constexpr int kMine = 2 / (int)kHalves;   // groups of 32 keys
-            uint32_t sc[kMine][32];
+            uint32_t sc[2][32];
 #pragma unroll
-            for (int g = 0; g < kMine; ++g) tmem_ld_32x32b_x32(at + (half + g) * 32, sc[g]);
+            for (int g = 0; g < 2; ++g) tmem_ld_32x32b_x32(at + g * 32, sc[g]);
             tmem_ld_wait();
             if (t0 + j < full_from || t0 + j >= full_to) {
                 int32_t k0, end;
                 tile_keys(t0 + j, k0, end);
                 const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
 #pragma unroll
-                for (int g = 0; g < kMine; ++g) {
-                    const uint32_t bits = (uint32_t)(seen >> 32 * (half + g));
+                for (int g = 0; g < 2; ++g) {
+                    const uint32_t bits = (uint32_t)(seen >> 32 * g);
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (!(bits >> i & 1u)) sc[g][i] = 0xFF800000u;
@@ -491,18 +461,13 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             {
                 float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < kMine; ++g)
+                for (int g = 0; g < 2; ++g)
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         x = max3(x, __uint_as_float(sc[g][i]), __uint_as_float(sc[g][i + 1]));
                         y = max3(y, __uint_as_float(sc[g][i + 2]), __uint_as_float(sc[g][i + 3]));
                     }
                 top = fmaxf(x, y) * c;
-                if constexpr (kHalves == 2) {
-                    float other;
-                    if (!exchange(top, other)) break;
-                    top = fmaxf(top, other);
-                }
             }
             // Another maximum, or another power of two of the values: the output so far is brought in line, where there is one.
             float more = kBoost;   // log2 of what this tile's weights carry
@@ -518,17 +483,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     if constexpr (F::kParts == 2) {
                         float big = 0.f;
 #pragma unroll 1
-                        for (uint32_t col = col0; col < col0 + kCols; col += 16) {
+                        for (uint32_t col = 0; col < DP; col += 16) {
                             uint32_t v[16];
                             tmem_ld_32x32b_x16(out_at + col, v);
                             tmem_ld_wait();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
-                        }
-                        if constexpr (kHalves == 2) {
-                            float other;
-                            if (!exchange(big, other)) break;
-                            big = fmaxf(big, other);
                         }
                         // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
                         const int x = max(-120, min(120, e - unit));
@@ -538,7 +498,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         }
                     }
 #pragma unroll 1
-                    for (uint32_t col = col0; col < col0 + kCols; col += 16) {
+                    for (uint32_t col = 0; col < DP; col += 16) {
                         uint32_t v[16];
                         tmem_ld_32x32b_x16(out_at + col, v);
                         tmem_ld_wait();
@@ -562,8 +522,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             uint64_t sum[2] = {0, 0};
             // Weights of 32 keys: of 16-bit types 16 columns, of fp32, where their own scores lay, 16 and as many of their rests.
 #pragma unroll
-            for (int g = 0; g < kMine; ++g) {
-                const uint32_t to = at + (half + g) * (F::kParts == 2 ? 32 : 16);
+            for (int g = 0; g < 2; ++g) {
+                const uint32_t to = at + g * (F::kParts == 2 ? 32 : 16);
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     uint32_t hi[8], lo[8];
@@ -589,22 +549,15 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
-        if constexpr (kHalves == 2) {
-            float other = 0.f;
-            exchange(l, other);
-            l += other;
-        }
         const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         add_chunk(done, norm);
         if (shares > 1) {
-            if (half == 0) {
-                s_m[r] = m;
-                s_l[r] = l;
-            }
-        } else {   // the warp's columns of its rows, whole lines (of fp32) at a time
+            s_m[r] = m;
+            s_l[r] = l;
+        } else {   // the warp's rows, whole lines at a time
             __syncwarp();
-            constexpr uint32_t kPerO = kCols / 4;
-            const uint32_t c4 = half * kPerO + lane % kPerO;
+            constexpr uint32_t kPerO = DP / 4;
+            const uint32_t c4 = lane % kPerO;
 #pragma unroll 4
             for (uint32_t i = lane / kPerO; i < 32; i += 32 / kPerO)
                 if (warp_row + i < n_rows && c4 * 4 < dim) write_row(warp_row + i, c4 * 4, s_o[out_place(warp_row + i, c4)]);
