@@ -306,11 +306,12 @@ int lutamm_rotary(lutamm_ctx* ctx, const lutamm_rotary_params* p, uint32_t flags
  * tokens behind a cache have first = lengths - queries and right = 0, a sliding window has left, and sinks are the
  * first keys, which stay visible.  A query that sees no key gives zeros.  Keys from lengths[b] on are not read; lengths are taken between 0
  * and keys.  Head h reads key head h / (heads / kv_heads).  A key that a query does not see has no part in its result, whatever it holds,
- * with one exception: a value that is not finite spreads to the queries whose tile of up to 128 query rows has another one that sees it.
+ * with one exception: a value that is not finite spreads to the queries whose tile of up to 256 query rows has another one that sees it.
  * q and out are [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim]; out shares no memory with the
  * others.  For serving: there is no backward pass. */
 typedef struct lutamm_attention_params {
-    uint32_t dtype, batch, queries, keys, heads, kv_heads, head_dim;  /* head_dim a multiple of 8 up to 128, keys below 2^31 */
+    uint32_t dtype, batch, queries, keys, heads, kv_heads, head_dim;  /* head_dim a multiple of 8 up to 128, keys at most
+                                                                         * 2^31 - 256, queries * heads below 2^31 */
     uint32_t sinks;
     int32_t  left, right;
     float    scale;

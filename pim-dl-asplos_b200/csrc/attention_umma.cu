@@ -807,8 +807,8 @@ template <typename T>
 cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
     if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads);
-    // fp32's keys and values are converted once for 256 rows (ViT's batch 148 us with 128, 116 with 256); 16-bit types, which are only copied, do
-    // better with two CTAs of 128 rows on an SM (8192 tokens in bf16 101 us, 116 with 256).
+    // fp32's keys and values are converted once for 256 rows (ViT's batch 101 us with 128, 96 with 256; BERT-large's 98 and 79); 16-bit types, which are only
+    // copied, do better with two CTAs of 128 rows on an SM (8192 tokens in bf16 97 us, 106 with 256).
     if constexpr (sizeof(T) == 4) {
         if (rows > kRows) return run<T, 64, 2>(a, sm_count, dev_err, s);
     }

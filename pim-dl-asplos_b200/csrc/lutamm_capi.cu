@@ -1033,7 +1033,7 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     if (!size) return fail(c, LUTAMM_EINVAL, "unknown dtype");
     if (!p->head_dim || p->head_dim % 8 || p->head_dim > 128) return fail(c, LUTAMM_EINVAL, "head_dim must be a multiple of 8 up to 128");
     if (!p->kv_heads || p->heads % p->kv_heads) return fail(c, LUTAMM_EINVAL, "heads must be a multiple of kv_heads");
-    if (p->keys >> 31 || p->queries >> 31) return fail(c, LUTAMM_EINVAL, "keys and queries must be below 2^31");
+    if (p->keys > 0x7FFFFF00u || p->queries >> 31) return fail(c, LUTAMM_EINVAL, "keys must be at most 2^31 - 256 and queries below 2^31");
     if (!std::isfinite(p->scale)) return fail(c, LUTAMM_EINVAL, "scale must be finite");
     if (!p->batch || !p->queries || !p->heads) return LUTAMM_OK;
     if ((uint64_t)p->queries * p->heads >> 31 || (uint64_t)p->batch * p->queries > (1ull << 40) / p->heads)
@@ -1065,10 +1065,8 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
     const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
-    // The tensor cores need many rows to be worth fp32's conversion (12 rows of 8 x 8192 keys, heads of 128: 695 us there, 568 here), and 16-bit types
-    // almost none (2 rows, heads of 64: 78 and 81 us; 8 rows 79 and 160).  What does not start on 16 bytes goes element by element here.
-    const cudaError_t e = rows <= (size == 4 ? 16 : 2) || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
-                                    : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
+    const cudaError_t e = rows <= attention_few_rows(size) || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
+                                                                              : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
     return dense_done(c, e, "attention", 1, flags);
 }
 

@@ -78,7 +78,7 @@ SET = {
     "lutamm_rotary": [dict(dtype=3), dict(axes=0), dict(axes=5), dict(head_dim=0), dict(head_dim=5000), dict(heads=1 << 21), dict(sections=(5, 4)), dict(sections=(2 ** 32 - 1, 9)), dict(positions=0),
                       dict(inv_freq=0), dict(positions="+2"), dict(x=(0, 96, 32, 16)), dict(out=(4096, 96, 32, 15)), dict(out=(4096, 0, 32, 16)), dict(x=(None, 96, 32, -16)),
                       dict(out=(0, 96, 32, 17)), dict(batch=1 << 30, tokens=1 << 30), dict(position_token_stride=-2)],
-    "lutamm_attention": [dict(dtype=4), dict(head_dim=0), dict(head_dim=12), dict(head_dim=136), dict(kv_heads=0), dict(heads=3), dict(keys=1 << 31), dict(queries=1 << 31), dict(scale=float("inf")),
+    "lutamm_attention": [dict(dtype=4), dict(head_dim=0), dict(head_dim=12), dict(head_dim=136), dict(kv_heads=0), dict(heads=3), dict(keys=1 << 31), dict(keys=(1 << 31) - 255), dict(queries=1 << 31), dict(scale=float("inf")),
                          dict(scale=float("nan")), dict(q=(None, 96, 32, 16)), dict(k=(None, 96, 32, 16)), dict(v=(None, 96, 32, 16)), dict(out=(None, 96, 32, 16)), dict(out=(0, 96, 32, 16)),
                          dict(out=(4096, 96, 32, 8)), dict(out=(4096, 96, 0, 16)), dict(k=(0, 96, -32, 16)), dict(lengths="+2"), dict(first="+1"), dict(batch=2 ** 31, queries=2 ** 30)],
 }
