@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) norm_grad_kernel(NormGradArgs a) 
     }
 }
 
-// Any length: dx alone, a row a CTA, read twice ...
+// Any length: dx alone, a row a CTA, read twice; and, before it, ...
 template <typename T, int E>
 __global__ void __launch_bounds__(512) norm_grad_long_kernel(NormGradArgs a) {
     __shared__ float s_sum[16][2];
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(512) norm_grad_long_kernel(NormGradArgs a) {
         store_elems<T, E>(dx + (size_t)g * E, o);
     }
 }
-// ... and the sums over rows, a column a thread, row block blockIdx.y.
+// ... the sums over rows, a column a thread, row block blockIdx.y.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_columns_kernel(NormGradArgs a) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
@@ -409,13 +409,13 @@ cudaError_t run_typed_grad(const NormGradArgs& a, int sm_count, cudaStream_t s) 
     const uint32_t parts = grad_parts(a.rows, a.width, sm_count);
     cudaError_t e = cudaSuccess;
     if (a.width > kMostElems) {
-        if (a.dx && a.rows) {
-            if (vec) norm_grad_long_kernel<T, kPer16<T>><<<a.rows, 512, 0, s>>>(a);
-            else norm_grad_long_kernel<T, 1><<<a.rows, 512, 0, s>>>(a);
+        if (a.partial) {   // first: dx may be written over x or dout
+            norm_columns_kernel<T><<<dim3((a.width + 255) / 256, parts), 256, 0, s>>>(a);
             e = cudaGetLastError();
         }
-        if (e == cudaSuccess && a.partial) {
-            norm_columns_kernel<T><<<dim3((a.width + 255) / 256, parts), 256, 0, s>>>(a);
+        if (e == cudaSuccess && a.dx && a.rows) {
+            if (vec) norm_grad_long_kernel<T, kPer16<T>><<<a.rows, 512, 0, s>>>(a);
+            else norm_grad_long_kernel<T, 1><<<a.rows, 512, 0, s>>>(a);
             e = cudaGetLastError();
         }
     } else {

@@ -105,6 +105,23 @@ def test_layer_norm_backward(ctx, rows, width, stride, shift, dtype):
             assert (buf[:, width:] == 7).all()
 
 
+@pytest.mark.parametrize("width", [33, 768, 1999, 8192, 8200, 9001])
+def test_layer_norm_backward_in_place(ctx, width):
+    """dx over x or over dout: the bits of dx elsewhere, dweight's and dbias's too."""
+    gen, rows = _gen(width), 37
+    x, dy = torch.randn(rows, width, generator=gen).cuda(), torch.randn(rows, width, generator=gen).cuda()
+    w, stats = torch.randn(width, generator=gen).cuda(), torch.empty(rows, 2, device="cuda")
+    ctx.layer_norm(x, w, None, torch.empty_like(x), stats=stats)
+    def grads(dy, x, dx):
+        dw, db = torch.empty(width, device="cuda"), torch.empty(width, device="cuda")
+        ctx.layer_norm_backward(dy, x, w, stats, dx, dw, db)
+        return dx, dw, db
+    want = grads(dy, x, torch.empty_like(x))
+    over_x, over_dy = x.clone(), dy.clone()
+    for got in (grads(dy, over_x, over_x), grads(over_dy, x, over_dy)):
+        assert all(torch.equal(g, r) for g, r in zip(got, want))
+
+
 def test_layer_norm_backward_against_differences(ctx):
     """dx, dw and db of a weighted sum of outputs against central differences of the forward formula in 64 bits."""
     gen = _gen(3)
