@@ -263,6 +263,14 @@ def _packed(name: str, t, dtype, shape) -> int:
     return at
 
 
+def _u32(*values):
+    """Counts as the C ABI has them: ctypes would cut them to their low bits."""
+    for v in values:
+        if not 0 <= v < 1 << 32:
+            raise ValueError(f"a count between 0 and 2^32 - 1 is wanted, got {v}")
+    return values
+
+
 def _heads(name: str, t, dtype, shape) -> Heads:
     at = _operand(name, t, dtype, shape)
     return Heads(at, *t.stride()[:3])
@@ -451,7 +459,7 @@ class LutAmmContext:
         import torch
         rows, width = x.shape
         f32 = torch.float32
-        p = NormParams(_dtype_of(x), rows, width, eps, _operand("x", x, x.dtype, (rows, width)), x.stride(0),
+        p = NormParams(_dtype_of(x), *_u32(rows, width), eps, _operand("x", x, x.dtype, (rows, width)), x.stride(0),
                        _operand("residual", residual, x.dtype, (rows, width)), residual.stride(0) if residual is not None else 0,
                        _operand("out", out, x.dtype, (rows, width)), out.stride(0),
                        _operand("weight", weight, f32, (width,)), _operand("bias", bias, f32, (width,)),
@@ -470,7 +478,7 @@ class LutAmmContext:
         if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()
                                       or workspace.numel() < self.layer_norm_backward_workspace(rows, width)):
             raise ValueError("workspace: a contiguous uint8 tensor of layer_norm_backward_workspace() bytes is wanted")
-        p = NormGradParams(_dtype_of(x), rows, width, _operand("dout", dout, x.dtype, (rows, width)), dout.stride(0),
+        p = NormGradParams(_dtype_of(x), *_u32(rows, width), _operand("dout", dout, x.dtype, (rows, width)), dout.stride(0),
                            _operand("x", x, x.dtype, (rows, width)), x.stride(0),
                            _operand("dx", dx, x.dtype, (rows, width)), dx.stride(0) if dx is not None else 0,
                            _operand("weight", weight, f32, (width,)), _packed("stats", stats, f32, (rows, 2)),
@@ -479,7 +487,7 @@ class LutAmmContext:
         self._check(self._L.lutamm_layer_norm_backward(self._h, ctypes.byref(p), flags))
 
     def layer_norm_backward_workspace(self, rows: int, width: int) -> int:
-        return int(self._L.lutamm_layer_norm_backward_workspace(self._h, rows, width))
+        return int(self._L.lutamm_layer_norm_backward_workspace(self._h, *_u32(rows, width)))
 
     def rotary(self, x, positions, inv_freq, sections, out, interleaved: bool = False, inverse: bool = False, flags: int = 0):
         """Rotary positions with several axes.  x and out [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], float32, float16
@@ -495,9 +503,9 @@ class LutAmmContext:
         if not own_positions:
             positions = positions.expand(x.shape[0], -1, -1)
         axes = len(sections)
-        if x.dim() != 4 or not 1 <= axes <= MAX_AXES or min(sections) < 0:
-            raise ValueError(f"x has three or four axes, sections 1 to {MAX_AXES} counts")
-        p = RotaryParams(_dtype_of(x), *x.shape, axes, tuple(sections), bool(interleaved), bool(inverse), _heads("x", x, x.dtype, x.shape),
+        if x.dim() != 4 or not 1 <= axes <= MAX_AXES:
+            raise ValueError(f"x has three or four axes, sections has 1 to {MAX_AXES} counts")
+        p = RotaryParams(_dtype_of(x), *_u32(*x.shape), axes, _u32(*sections), bool(interleaved), bool(inverse), _heads("x", x, x.dtype, x.shape),
                          _heads("out", out, x.dtype, x.shape), _operand("positions", positions, torch.int32, (*x.shape[:2], axes)),
                          positions.stride(0) if own_positions else 0, positions.stride(1), _packed("inv_freq", inv_freq, torch.float32, (sum(sections),)))
         if not batched:
@@ -516,7 +524,9 @@ class LutAmmContext:
         import torch
         B, Q, H, D = q.shape
         K, G = k.shape[1:3]
-        p = AttentionParams(_dtype_of(q), B, Q, K, H, G, D, sinks, *window, D ** -0.5 if scale is None else scale,
+        if len(window) != 2 or not all(-1 << 31 <= w < 1 << 31 for w in window):
+            raise ValueError(f"window: two numbers of 32 bits are wanted, got {window}")
+        p = AttentionParams(_dtype_of(q), *_u32(B, Q, K, H, G, D, sinks), *window, D ** -0.5 if scale is None else scale,
                             _heads("q", q, q.dtype, (B, Q, H, D)), _heads("k", k, q.dtype, (B, K, G, D)),
                             _heads("v", v, q.dtype, (B, K, G, D)), _heads("out", out, q.dtype, (B, Q, H, D)),
                             _packed("lengths", lengths, torch.int32, (B,)), _packed("first", first, torch.int32, (B,)))

@@ -78,6 +78,30 @@ def test_the_ordinary_call_takes_the_short_way(monkeypatch):
     assert len(ctx.seen) == 3
 
 
+@pytest.mark.parametrize("fast", [True, False])
+def test_numbers_beyond_the_blocks_fields_are_refused(monkeypatch, fast):
+    if not fast:
+        monkeypatch.setattr(P, "_fast", None)
+    ctx = _Context()
+    q, k = torch.zeros(1, 2, 1, 8), torch.zeros(1, 3, 1, 8)
+    for kw in (dict(sinks=-1), dict(sinks=1 << 32), dict(window=(1 << 31, 0)), dict(window=(0, -(1 << 31) - 1)), dict(window=((1 << 32) + 3, 0)), dict(window=(1, 2, 3))):
+        with pytest.raises(ValueError):
+            ctx.attention(q, k, k, q.clone(), **kw)
+    x = torch.zeros(1, dtype=torch.float16)
+    tall = x.expand((1 << 32) + 1).unsqueeze(1)
+    with pytest.raises(ValueError):
+        ctx.layer_norm(tall, None, None, tall)
+    with pytest.raises(ValueError):
+        ctx.layer_norm_backward(tall, tall, None, torch.zeros(2).expand(tall.shape[0], 2), dbias=torch.zeros(1))
+    with pytest.raises(ValueError):
+        ctx.layer_norm_backward_workspace(1 << 32, 1)
+    h = torch.zeros(3, 2, 8)
+    for sections in ((-1, 5), (1 << 32, 4)):
+        with pytest.raises(ValueError):
+            ctx.rotary(h, torch.zeros(3, 2, dtype=torch.int32), torch.zeros(4), sections, h)
+    assert not ctx.seen
+
+
 def test_blocks_have_the_headers_layout(tmp_path):
     """Sizes and offsets of the ctypes blocks are those a C compiler gives the header's."""
     import os
