@@ -142,6 +142,11 @@ class Dense:
     sections: tuple = ()
     interleaved: bool = False
 
+    def key(self):
+        """All that a recorded forward has taken from here."""
+        tensors = ((t.data_ptr(), t.dtype, t.shape, t.stride()) if t is not None else None for t in (self.lengths, self.positions, self.inv_freq))
+        return (tuple(self.window), self.sinks, tuple(self.sections), self.interleaved, *tensors)
+
 
 class LutTransformerLayer:
     """One encoder layer; `forward` takes and returns a device tensor [n, token_dim].  dense: a Dense, None for PyTorch's operators."""
@@ -179,8 +184,6 @@ class LutTransformerLayer:
         else:
             self.buf["qkv"] = torch.empty(self.n, 3 * self.token_dim, **f32)
         self.dense = dense
-        if dense is not None:
-            self.buf["att"], self.buf["h"] = torch.empty(self.n, self.token_dim, **f32), torch.empty(self.n, self.token_dim, **f32)
         self.amm_ms = 0.0
         self._graph = None          # (key, graph, input copy, h, f, launches) of the captured forward
         self._seen, self._seen_key = 0, None
@@ -239,7 +242,8 @@ class LutTransformerLayer:
         sdp = torch.backends.cuda
         return (stream, self.ctx.generation, self.fused_gelu, torch.is_inference_mode_enabled(),
                 sdp.flash_sdp_enabled(), sdp.mem_efficient_sdp_enabled(), sdp.math_sdp_enabled(), sdp.cudnn_sdp_enabled(),
-                tuple(torch._C._get_sdp_priority_order()), sdp.matmul.fp32_precision, tuple(t.data_ptr() for t in norms))
+                tuple(torch._C._get_sdp_priority_order()), sdp.matmul.fp32_precision, tuple(t.data_ptr() for t in norms),
+                self.dense.key() if getattr(self, "dense", None) is not None else None)
 
     def _capture(self, x, key):
         """Record the layer up to its last addition on a copy of the input: 16 launches and their Python become one.
@@ -264,8 +268,14 @@ class LutTransformerLayer:
 
     def _dense_body(self, x):
         """The layer up to its second norm, all in the library."""
+        torch = self.torch
+        if (torch.is_grad_enabled() and any(t.requires_grad for t in (x, *(t for pair in self.ln.values() for t in pair)))
+                or torch.autograd.forward_ad.unpack_dual(x).tangent is not None):
+            raise RuntimeError("the library's dense operators leave no graph behind for autograd: call under torch.no_grad()")
         B, S, H, D = self.batch, self.seq_len, self.heads, self.token_dim
         hd, d, ctx = D // H, self.dense, self.ctx
+        if "att" not in self.buf:
+            self.buf["att"], self.buf["h"] = torch.empty_like(self.buf["o"]), torch.empty_like(self.buf["o"])
         if self.separate_qkv:
             q, k, v = (self._amm(name, x).view(B, S, H, hd) for name in ("q", "k", "v"))
             turned = (q, k)
@@ -282,7 +292,7 @@ class LutTransformerLayer:
         ctx.layer_norm(self._amm("o", att), *self.ln["ln1"], h, eps=1e-6, residual=x, flags=FLAG_ASYNC)
         f = self._amm("ffn1", h)
         if not self.fused_gelu:
-            f = self.torch.nn.functional.gelu(f, approximate="tanh")
+            f = torch.nn.functional.gelu(f, approximate="tanh")
         return h, self._amm("ffn2", f)
 
     def _body(self, x):

@@ -162,6 +162,56 @@ def test_recorded_and_replayed_with_other_inputs(ctx, stream):
     assert all(torch.equal(out[k], eager[1][k]) for k in out)
 
 
+def test_a_recorded_layer_follows_its_operators(ctx, stream):
+    """After three forwards the layer replays a recording: a window, sinks, lengths, positions or a whole Dense set since count as in a layer of its own."""
+    S, B, H, D = 24, 2, 2, 64
+    w = _weights(D, 2 * D, False, 9)
+    gen = torch.Generator().manual_seed(4)
+
+    def positions(most):
+        return dict(positions=torch.randint(0, most, (S, 1), generator=gen, dtype=torch.int32).cuda(), sections=(16,),
+                    inv_freq=(50.0 ** -(torch.arange(16) / 16)).cuda())
+    turned, turned_else = positions(20), positions(900)
+    short = dict(lengths=torch.tensor([S, 5], dtype=torch.int32).cuda())
+    steps = [dict(window=(4, 4)), dict(window=(2, 9)), dict(window=(2, 9), sinks=2), dict(window=(2, 9), sinks=2, **short), dict(**turned), dict(**turned_else),
+             dict(interleaved=True, **turned_else), dict(), None]
+    x = torch.from_numpy(L.synth.make_input(S * B, D, seed=7)).cuda()
+    torch.cuda.synchronize()
+
+    def layer(dense):
+        return L.LutTransformerLayer(ctx, w, S, B, H, first_layer_id=320, dense=dense)
+    with torch.no_grad(), torch.cuda.stream(stream):
+        want = [layer(None if s is None else L.Dense(**s)).forward(x).clone() for s in steps]
+        for whole in (False, True):
+            lay = layer(L.Dense())
+            for s, y in zip(steps, want):
+                if whole or s is None:
+                    lay.dense = None if s is None else L.Dense(**s)
+                else:
+                    for name, value in L.Dense(**s).__dict__.items():
+                        setattr(lay.dense, name, value)
+                for _ in range(4):
+                    assert torch.equal(lay.forward(x), y), s
+                assert lay._graph is not None
+        stream.synchronize()
+    assert len({tuple(y.flatten()[:4].tolist()) for y in want[:-1]}) > 4
+
+
+def test_autograd_is_refused(ctx, stream):
+    S, B, H, D = 8, 1, 2, 64
+    lay = L.LutTransformerLayer(ctx, _weights(D, 2 * D, False, 9), S, B, H, first_layer_id=330, dense=L.Dense())
+    x = torch.from_numpy(L.synth.make_input(S * B, D, seed=7)).cuda()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        with pytest.raises(RuntimeError, match="autograd"):
+            lay.forward(x.requires_grad_())
+        with torch.no_grad():
+            assert lay.forward(x).shape == x.shape
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="autograd"):
+            lay.forward(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()))
+        stream.synchronize()
+
+
 def test_contexts_on_streams_of_their_own_at_once(ctx):
     """Two contexts, each with its stream, queue the same operators side by side many times: no scratch is shared between them."""
     other = P.LutAmmContext(0)
