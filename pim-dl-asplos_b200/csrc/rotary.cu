@@ -44,6 +44,26 @@ template <typename T, int E, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, uint32_t per, uint32_t blocks) {
     extern __shared__ float2 s_turn[];   // [token][pair]
     const uint32_t b = blockIdx.x / blocks, t0 = (blockIdx.x - b * blocks) * per, n = min(per, a.tokens - t0);
+    // A unit is E pairs.  A thread has one unit of one token, takes its sines and cosines into registers, and goes through the heads, some on their way.
+    const uint32_t units = a.pairs / E, slots = n * units, width = min(max(slots, 1u), (uint32_t)kThreads), groups = kThreads / width, group = threadIdx.x / width;
+    const uint32_t slot0 = group < groups ? threadIdx.x - group * width : slots;
+    const T* xb = static_cast<const T*>(a.x) + (int64_t)b * a.x_batch + (int64_t)t0 * a.x_token;
+    T* yb = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)t0 * a.out_token;
+    constexpr int kInFlight = 4;
+    Piece<T, E> p_raw[kInFlight], q_raw[kInFlight];
+    auto fetch = [&](uint32_t slot, uint32_t first) {
+        const uint32_t local = slot / units, u = slot - local * units, c0 = INTERLEAVED ? 2 * u * E : u * E, c1 = c0 + (INTERLEAVED ? E : a.pairs);
+        const T* x = xb + (int64_t)local * a.x_token;
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k) {
+            const uint32_t head = first + k * groups;
+            if (head < a.heads) {
+                p_raw[k].load(x + (int64_t)head * a.x_head + c0);
+                q_raw[k].load(x + (int64_t)head * a.x_head + c1);
+            }
+        }
+    };
+    if (slot0 < slots) fetch(slot0, group);   // the first ones while the sines are formed
     for (uint32_t i = threadIdx.x; i < n * a.pairs; i += kThreads) {
         const uint32_t local = i / a.pairs, pair = i - local * a.pairs;
         const uint32_t axis = (pair >= a.ends[0]) + (pair >= a.ends[1]) + (pair >= a.ends[2]);
@@ -57,29 +77,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, uint32_t
         s_turn[i] = make_float2(c, a.inverse ? -s : s);
     }
     __syncthreads();
-    // A unit is E pairs.  A thread has one unit of one token, takes its sines and cosines into registers, and goes through the heads, four on their way.
-    const uint32_t units = a.pairs / E, slots = n * units, width = min(max(slots, 1u), (uint32_t)kThreads), groups = kThreads / width, group = threadIdx.x / width;
-    const T* xb = static_cast<const T*>(a.x) + (int64_t)b * a.x_batch + (int64_t)t0 * a.x_token;
-    T* yb = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)t0 * a.out_token;
-    for (uint32_t slot = group < groups ? threadIdx.x - group * width : slots; slot < slots; slot += width) {
+    for (uint32_t slot = slot0; slot < slots; slot += width) {
         const uint32_t local = slot / units, u = slot - local * units;
         float2 turn[E];
 #pragma unroll
         for (int k = 0; k < E; ++k) turn[k] = s_turn[slot * E + k];
         const uint32_t c0 = INTERLEAVED ? 2 * u * E : u * E, c1 = c0 + (INTERLEAVED ? E : a.pairs);
-        const T* x = xb + (int64_t)local * a.x_token;
         T* y = yb + (int64_t)local * a.out_token;
-        constexpr int kInFlight = 4;
         for (uint32_t first = group; first < a.heads; first += kInFlight * groups) {
-            Piece<T, E> p_raw[kInFlight], q_raw[kInFlight];
-#pragma unroll
-            for (int k = 0; k < kInFlight; ++k) {
-                const uint32_t head = first + k * groups;
-                if (head < a.heads) {
-                    p_raw[k].load(x + (int64_t)head * a.x_head + c0);
-                    q_raw[k].load(x + (int64_t)head * a.x_head + c1);
-                }
-            }
+            if (slot != slot0 || first != group) fetch(slot, first);
 #pragma unroll
             for (int k = 0; k < kInFlight; ++k) {
                 const uint32_t head = first + k * groups;
