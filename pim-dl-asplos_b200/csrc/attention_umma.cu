@@ -174,10 +174,13 @@ Divisor divisor(uint32_t d) {
     return Divisor{d, (uint32_t)(d == 1 ? 0 : (1ull << (31 + bits)) / d + 1), 31 + bits};
 }
 
-template <typename T, int DP, int RT>
+// FEW: at most 32 rows.  All four warps of rows have them, each with sixteen keys of every tile and an output of its own; they join in the end.  One warp with
+// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 55 us so, 49 with four warps, 5.5 TB/s.
+template <typename T, int DP, int RT, bool FEW>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
     using F = Form<T, DP, RT>;
+    static_assert(!FEW || RT == 1);
     constexpr uint32_t kSlots = F::kSlots, kThreads = F::kThreads;
     extern __shared__ unsigned char s_raw[];
     __shared__ __align__(8) uint64_t s_full_bar[kSlots], s_empty_bar[kSlots];
@@ -268,15 +271,15 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     // The first copies leave before the CTA has met.  Queries go row by row through shared memory, 32 rows a warp, so that loads are of whole
     // lines; then a thread has its own row.
     constexpr int kPerQ = DP / kPer16<T>;   // pieces of 16 bytes a row
-    const uint32_t warp_row = warp * 32u, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
+    const uint32_t warp_row = warp * 32u, first_row = FEW ? 0u : warp_row, q_stage = kSlots * F::kTile + warp_row * DP * 4;   // where the warp's output goes
     if (warp < F::kRowWarps) {
         const uint32_t c = lane % kPerQ;
         const bool in_row = c * kPer16<T> < dim;
         const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)(g * per_head.d) * a.q_head + (in_row ? c * kPer16<T> : 0);
 #pragma unroll 4
         for (uint32_t r = lane / kPerQ; r < 32; r += 32 / kPerQ) {
-            const bool in = in_row && warp_row + r < n_rows;
-            const uint32_t row = r0 + (in ? warp_row + r : 0u), qi = per_head(row);
+            const bool in = in_row && first_row + r < n_rows;
+            const uint32_t row = r0 + (in ? first_row + r : 0u), qi = per_head(row);
             const T* p = qb + (int64_t)qi * a.q_token + (int64_t)(row - qi * per_head.d) * a.q_head;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + q_stage + (r * kPerQ + (c ^ (r & (kPerQ - 1)))) * 16), "l"(p), "r"(in ? 16 : 0) : "memory");
         }
@@ -322,7 +325,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const uint32_t rt = warp / 4, lanes = ((warp & 3u) * 32u) << 16, r = warp_row + lane;
         RowBars& bar = s_row[rt];
         const uint32_t my_tmem = tmem + rt * 256u + lanes;
-        const uint32_t row = r0 + min(r, n_rows - 1), qi = per_head(row);
+        const uint32_t row = r0 + min(first_row + lane, n_rows - 1), qi = per_head(row);
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
         float factor = fabsf(a.scale);   // of this row's scores
@@ -417,7 +420,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if (RT == 2 && !sees(t0 + j)) continue;
             if (!wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
-            if (warp_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
+            if (first_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
                 if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
                 ++n;
                 continue;
@@ -441,19 +444,24 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 e = s_exp_v[j % 8];
             }
             c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
-            uint32_t sc[2][32];
+            constexpr int kGroups = FEW ? 1 : 2, kWide = FEW ? 16 : 32;
+            uint32_t sc[kGroups][kWide];
+            if constexpr (FEW) {
+                tmem_ld_32x32b_x16(at + warp * 16, sc[0]);
+            } else {
 #pragma unroll
-            for (int g = 0; g < 2; ++g) tmem_ld_32x32b_x32(at + g * 32, sc[g]);
+                for (int g = 0; g < 2; ++g) tmem_ld_32x32b_x32(at + g * 32, sc[g]);
+            }
             tmem_ld_wait();
             if (t0 + j < full_from || t0 + j >= full_to) {
                 int32_t k0, end;
                 tile_keys(t0 + j, k0, end);
                 const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const uint32_t bits = (uint32_t)(seen >> 32 * g);
+                for (int g = 0; g < kGroups; ++g) {
+                    const uint32_t bits = (uint32_t)(seen >> (FEW ? 16 * warp : 32 * g));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < kWide; ++i)
                         if (!(bits >> i & 1u)) sc[g][i] = 0xFF800000u;
                 }
             }
@@ -461,9 +469,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             {
                 float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+                for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
+                    for (int i = 0; i < kWide; i += 4) {
                         x = max3(x, __uint_as_float(sc[g][i]), __uint_as_float(sc[g][i + 1]));
                         y = max3(y, __uint_as_float(sc[g][i + 2]), __uint_as_float(sc[g][i + 3]));
                     }
@@ -522,10 +530,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             uint64_t sum[2] = {0, 0};
             // Weights of 32 keys: of 16-bit types 16 columns, of fp32, where their own scores lay, 16 and as many of their rests.
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const uint32_t to = at + g * (F::kParts == 2 ? 32 : 16);
+            for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
+                for (int part = 0; part < kWide / 16; ++part) {
+                    const uint32_t sixteen = FEW ? warp : 2 * g + part, to = at + (F::kParts == 2 ? sixteen / 2 * 32 + sixteen % 2 * 8 : sixteen * 8);
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
@@ -535,8 +543,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
                         else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
                     }
-                    tmem_st_32x32b_x8(to + part * 8, hi);
-                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16 + part * 8, lo);
+                    tmem_st_32x32b_x8(to, hi);
+                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16, lo);
+                }
+            }
+            if constexpr (FEW) {   // the other warps' keys have no weight here
+                const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int i = 1; i < 4; ++i) {
+                    const uint32_t sixteen = (warp + i) & 3u, to = at + (F::kParts == 2 ? sixteen / 2 * 32 + sixteen % 2 * 8 : sixteen * 8);
+                    tmem_st_32x32b_x8(to, none);
+                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16, none);
                 }
             }
             tmem_st_wait();
@@ -549,9 +566,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
-        const float norm = shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float norm = FEW || shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         add_chunk(done, norm);
-        if (shares > 1) {
+        if (FEW || shares > 1) {
             s_m[r] = m;
             s_l[r] = l;
         } else {   // the warp's rows, whole lines at a time
@@ -721,8 +738,38 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         }
     }
 
-    if (shares > 1) {
-        cluster_sync();
+    if constexpr (FEW) {   // the four warps' parts into the first one's place
+        __syncthreads();
+        for (uint32_t i = tid; i < n_rows * (DP / 4); i += kThreads) {
+            const uint32_t r = i / (DP / 4), c = i % (DP / 4);
+            float mk[4], top = -INFINITY;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, mk[w] = s_m[w * 32 + r]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float4 x = s_o[out_place(w * 32 + r, c)];
+                const float f = mk[w] == -INFINITY ? 0.f : exp2_approx(mk[w] - top);
+                if (f != 0.f) { v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w); }
+            }
+            s_o[out_place(r, c)] = v;
+        }
+        __syncthreads();
+        if (tid < n_rows) {
+            float top = s_m[tid], total = 0.f;
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * 32 + tid]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float mk = s_m[w * 32 + tid], lk = s_l[w * 32 + tid], f = mk == -INFINITY ? 0.f : exp2_approx(mk - top);
+                total += f == 0.f ? (lk != lk ? lk : 0.f) : lk * f;
+            }
+            s_m[tid] = top;
+            s_l[tid] = total;
+        }
+    }
+    if (FEW || shares > 1) {
+        if (shares > 1) cluster_sync(); else __syncthreads();
         if (tid < n_rows) {   // what each part of a row counts for in the result
             float mk[kMostShares], lk[kMostShares], top = -INFINITY, total = 0.f;
 #pragma unroll
@@ -757,7 +804,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 }
             write_row(r, c * 4, v);
         }
-        cluster_sync();   // what the others read is read
+        if (shares > 1) cluster_sync();   // what the others read is read
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -770,11 +817,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     if (warp == F::kIssueAt) tmem_dealloc(tmem, F::kColumns);
 }
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int RT, bool FEW = false>
 cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
     using F = Form<T, DP, RT>;
     static SmemOptIn memo;
-    cudaError_t e = allow_smem(memo, attention_umma_kernel<T, DP, RT>, F::kSmem);
+    cudaError_t e = allow_smem(memo, attention_umma_kernel<T, DP, RT, FEW>, F::kSmem);
     if (e != cudaSuccess) return e;
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads), tiles = (rows + RT * kRows - 1) / (RT * kRows);
     const uint64_t items = (uint64_t)a.batch * a.kv_heads * tiles;
@@ -800,13 +847,14 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP, RT>, a, divisor((uint32_t)tiles), divisor(a.kv_heads), divisor(a.heads / a.kv_heads), dev_err);
+    return cudaLaunchKernelEx(&cfg, attention_umma_kernel<T, DP, RT, FEW>, a, divisor((uint32_t)tiles), divisor(a.kv_heads), divisor(a.heads / a.kv_heads), dev_err);
 }
 
 template <typename T>
 cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStream_t s) {
-    if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads);
+    if (rows <= 32) return a.head_dim > 64 ? run<T, 128, 1, true>(a, sm_count, dev_err, s) : run<T, 64, 1, true>(a, sm_count, dev_err, s);
+    if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
     // fp32's keys and values are converted once for 256 rows (ViT's batch 101 us with 128, 96 with 256; BERT-large's 98 and 79); 16-bit types, which are only
     // copied, do better with two CTAs of 128 rows on an SM (8192 tokens in bf16 97 us, 106 with 256).
     if constexpr (sizeof(T) == 4) {
