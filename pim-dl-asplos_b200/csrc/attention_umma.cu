@@ -1,4 +1,5 @@
-// Attention for many rows, on the tensor cores:  out = softmax(scale q k^T) v  over the keys that a query sees (attention.cuh).
+// Attention for two rows and more (query tokens times the heads of a key head), on the tensor cores:  out = softmax(scale q k^T) v  over the keys that a
+// query sees (attention.cuh).
 //
 // A CTA takes 128 rows - query tokens times the query heads that share a key head - or, of fp32, twice 128, of one sequence through the keys that
 // any of them sees, 64 keys a tile: first the tiles of the sinks, then those of the window; tiles in between are never loaded.  Scores S = Q K^T
@@ -17,7 +18,7 @@
 // converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
 // CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no scratch memory and one order of summation.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 98 us, 350 TFLOP/s; of 2900 warp instructions a
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 97 us, 346 TFLOP/s; of 2900 warp instructions a
 // tile 680 form its weights.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 32 us, 540 TFLOP/s.  fp32,
 // three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 96 us, of which a CTA spends half before its first and behind its last tile.
 #include "attention.cuh"
@@ -53,10 +54,10 @@ struct Form {
     static_assert(RT == 1 || kUsed <= 256);
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
     // Warpgroups: one for each tile of rows, a row a thread, one for each tile of rows that loads, one that issues.  Registers a thread of each; their sum is
-    // what the warpgroups are launched with.
+    // what the warpgroups are launched with, and none of them spills (the issuing warps did with 24: 24 rows of 8 x 8192 keys in bf16 59.9 us, 54.4 so).
     static constexpr int kRowWarps = 4 * RT, kIssueAt = 8 * RT, kThreads = (2 * RT + 1) * 128;
-    static constexpr int kLaunchRegs = DP > 64 ? 168 : RT == 2 ? 96 : 80, kRowRegs = DP > 64 ? 232 : 152, kLoadRegs = DP > 64 ? 136 : RT == 2 ? 72 : 64;
-    static constexpr int kIssueRegs = DP > 64 ? 136 : RT == 2 ? 32 : 24;
+    static constexpr int kLaunchRegs = DP > 64 ? 168 : RT == 2 ? 96 : 80, kRowRegs = DP > 64 ? 232 : 136, kLoadRegs = DP > 64 ? 136 : RT == 2 ? 80 : 56;
+    static constexpr int kIssueRegs = DP > 64 ? 136 : 48;
     static_assert(RT * (kRowRegs + kLoadRegs) + kIssueRegs == (2 * RT + 1) * kLaunchRegs && kCtas * kThreads * kLaunchRegs <= 65536);
 };
 
