@@ -263,7 +263,7 @@ int lutamm_layer_norm(lutamm_ctx* ctx, const lutamm_norm_params* p, uint32_t fla
  * Sums over rows are made in a fixed order: equal calls give equal bits.  They pass through
  * lutamm_layer_norm_backward_workspace() bytes of `workspace`, device memory on 16 bytes that the caller keeps, or, where that is
  * NULL, through memory of the context.  Graphs captured from calls on one context share the latter and must not be replayed
- * at the same time. */
+ * at the same time, nor once it has grown (lutamm_generation). */
 typedef struct lutamm_norm_grad_params {
     uint32_t dtype, rows, width;
     const void* dout;     int64_t dout_stride;

@@ -263,7 +263,7 @@ def _check_attention(ctx, B, Q, K, H, G, D, t, window=(-1, -1), sinks=0, lengths
 @pytest.mark.parametrize("K,lengths,window,sinks", [
     (1, None, (-1, -1), 0), (2, [2, 1, 0], (-1, 0), 0), (63, [63, 1, 40], (-1, -1), 0), (64, None, (10, 0), 3), (65, [65, 64, 63], (0, 0), 0), (200, [200, 3, 0], (7, 0), 2),
     (1000, [1000, 500, 129], (100, 0), 64), (4097, [4097, 4000, 17], (2047, 0), 8), (5000, [6000, -3, 5000], (-1, -1), 0), (333, None, (0, 0), 400)])
-@pytest.mark.parametrize("Q,H,G,D", [(1, 1, 1, 64), (1, 12, 12, 64), (1, 4, 1, 128), (1, 16, 2, 32), (3, 2, 2, 80), (2, 6, 2, 8), (5, 3, 1, 64)])
+@pytest.mark.parametrize("Q,H,G,D", [(1, 1, 1, 64), (1, 12, 12, 64), (1, 4, 1, 128), (1, 16, 2, 32), (3, 2, 2, 80), (2, 6, 2, 8), (5, 3, 1, 64), (4, 8, 1, 128), (3, 11, 1, 72)])
 def test_attention_of_few_rows(ctx, Q, H, G, D, K, lengths, window, sinks, dtype):
     B = 3
     first = [max(0, min(n, K)) - Q for n in (lengths or [K] * B)]
@@ -295,7 +295,7 @@ def test_attention_of_a_chunk_behind_a_cache(ctx, Q, K, H, G, D, window, sinks, 
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("Q", [1, 5, 64, 200])
+@pytest.mark.parametrize("Q", [1, 5, 23, 64, 200])
 def test_attention_far_from_its_keys(ctx, Q, dtype):
     """Positions in front of and behind all keys, up to the ends of int32: rows that see nothing give zeros."""
     for first, window, sinks in (([-5, 2 ** 31 - 1], (3, 3), 0), ([-(2 ** 31), 90], (2 ** 31 - 1, 2 ** 31 - 1), 0), ([50, 60], (0, 0), 7), ([2 ** 31 - 1, 200], (10, 0), 2)):
@@ -304,7 +304,7 @@ def test_attention_far_from_its_keys(ctx, Q, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("Q,K", [(1, 300), (4, 90), (90, 90), (260, 260)])
+@pytest.mark.parametrize("Q,K", [(1, 300), (4, 90), (20, 90), (20, 2500), (90, 90), (260, 260)])
 def test_attention_does_not_touch_what_no_query_sees(ctx, Q, K, dtype):
     """NaN and infinities behind the lengths and outside all windows; scores of any scale; a scale of zero."""
     t, gen = TYPES[dtype], _gen(Q + K)
@@ -326,7 +326,7 @@ def test_attention_does_not_touch_what_no_query_sees(ctx, Q, K, dtype):
         O.close(out, want, t, floor=_attention_floor(q, kz, vz, t, abs(0.125 if scale is None else scale)))
 
 
-@pytest.mark.parametrize("Q", [1, 8, 150])
+@pytest.mark.parametrize("Q", [1, 8, 20, 150])
 @pytest.mark.parametrize("magnitude", [1e-20, 1e-6, 1e-3, 300.0, 1e5, 1e15])
 def test_attention_fp32_of_any_magnitude(ctx, Q, magnitude):
     """Values, and keys with the scale against them, far outside the range of half the bits; one key far above the others."""
