@@ -313,9 +313,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     const uint32_t tmem = s_tmem;
     float4* s_o = reinterpret_cast<float4*>(smem + kSlots * F::kTile);   // the CTA's part of the result, [row][column / 4], the columns of a row turned
     auto out_place = [](uint32_t r, uint32_t c4) -> uint32_t { return r * (DP / 4) + (c4 ^ (r & (DP / 4 - 1))); };
-    auto write_row = [&](uint32_t r, uint32_t c, const float4& v) {   // four elements from column c
+    auto row_at = [&](uint32_t r) -> T* {   // where a row goes
         const uint32_t row = r0 + r, qi = per_head(row), head = g * per_head.d + (row - qi * per_head.d);
-        T* p = static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head + c;
+        return static_cast<T*>(a.out) + (int64_t)b * a.out_batch + (int64_t)qi * a.out_token + (int64_t)head * a.out_head;
+    };
+    auto write_row = [&](uint32_t r, uint32_t c, const float4& v) {   // four elements from column c
+        T* p = row_at(r) + c;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = v;
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
     };
@@ -574,11 +577,19 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             s_l[r] = l;
         } else {   // the warp's rows, whole lines at a time
             __syncwarp();
-            constexpr uint32_t kPerO = DP / 4;
-            const uint32_t c4 = lane % kPerO;
+            constexpr uint32_t kE = kPer16<T>, kPerO = DP / kE;   // pieces of 16 bytes a row
+            const uint32_t c = lane % kPerO * kE;
 #pragma unroll 4
-            for (uint32_t i = lane / kPerO; i < 32; i += 32 / kPerO)
-                if (warp_row + i < n_rows && c4 * 4 < dim) write_row(warp_row + i, c4 * 4, s_o[out_place(warp_row + i, c4)]);
+            for (uint32_t i = lane / kPerO; i < 32; i += 32 / kPerO) {
+                if (warp_row + i >= n_rows || c >= dim) continue;
+                float v[kE];
+#pragma unroll
+                for (uint32_t e = 0; e < kE; e += 4) {
+                    const float4 x = s_o[out_place(warp_row + i, (c + e) / 4)];
+                    v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
+                }
+                store_elems<T, kE>(row_at(warp_row + i) + c, v);
+            }
         }
     } else if (warp < F::kIssueAt) {
         // ---------------------------------------------------------------- keys and values into shared memory
