@@ -188,7 +188,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     __shared__ __align__(8) RowBars s_row[RT];
     __shared__ uint32_t s_tmem, s_abort, s_top[RT][3][4];
     __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most four tiles ahead of who reads these
-    __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_part[kMostShares][RT * kRows];
+    __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_join[FEW ? 2 : 1][32];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -321,6 +321,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         T* p = row_at(r) + c;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = v;
         else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
+    };
+
+    auto add_part = [](float4& v, float& total, const float4& x, float l, float f) {   // a part that counts f times
+        if (f != 0.f) { v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w); }
+        total += f == 0.f ? (l != l ? l : 0.f) : l * f;   // a sum that is no number stays one
     };
 
     if (warp < F::kRowWarps) {
@@ -754,67 +759,50 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         __syncthreads();
         for (uint32_t i = tid; i < n_rows * (DP / 4); i += kThreads) {
             const uint32_t r = i / (DP / 4), c = i % (DP / 4);
-            float mk[4], top = -INFINITY;
+            float mk[4], top = -INFINITY, total = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < 4; ++w) top = fmaxf(top, mk[w] = s_m[w * 32 + r]);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float4 x = s_o[out_place(w * 32 + r, c)];
-                const float f = mk[w] == -INFINITY ? 0.f : exp2_approx(mk[w] - top);
-                if (f != 0.f) { v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w); }
-            }
+            for (int w = 0; w < 4; ++w) add_part(v, total, s_o[out_place(w * 32 + r, c)], s_l[w * 32 + r], mk[w] == -INFINITY ? 0.f : exp2_approx(mk[w] - top));
             s_o[out_place(r, c)] = v;
-        }
-        __syncthreads();
-        if (tid < n_rows) {
-            float top = s_m[tid], total = 0.f;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * 32 + tid]);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float mk = s_m[w * 32 + tid], lk = s_l[w * 32 + tid], f = mk == -INFINITY ? 0.f : exp2_approx(mk - top);
-                total += f == 0.f ? (lk != lk ? lk : 0.f) : lk * f;
+            if (c == 0) {
+                s_join[0][r] = top;
+                s_join[FEW][r] = total;
             }
-            s_m[tid] = top;
-            s_l[tid] = total;
         }
     }
-    if (FEW || shares > 1) {
+    if (FEW || shares > 1) {   // the CTAs' parts, four at a time on their way
         if (shares > 1) cluster_sync(); else __syncthreads();
-        if (tid < n_rows) {   // what each part of a row counts for in the result
-            float mk[kMostShares], lk[kMostShares], top = -INFINITY, total = 0.f;
+        const float *from_m = FEW ? s_join[0] : s_m, *from_l = FEW ? s_join[FEW] : s_l;
+        for (uint32_t i = share * kThreads + tid; i < n_rows * (DP / 4); i += shares * kThreads) {
+            const uint32_t r = i / (DP / 4), c = i % (DP / 4), at_o = smem_u32(&s_o[out_place(r, c)]), at_m = smem_u32(from_m + r), at_l = smem_u32(from_l + r);
+            if (c * 4 >= dim) continue;
+            float top = -INFINITY, total = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t k0 = 0; k0 < shares; k0 += 4) {
+                float mk[4], lk[4], most = top;
+                float4 x[4];
 #pragma unroll
-            for (uint32_t k = 0; k < kMostShares; ++k) {
-                mk[k] = k < shares ? load_shared_cluster(map_to_rank(smem_u32(&s_m[tid]), k)) : -INFINITY;
-                lk[k] = k < shares ? load_shared_cluster(map_to_rank(smem_u32(&s_l[tid]), k)) : 0.f;
-                top = fmaxf(top, mk[k]);
-            }
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const bool in = k0 + k < shares;
+                    mk[k] = in ? load_shared_cluster(map_to_rank(at_m, k0 + k)) : -INFINITY;
+                    lk[k] = in ? load_shared_cluster(map_to_rank(at_l, k0 + k)) : 0.f;
+                    x[k] = in ? load_shared_cluster4(map_to_rank(at_o, k0 + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
 #pragma unroll
-            for (uint32_t k = 0; k < kMostShares; ++k) {
-                mk[k] = mk[k] == -INFINITY ? 0.f : exp2_approx(mk[k] - top);
-                total += mk[k] == 0.f ? (lk[k] != lk[k] ? lk[k] : 0.f) : lk[k] * mk[k];   // a sum that is no number stays one
+                for (uint32_t k = 0; k < 4; ++k) most = fmaxf(most, mk[k]);
+                const float4 before = v;
+                const float total_before = total, f = top == -INFINITY ? 0.f : exp2_approx(top - most);
+                v = make_float4(0.f, 0.f, 0.f, 0.f);
+                total = 0.f;
+                add_part(v, total, before, total_before, f);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) add_part(v, total, x[k], lk[k], mk[k] == -INFINITY ? 0.f : exp2_approx(mk[k] - most));
+                top = most;
             }
             const float norm = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-            for (uint32_t k = 0; k < kMostShares; ++k)
-                if (k < shares) s_part[k][tid] = mk[k] == 0.f && norm == norm ? 0.f : mk[k] * norm;
-        }
-        __syncthreads();
-        for (uint32_t i = share * kThreads + tid; i < n_rows * (DP / 4); i += shares * kThreads) {
-            const uint32_t r = i / (DP / 4), c = i % (DP / 4), at_o = smem_u32(&s_o[out_place(r, c)]);
-            if (c * 4 >= dim) continue;
-            float4 x[kMostShares], v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (uint32_t k = 0; k < kMostShares; ++k)
-                if (k < shares) x[k] = load_shared_cluster4(map_to_rank(at_o, k));
-#pragma unroll
-            for (uint32_t k = 0; k < kMostShares; ++k)
-                if (k < shares) {
-                    const float f = s_part[k][r];
-                    if (f != 0.f) { v.x = fmaf(x[k].x, f, v.x); v.y = fmaf(x[k].y, f, v.y); v.z = fmaf(x[k].z, f, v.z); v.w = fmaf(x[k].w, f, v.w); }
-                }
-            write_row(r, c * 4, v);
+            write_row(r, c * 4, make_float4(v.x * norm, v.y * norm, v.z * norm, v.w * norm));
         }
         if (shares > 1) cluster_sync();   // what the others read is read
     }
