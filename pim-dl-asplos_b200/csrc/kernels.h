@@ -207,10 +207,10 @@ struct AttentionArgs {
     bool vec;                         // rows of all four tensors start on 16 bytes
 };
 // Few rows (query tokens x heads of a key head), up to eight of them in one pass over keys and values, on the CUDA cores.  fp32, for which the
-// tensor cores take three products and a conversion, eight rows of 8 x 8192 keys, 16 heads of 128 (of 64): 314 us (174) there, 361 (156) on
-// the tensor cores; twelve 569 (301) and 361 (156).  bf16, one row of heads of 64: 55 and 54 us, of a few hundred keys 17 and 28, two 80 and 54.  What does not start on 16 bytes goes there
-// too, element by element.
-constexpr uint64_t attention_few_rows(size_t element) { return element == 4 ? 8 : 1; }
+// tensor cores take three products and a conversion, eight rows of 8 x 8192 keys, 16 heads of 128: 313 us there, 360 on the tensor cores, of 64:
+// 173 and 153; twelve 569 (of 64 301) and 360 (153).  bf16, one row of heads of 64: 55 and 54 us, of 64 x 197 keys 17 and 28, two 80 and 53.  What does not
+// start on 16 bytes goes there too, element by element.
+constexpr uint64_t attention_few_rows(size_t element, uint32_t head_dim) { return element == 2 ? 1 : head_dim > 64 ? 8 : 4; }
 cudaError_t launch_attention_rows(const AttentionArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
 // Many rows: on the tensor cores.
 cudaError_t launch_attention_umma(const AttentionArgs& a, uint32_t dtype, int sm_count, uint32_t* dev_err, cudaStream_t s);
