@@ -347,30 +347,47 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             float up = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
             if (a.scale == 0.f) factor = 1.f;
             if constexpr (F::kParts == 2) {   // the power of two is the row's
-                uint32_t top = 0;
-                auto look = [&](uint32_t bits) {
-                    bits &= 0x7FFFFFFFu;
-                    if (bits < 0x7F800000u) top = max(top, bits);
-                };
+                float big = 0.f;   // (what is no number is passed over here, and is itself in both parts)
 #pragma unroll
-                for (int i = 0; i < kPerQ; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
+                for (int i = 0; i < kPerQ; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(&raw[i]);
+                    big = max3(big, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
+                }
+                uint32_t top = __float_as_uint(big);
+                const bool infinite = __any_sync(0xffffffffu, top >= 0x7F800000u);
+                if (infinite) {   // the largest that is a number
+                    top = 0;
+                    auto look = [&](uint32_t bits) {
+                        bits &= 0x7FFFFFFFu;
+                        if (bits < 0x7F800000u) top = max(top, bits);
+                    };
+#pragma unroll
+                    for (int i = 0; i < kPerQ; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
+                }
                 const int e = exponent_for(top);
                 up *= power2(e);
                 factor *= power2(-e);
-            }
+                const uint64_t up2 = pair(up, up);
+                auto convert = [&](auto split) {   // 16 elements: 8 columns of either part
 #pragma unroll
-            for (int part = 0; part < kPerQ / 4; ++part) {   // 4 E elements: 16 columns of 16-bit types, 8 and 8 of fp32
-                if constexpr (F::kParts == 2) {
-                    uint32_t hi[8], lo[8];
+                    for (int part = 0; part < kPerQ / 4; ++part) {
+                        uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 w = raw[part * 4 + i];
-                        split2_any(__uint_as_float(w.x) * up, __uint_as_float(w.y) * up, hi[2 * i], lo[2 * i]);
-                        split2_any(__uint_as_float(w.z) * up, __uint_as_float(w.w) * up, hi[2 * i + 1], lo[2 * i + 1]);
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 x = *reinterpret_cast<const float4*>(&raw[part * 4 + i]);
+                            const float2 front = unpair(mul2(pair(x.x, x.y), up2)), back = unpair(mul2(pair(x.z, x.w), up2));
+                            split(front.x, front.y, hi[2 * i], lo[2 * i]);
+                            split(back.x, back.y, hi[2 * i + 1], lo[2 * i + 1]);
+                        }
+                        tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
+                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, lo);
                     }
-                    tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
-                    tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, lo);
-                } else {
+                };
+                if (infinite) convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2_any(x, y, hi, lo); });
+                else convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, hi, lo); });
+            } else {
+#pragma unroll
+                for (int part = 0; part < kPerQ / 4; ++part) {   // 32 elements: 16 columns
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
