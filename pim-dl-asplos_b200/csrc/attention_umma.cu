@@ -18,9 +18,9 @@
 // converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
 // CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no scratch memory and one order of summation.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 97 us, 346 TFLOP/s; of 2900 warp instructions a
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 96 us, 349 TFLOP/s; of 2850 warp instructions a
 // tile 680 form its weights.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 32 us, 540 TFLOP/s.  fp32,
-// three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 96 us, of which a CTA spends half before its first and behind its last tile.
+// three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 92 us, of which a CTA spends half before its first and behind its last tile.
 #include "attention.cuh"
 #include "ptx.cuh"
 
@@ -176,7 +176,7 @@ Divisor divisor(uint32_t d) {
 }
 
 // FEW: at most 32 rows.  All four warps of rows have them, each with sixteen keys of every tile and an output of its own; they join in the end.  One warp with
-// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 55 us so, 49 with four warps, 5.5 TB/s.
+// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 55 us so, 48 with four warps, 5.5 TB/s.
 template <typename T, int DP, int RT, bool FEW>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
@@ -872,8 +872,8 @@ cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaSt
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads);
     if (rows <= 32) return a.head_dim > 64 ? run<T, 128, 1, true>(a, sm_count, dev_err, s) : run<T, 64, 1, true>(a, sm_count, dev_err, s);
     if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
-    // fp32's keys and values are converted once for 256 rows (ViT's batch 101 us with 128, 96 with 256; BERT-large's 98 and 79); 16-bit types, which are only
-    // copied, do better with two CTAs of 128 rows on an SM (8192 tokens in bf16 97 us, 106 with 256).
+    // fp32's keys and values are converted once for 256 rows (ViT's batch 97 us with 128, 92 with 256; BERT-large's 94 and 76); 16-bit types, which are only
+    // copied, do better with two CTAs of 128 rows on an SM (8192 tokens in bf16 96 us, 107 with 256).
     if constexpr (sizeof(T) == 4) {
         if (rows > kRows) return run<T, 64, 2>(a, sm_count, dev_err, s);
     }
