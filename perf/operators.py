@@ -170,11 +170,14 @@ _ctx = None
 
 
 def _context():
-    """What a process keeps: one context on the GPU."""
+    """What a process keeps: one context on the GPU, on the stream that makes the inputs and reads the outputs."""
     global _ctx
     if _ctx is None:
         import pim_dl_asplos_b200 as P
         _ctx = P.LutAmmContext(0)
+    stream = torch.cuda.current_stream().cuda_stream or 1   # 0, torch's default stream, would be the context's own: 1 is CUDA's handle for it
+    if _ctx.stream != stream:
+        _ctx.set_stream(stream)
     return _ctx
 
 
