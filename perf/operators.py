@@ -175,9 +175,8 @@ def _context():
     if _ctx is None:
         import pim_dl_asplos_b200 as P
         _ctx = P.LutAmmContext(0)
-    stream = torch.cuda.current_stream().cuda_stream or 1   # 0, torch's default stream, would be the context's own: 1 is CUDA's handle for it
-    if _ctx.stream != stream:
-        _ctx.set_stream(stream)
+        # 0, torch's default stream, would be the context's own: 1 is CUDA's handle for it
+        _ctx.set_stream(torch.cuda.current_stream().cuda_stream or 1)
     return _ctx
 
 
