@@ -410,7 +410,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const uint32_t full_from = sink_tiles + (uint32_t)max(0, (common_lo - span.lo + kKeys - 1) / kKeys);
         const uint32_t full_to = sink_tiles + (uint32_t)max(0, (min(span.hi, common_hi) - span.lo) / kKeys);
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
-        const uint32_t out_at = my_tmem + F::kProduct;
+        const uint32_t out_at = my_tmem + F::kProduct, columns = (dim + 15) / 16 * 16;   // the products write those; behind them lies what other kernels left
         // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is in shared memory, against m_o
         float m_o = -INFINITY;
         int unit = 0;
@@ -419,7 +419,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         auto add_chunk = [&](bool chunk, float norm) {
             const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm, up = power2(-unit) * norm;
 #pragma unroll 2
-            for (uint32_t col = 0; col < DP; col += 16) {
+            for (uint32_t col = 0; col < columns; col += 16) {
                 uint32_t v[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] = 0;
@@ -517,7 +517,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     if constexpr (F::kParts == 2) {
                         float big = 0.f;
 #pragma unroll 1
-                        for (uint32_t col = 0; col < DP; col += 16) {
+                        for (uint32_t col = 0; col < columns; col += 16) {
                             uint32_t v[16];
                             tmem_ld_32x32b_x16(out_at + col, v);
                             tmem_ld_wait();
@@ -532,7 +532,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         }
                     }
 #pragma unroll 1
-                    for (uint32_t col = 0; col < DP; col += 16) {
+                    for (uint32_t col = 0; col < columns; col += 16) {
                         uint32_t v[16];
                         tmem_ld_32x32b_x16(out_at + col, v);
                         tmem_ld_wait();
