@@ -507,6 +507,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             float more = kBoost;   // log2 of what this tile's weights carry
             if (m == -INFINITY) m = top;
             if (!begun || m == -INFINITY) unit = e;
+            if (top == -INFINITY) e = unit;   // none of this tile's values is this row's: its output stays as it is
             if (__any_sync(0xffffffffu, top > m + kSlack || unit != e)) {
                 const float m_new = top > m + kSlack ? top : m;
                 const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
@@ -525,9 +526,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                             for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
                         }
                         // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
-                        const int x = max(-120, min(120, e - unit));
-                        if (x <= 0 || big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2))) {
-                            f *= power2(x);
+                        const int x = e - unit;   // -232 .. 232: as two factors
+                        if (x <= 0 || (x <= 120 && big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2)))) {
+                            f *= power2(x / 2) * power2(x - x / 2);
                             unit = e;
                         }
                     }

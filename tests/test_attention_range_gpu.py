@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import dense_oracle as O
+
 pytestmark = pytest.mark.gpu
 ROWS = [1, 3, 6, 20, 100, 200]   # one, few and many rows: every kernel and form
 
@@ -40,3 +42,17 @@ def test_what_other_kernels_left_in_tensor_memory(ctx, Q, D):
         _fill_tensor_memory(ctx, value)
         outs.append(_run(ctx, q, k, v))
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("Q", ROWS)
+def test_a_tile_of_large_values_that_half_of_the_rows_do_not_see(ctx, Q):
+    """Values of 1e-27 in one tile, of 1e30 in the next: rows that see the first alone have theirs."""
+    q, k, v = _inputs(7, Q, 128, 64)
+    v[0, :64] *= 1e-27
+    v[0, 64:] *= 1e30
+    first = 63 - Q // 2
+    got, want = _run(ctx, q, k, v, first=[first], window=(63, 0)), O.attention(q, k, v, None, (63, 0), 0, None, [first])
+    rows = max(0, min(Q, 64 - first))
+    # fp32 all the way: 64 products and sums of a score and its exponential, 64 of the result
+    O.close(got[:, :rows], want[:, :rows], torch.float32, floor=256 * 2.0 ** -24 * float(v[0, :64].abs().amax()))
+    assert got.isfinite().all()
