@@ -9,10 +9,11 @@
 // weights are formed against the old m.  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
 // Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.  fp32 operands are split into
-// two f16 numbers, x = hi + lo to 22 bits, and hi hi + hi lo + lo hi is summed; the product of the rests, 2^-22 of the whole, is left out.  f16 ends at
-// 65504 and thins out below 2^-14, so operands carry a power of two: queries one per row, keys and values one per tile, kept from tile to tile for as long
-// as the tile's largest value lies in 1/4 .. 32768 under it.  Weights carry 2^6 and up to 2^8 more, the sum l with them.  Maxima, sums and outputs
-// are fp32; the rescaling of the output in tensor memory, and the sum over tiles that fp32 takes out of it (kChunk), round once each.
+// three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
+// its size.  Of the nine products the six down to 2^-16 of the whole are summed, the small ones first; b c + c b, 2^-25 of it, is left out.  So an element's
+// digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  In 16 bits weights
+// carry 2^6 and up to 2^8 more, the sum l with them.  Maxima, sums and outputs are fp32; maxima are taken up to whole numbers, so that what is against an older
+// one is brought in line without rounding; the sum over tiles that fp32 makes outside of tensor memory rounds once each.
 //
 // Loading warps copy 16 bytes a piece (cp.async): no tensor maps to be made by the host, and rows behind the last key become zeros.  fp32 is
 // converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
@@ -33,25 +34,26 @@ namespace {
 constexpr int kRows = 128, kKeys = 64;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
 constexpr uint32_t kMostShares = 8;
-// Tensor memory adds up towards zero: each of a tile's twelve products takes half a unit of the sum off, 3.5e-7 of it a tile.  fp32's output is taken out
-// and summed with rounding every other tile: 4000 keys of values around 0 (around 1) come out 5.0e-7 (4.8e-7) off, plain fp32 4.8e-7 (1.2e-7); every
-// four tiles 9.2e-7 (1.2e-6), every eight 1.8e-6 (2.8e-6), never 1.8e-6 (1.3e-5 at 16000 keys).  Half the bits do not show it.
-constexpr uint32_t kChunk = 2;
+// Tensor memory adds up towards zero: fp32's product of a tile takes four units of 2^-24 off the sum at most, its small terms being first, and would take
+// twenty-four off with the tiles before in there.  So each tile's is taken out and summed with rounding.  Half the bits do not show it.
 constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 // DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
 template <typename T, int DP, int RT>
 struct Form {
-    static constexpr int kParts = sizeof(T) == 4 ? 2 : 1, kPanels = DP / 64;
-    static constexpr int kTile = kParts * kPanels * kPanel;          // bytes of a tile of keys or values
-    static constexpr int kSlots = RT == 1 && sizeof(T) == 4 ? 4 : 8;       // of the ring that keys and values take by turns
-    static constexpr int kAhead = RT == 2 ? 2 : sizeof(T) == 4 ? 2 : 4;    // tiles that a warpgroup has on their way
-    static constexpr int kOut = RT * kRows * DP * 4;                 // bytes of the output, in fp32: queries come, and results leave, through there
+    static constexpr bool kFp32 = sizeof(T) == 4;
+    static constexpr int kParts = kFp32 ? 3 : 1, kPanels = DP / 64;
+    static constexpr int kPart = kPanels * kPanel, kTile = kParts * kPart;   // bytes of a part of a tile of keys or values, of the tile
+    static constexpr int kSlots = !kFp32 ? 8 : RT == 2 ? 6 : 3;              // of the ring that keys and values take by turns
+    static constexpr int kAhead = kFp32 ? 1 : 4;                             // tiles that a warpgroup has on their way
+    static constexpr int kOut = RT * kRows * DP * 4;                         // bytes of the output, in fp32: queries come, and results leave, through there
     static constexpr int kSmem = kSlots * kTile + kOut + 1024;
-    static constexpr bool kSums = sizeof(T) == 4;                    // sums of products over the tiles outside tensor memory: see kChunk
-    static constexpr int kScores = 0, kProduct = 2 * kKeys, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;   // columns of a tile of rows
+    // Columns of tensor memory of a tile of rows: scores, over which its weights are written, kBufs times; the product; the queries.  Where two buffers of scores
+    // find no room, the next tile's are formed behind the product, while the other tile of rows, or the other CTA on the SM, has its weights formed.
+    static constexpr int kScoreCols = kFp32 ? 96 : 64, kBufs = kFp32 && DP <= 64 ? 1 : 2;
+    static constexpr int kScores = 0, kProduct = kBufs * kScoreCols, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
-    static_assert(RT == 1 || kUsed <= 256);
+    static_assert(RT * kUsed <= 512 && (RT == 1 || kUsed <= 256));
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
     // Warpgroups: one for each tile of rows, a row a thread, one for each tile of rows that loads, one that issues.  Registers a thread of each; their sum is
     // what the warpgroups are launched with, and none of them spills (the issuing warps did with 24: 24 rows of 8 x 8192 keys in bf16 59.9 us, 54.4 so).
@@ -75,7 +77,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 }
 template <typename T>
 __device__ __forceinline__ uint32_t idesc_f16(uint32_t n) {
-    constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t bf = std::is_same<T, __half>::value ? 0u : 1u;
     return (1u << 4) | (bf << 7) | (bf << 10) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
 }
 // B whose rows are the contraction axis: 64 elements, one swizzle row of 128 bytes, a row; eight rows a group.
@@ -84,9 +86,6 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t smem_addr) {
 }
 
 __device__ __forceinline__ void sync_128(uint32_t id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
-// The power of two that takes a largest value to 8 .. 16, up to 2^108 (results below 1e-32 have fewer bits); 0 for 0.
-__device__ __forceinline__ int exponent_for(uint32_t top_bits) { return top_bits == 0 ? 0 : min(108, 130 - (int)(top_bits >> 23)); }
 // A warp's bounded wait, with one answer.  The hint lets the hardware hold a waiting warp for up to two microseconds a look: without it the fifteen warps
 // of a CTA that wait for one another took a third of all instructions.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word) {
@@ -136,19 +135,31 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// x = hi + lo in f16, two at a time
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pack2(a, b, static_cast<__half*>(nullptr));
-    const float2 h = unpack2(hi, static_cast<__half*>(nullptr));
-    const float2 rest = unpair(fma2(pair(h.x, h.y), pair(-1.f, -1.f), pair(a, b)));
-    lo = pack2(rest.x, rest.y, static_cast<__half*>(nullptr));
+// x = hi + mid + lo in bf16, two at a time: hi cut off, which no finite number makes an infinity of, the others to nearest
+__device__ __forceinline__ void split3(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    const uint64_t minus = pair(-1.f, -1.f);
+    const float2 h = unpack2(hi, static_cast<__nv_bfloat16*>(nullptr));
+    const float2 rest = unpair(fma2(pair(h.x, h.y), minus, pair(a, b)));
+    mid = pack2(rest.x, rest.y, static_cast<__nv_bfloat16*>(nullptr));
+    const float2 m = unpack2(mid, static_cast<__nv_bfloat16*>(nullptr));
+    const float2 last = unpair(fma2(pair(m.x, m.y), minus, pair(rest.x, rest.y)));
+    lo = pack2(last.x, last.y, static_cast<__nv_bfloat16*>(nullptr));
 }
-// ... of numbers that may be infinite: their rest is none
-__device__ __forceinline__ void split2_any(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pack2(a, b, static_cast<__half*>(nullptr));
-    const float2 h = unpack2(hi, static_cast<__half*>(nullptr));
-    const float x = a - h.x, y = b - h.y;
-    lo = pack2(x == x ? x : 0.f, y == y ? y : 0.f, static_cast<__half*>(nullptr));
+// ... of numbers that may be infinite: their rests are none
+__device__ __forceinline__ void split3_any(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    split3(a, b, hi, mid, lo);
+    const uint32_t keep = (fabsf(a) == INFINITY ? 0u : 0xFFFFu) | (fabsf(b) == INFINITY ? 0u : 0xFFFF0000u);
+    mid &= keep;
+    lo &= keep;
+}
+// 0, or NaN where one of the numbers is none or infinite: what is added to `odd`
+__device__ __forceinline__ uint64_t look(const float4& x, uint64_t odd) {
+    return fma2(pair(x.x, x.y), pair(0.f, 0.f), fma2(pair(x.z, x.w), pair(0.f, 0.f), odd));
+}
+__device__ __forceinline__ bool is_odd(uint64_t odd) {
+    const float2 v = unpair(odd);
+    return v.x + v.y != 0.f;
 }
 
 // ones below bit n
@@ -186,8 +197,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     extern __shared__ unsigned char s_raw[];
     __shared__ __align__(8) uint64_t s_full_bar[kSlots], s_empty_bar[kSlots];
     __shared__ __align__(8) RowBars s_row[RT];
-    __shared__ uint32_t s_tmem, s_abort, s_top[RT][3][4];
-    __shared__ int32_t s_exp_k[8], s_exp_v[8];   // by tile: the loading warps are at most four tiles ahead of who reads these
+    __shared__ uint32_t s_tmem, s_abort;
     __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_join[FEW ? 2 : 1][32];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
@@ -253,7 +263,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const T* from = base + (int64_t)(k0 + (int32_t)my_row) * token + (in_dim ? my_col : 0);
         const int64_t step = token * kStepRows;
         const uint32_t at = smem_at + job % kSlots * F::kTile;
-        auto to = [&](int i) -> uint32_t { return at + (F::kParts == 2 ? i * 2048 + t * 16 : place_of(i)); };   // (fp32: to where this thread alone reads it)
+        auto to = [&](int i) -> uint32_t { return at + (F::kFp32 ? i * 2048 + t * 16 : place_of(i)); };   // (fp32: to where this thread alone reads it)
         if ((uint32_t)k0 + kKeys <= (uint32_t)end && (k0 >= gap_to || (uint32_t)k0 + kKeys <= (uint32_t)gap_from)) {
             const uint32_t size = in_dim ? 16u : 0u;
 #pragma unroll
@@ -341,57 +351,41 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         {
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
-            uint4 raw[kPerQ];
-#pragma unroll
-            for (int i = 0; i < kPerQ; ++i) raw[i] = *reinterpret_cast<const uint4*>(smem + q_stage + (lane * kPerQ + (i ^ (lane & (kPerQ - 1)))) * 16);
-            float up = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+            auto raw = [&](int i) -> uint4 { return *reinterpret_cast<const uint4*>(smem + q_stage + (lane * kPerQ + (i ^ (lane & (kPerQ - 1)))) * 16); };
+            auto raw4 = [&](int i) -> float4 { const uint4 u = raw(i); return *reinterpret_cast<const float4*>(&u); };
+            const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
             if (a.scale == 0.f) factor = 1.f;
-            if constexpr (F::kParts == 2) {   // the power of two is the row's
-                float big = 0.f;   // (what is no number is passed over here, and is itself in both parts)
+            if constexpr (F::kFp32) {
+                uint64_t odd = 0;
 #pragma unroll
-                for (int i = 0; i < kPerQ; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(&raw[i]);
-                    big = max3(big, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
-                }
-                uint32_t top = __float_as_uint(big);
-                const bool infinite = __any_sync(0xffffffffu, top >= 0x7F800000u);
-                if (infinite) {   // the largest that is a number
-                    top = 0;
-                    auto look = [&](uint32_t bits) {
-                        bits &= 0x7FFFFFFFu;
-                        if (bits < 0x7F800000u) top = max(top, bits);
-                    };
-#pragma unroll
-                    for (int i = 0; i < kPerQ; ++i) { look(raw[i].x); look(raw[i].y); look(raw[i].z); look(raw[i].w); }
-                }
-                const int e = exponent_for(top);
-                up *= power2(e);
-                factor *= power2(-e);
-                const uint64_t up2 = pair(up, up);
-                auto convert = [&](auto split) {   // 16 elements: 8 columns of either part
-#pragma unroll
+                for (int i = 0; i < kPerQ; ++i) odd = look(raw4(i), odd);
+                const uint64_t sign2 = pair(sign, sign);
+                auto convert = [&](auto split) {   // 16 elements: 8 columns of each part
+#pragma unroll 1
                     for (int part = 0; part < kPerQ / 4; ++part) {
-                        uint32_t hi[8], lo[8];
+                        uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float4 x = *reinterpret_cast<const float4*>(&raw[part * 4 + i]);
-                            const float2 front = unpair(mul2(pair(x.x, x.y), up2)), back = unpair(mul2(pair(x.z, x.w), up2));
-                            split(front.x, front.y, hi[2 * i], lo[2 * i]);
-                            split(back.x, back.y, hi[2 * i + 1], lo[2 * i + 1]);
+                            const float4 x = raw4(part * 4 + i);
+                            const float2 front = unpair(mul2(pair(x.x, x.y), sign2)), back = unpair(mul2(pair(x.z, x.w), sign2));
+                            split(front.x, front.y, hi[2 * i], mid[2 * i], lo[2 * i]);
+                            split(back.x, back.y, hi[2 * i + 1], mid[2 * i + 1], lo[2 * i + 1]);
                         }
                         tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
-                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, lo);
+                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, mid);
+                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP + part * 8, lo);
                     }
                 };
-                if (infinite) convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2_any(x, y, hi, lo); });
-                else convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, hi, lo); });
+                if (__any_sync(0xffffffffu, is_odd(odd))) convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3_any(x, y, hi, mid, lo); });
+                else convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3(x, y, hi, mid, lo); });
             } else {
 #pragma unroll
                 for (int part = 0; part < kPerQ / 4; ++part) {   // 32 elements: 16 columns
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t u[4] = {raw[part * 4 + i].x, raw[part * 4 + i].y, raw[part * 4 + i].z, raw[part * 4 + i].w};
+                        const uint4 r = raw(part * 4 + i);
+                        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) w[4 * i + k] = a.scale > 0.f ? u[k] : a.scale < 0.f ? u[k] ^ 0x80008000u : 0u;
                     }
@@ -411,13 +405,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const uint32_t full_to = sink_tiles + (uint32_t)max(0, (min(span.hi, common_hi) - span.lo) / kKeys);
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
         const uint32_t out_at = my_tmem + F::kProduct, columns = (dim + 15) / 16 * 16;   // the products write those; behind them lies what other kernels left
-        // fp32: the output of the tiles since the last chunk's end is the one in tensor memory * 2^-unit; that of those before is in shared memory, against m_o
+        // fp32: the output of the last tile is in tensor memory; that of those before in shared memory, against m_o
         float m_o = -INFINITY;
-        int unit = 0;
         bool o_any = false;
         // ... both together, times norm
         auto add_chunk = [&](bool chunk, float norm) {
-            const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm, up = power2(-unit) * norm;
+            const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm;
 #pragma unroll 2
             for (uint32_t col = 0; col < columns; col += 16) {
                 uint32_t v[16];
@@ -430,8 +423,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     float4& at = s_o[out_place(r, (col + i) / 4)];
-                    float4 x = make_float4(__uint_as_float(v[i]) * up, __uint_as_float(v[i + 1]) * up, __uint_as_float(v[i + 2]) * up, __uint_as_float(v[i + 3]) * up);
-                    if (F::kSums && o_any) {
+                    float4 x = make_float4(__uint_as_float(v[i]) * norm, __uint_as_float(v[i + 1]) * norm, __uint_as_float(v[i + 2]) * norm, __uint_as_float(v[i + 3]) * norm);
+                    if (F::kFp32 && o_any) {
                         const float4 y = at;
                         x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
                     }
@@ -444,6 +437,13 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         uint32_t n = 0;   // tiles so far
         for (uint32_t j = 0; j < tiles; ++j) {
             if (RT == 2 && !sees(t0 + j)) continue;
+            if constexpr (F::kFp32) {
+                if (n > 0 && first_row < n_rows) {   // the last tile's output, while this one's scores are formed
+                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
+                    tc_fence_after_sync();
+                    add_chunk(true, 1.f);
+                }
+            }
             if (!wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
             tc_fence_after_sync();
             if (first_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
@@ -451,25 +451,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 ++n;
                 continue;
             }
-            const uint32_t at = my_tmem + F::kScores + (n & 1u) * kKeys;
-            bool begun = n > 0;   // whether tensor memory holds an output to go on with
-            if constexpr (F::kSums) {
-                begun = n % kChunk != 0;
-                if (n > 0 && !begun) {
-                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
-                    tc_fence_after_sync();
-                    add_chunk(true, 1.f);
-                }
-            }
-            float c = factor;
-            int e = 0;
-            if constexpr (F::kParts == 2) {
-                c *= power2(-s_exp_k[j % 8]);
-                // the values' power of two is known once they are in shared memory, which the keys' turn does not wait for
-                if (!wait_warp(smem_u32(&s_full_bar[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort)) break;
-                e = s_exp_v[j % 8];
-            }
-            c = fmaxf(c, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
+            const uint32_t at = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
+            const float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             constexpr int kGroups = FEW ? 1 : 2, kWide = FEW ? 16 : 32;
             uint32_t sc[kGroups][kWide];
             if constexpr (FEW) {
@@ -503,84 +486,66 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     }
                 top = fmaxf(x, y) * c;
             }
-            // Another maximum, or another power of two of the values: the output so far is brought in line, where there is one.
-            float more = kBoost;   // log2 of what this tile's weights carry
-            if (m == -INFINITY) m = top;
-            if (!begun || m == -INFINITY) unit = e;
-            if (top == -INFINITY) e = unit;   // none of this tile's values is this row's: its output stays as it is
-            if (__any_sync(0xffffffffu, top > m + kSlack || unit != e)) {
-                const float m_new = top > m + kSlack ? top : m;
-                const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
-                if (begun) {
-                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
-                    tc_fence_after_sync();
-                    float f = shrink;
-                    if constexpr (F::kParts == 2) {
-                        float big = 0.f;
+            top = ceilf(top);
+            if constexpr (F::kFp32) {
+                const float m_new = fmaxf(m, top);
+                l *= m == -INFINITY ? 1.f : exp2_approx(m - m_new);
+                m = m_new;
+            } else {
+                // A maximum that has grown by far: the output so far is brought in line, where there is one.
+                if (m == -INFINITY) m = top;
+                if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                    const float m_new = top > m + kSlack ? top : m;
+                    const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
+                    if (n > 0) {
+                        if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
+                        tc_fence_after_sync();
 #pragma unroll 1
                         for (uint32_t col = 0; col < columns; col += 16) {
                             uint32_t v[16];
                             tmem_ld_32x32b_x16(out_at + col, v);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(__uint_as_float(v[i])));
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * shrink);
+                            tmem_st_32x32b_x16(out_at + col, v);
                         }
-                        // Not to where the output would overflow: then this tile's weights carry the difference, which leaves them without weight.
-                        const int x = e - unit;   // -232 .. 232: as two factors
-                        if (x <= 0 || (x <= 120 && big * shrink < power2(60 - max(x, 0) / 2) * power2(-((max(x, 0) + 1) / 2)))) {
-                            f *= power2(x / 2) * power2(x - x / 2);
-                            unit = e;
-                        }
+                        tmem_st_wait();
                     }
-#pragma unroll 1
-                    for (uint32_t col = 0; col < columns; col += 16) {
-                        uint32_t v[16];
-                        tmem_ld_32x32b_x16(out_at + col, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st_32x32b_x16(out_at + col, v);
-                    }
-                    tmem_st_wait();
+                    l *= shrink;
+                    m = m_new;
                 }
-                l *= shrink;
-                m = m_new;
             }
-            const float against = m == -INFINITY ? 0.f : m;
-            float back = 1.f;
-            if constexpr (F::kParts == 2) {
-                const int x = max(-120, unit - e);
-                more += (float)x;
-                back = power2(-x);
-            }
-            const uint64_t off = pair(more - against, more - against), cc = pair(c, c);
+            const float more = (F::kFp32 ? 0.f : kBoost) - (m == -INFINITY ? 0.f : m);
+            const uint64_t off = pair(more, more), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
-            // Weights of 32 keys: of 16-bit types 16 columns, of fp32, where their own scores lay, 16 and as many of their rests.
+            // Weights of 16 keys: 8 columns, of fp32 three times.
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
                 for (int part = 0; part < kWide / 16; ++part) {
-                    const uint32_t sixteen = FEW ? warp : 2 * g + part, to = at + (F::kParts == 2 ? sixteen / 2 * 32 + sixteen % 2 * 8 : sixteen * 8);
-                    uint32_t hi[8], lo[8];
+                    const uint32_t to = at + (FEW ? warp : 2 * g + part) * 8;
+                    uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float2 x = unpair(fma2(pair(__uint_as_float(sc[g][part * 16 + i]), __uint_as_float(sc[g][part * 16 + i + 1])), cc, off));
                         const float p = exp2_approx(x.x), q = exp2_approx(x.y);
                         sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
-                        if constexpr (F::kParts == 2) split2(p, q, hi[i / 2], lo[i / 2]);
+                        if constexpr (F::kFp32) split3(p, q, hi[i / 2], mid[i / 2], lo[i / 2]);
                         else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
                     }
                     tmem_st_32x32b_x8(to, hi);
-                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16, lo);
+                    if constexpr (F::kFp32) {
+                        tmem_st_32x32b_x8(to + 32, mid);
+                        tmem_st_32x32b_x8(to + 64, lo);
+                    }
                 }
             }
             if constexpr (FEW) {   // the other warps' keys have no weight here
                 const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
                 for (int i = 1; i < 4; ++i) {
-                    const uint32_t sixteen = (warp + i) & 3u, to = at + (F::kParts == 2 ? sixteen / 2 * 32 + sixteen % 2 * 8 : sixteen * 8);
-                    tmem_st_32x32b_x8(to, none);
-                    if constexpr (F::kParts == 2) tmem_st_32x32b_x8(to + 16, none);
+#pragma unroll
+                    for (int part = 0; part < F::kParts; ++part) tmem_st_32x32b_x8(at + ((warp + i) & 3u) * 8 + part * 32, none);
                 }
             }
             tmem_st_wait();
@@ -588,7 +553,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
             const float2 sums = unpair(add2(sum[0], sum[1]));
-            l = fmaf(sums.x + sums.y, back, l);
+            l += sums.x + sums.y;
             ++n;
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
@@ -622,63 +587,34 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_full_bar[job % kSlots]));
         };
-        // The largest of all loading threads' bits, by turns in three places: a warp is at most one tile ahead of another.
-        auto tile_top = [&](uint32_t top, uint32_t turn) -> uint32_t {
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) s_top[wg][turn][warp & 3u] = top;
-            sync_128(1 + wg);
-            return max(max(s_top[wg][turn][0], s_top[wg][turn][1]), max(s_top[wg][turn][2], s_top[wg][turn][3]));
-        };
-        int exp_k = 0, exp_v = 0;
         for (uint32_t job = wg; job < jobs; job += RT) {
             if (job + F::kAhead * RT < jobs) copy(job + F::kAhead * RT);
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(F::kAhead) : "memory");
-            if constexpr (F::kParts == 2) {   // in place, from what this thread has copied itself
+            if constexpr (F::kFp32) {   // in place, from what this thread has copied itself
                 unsigned char* at = smem + job % kSlots * F::kTile;
-                float buf[kPerThread][4];
-                float big = 0.f;   // (what is no number is passed over here, and is itself in both parts)
+                float4 buf[kPerThread];
+                uint64_t odd = 0;
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(at + i * 2048 + t * 16);
-                    buf[i][0] = x.x; buf[i][1] = x.y; buf[i][2] = x.z; buf[i][3] = x.w;
-                    big = max3(big, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
+                    buf[i] = *reinterpret_cast<const float4*>(at + i * 2048 + t * 16);
+                    odd = look(buf[i], odd);
                 }
-                uint32_t top = tile_top(__float_as_uint(big), job / RT & 1u);   // behind it everybody has read
-                // 0, or 2^-2 .. 2^15 under the power of two in use, or the tile gets one of its own.
-                int& e_now = job & 1u ? exp_v : exp_k;
-                const bool infinite = top >= 0x7F800000u;
-                if (infinite) {   // the largest that is a number
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int i = 0; i < kPerThread; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t bits = __float_as_uint(buf[i][e]) & 0x7FFFFFFFu;
-                            if (bits < 0x7F800000u) most = max(most, bits);
-                        }
-                    top = tile_top(most, 2);
-                }
-                const int reach = (int)(top >> 23) - 127 + e_now;
-                if (top != 0 && (reach >= 15 || reach < -2)) e_now = exponent_for(top);
-                const uint64_t up = pair(power2(e_now), power2(e_now));
+                sync_128(1 + wg);   // everybody has read
                 auto convert = [&](auto split) {
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i) {
-                        uint32_t hi[2], lo[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float2 x = unpair(mul2(pair(buf[i][2 * e], buf[i][2 * e + 1]), up));
-                            split(x.x, x.y, hi[e], lo[e]);
-                        }
+                        uint32_t hi[2], mid[2], lo[2];
+                        split(buf[i].x, buf[i].y, hi[0], mid[0], lo[0]);
+                        split(buf[i].z, buf[i].w, hi[1], mid[1], lo[1]);
                         unsigned char* to = at + place_of(i);
                         *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(to + F::kPanels * kPanel) = make_uint2(lo[0], lo[1]);
+                        *reinterpret_cast<uint2*>(to + F::kPart) = make_uint2(mid[0], mid[1]);
+                        *reinterpret_cast<uint2*>(to + 2 * F::kPart) = make_uint2(lo[0], lo[1]);
                     }
                 };
-                if (infinite) convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2_any(x, y, hi, lo); });
-                else convert([](float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, hi, lo); });
-                if (t == 0) (job & 1u ? s_exp_v : s_exp_k)[job / 2 % 8] = e_now;
+                if (is_odd(odd)) convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3_any(x, y, hi, mid, lo); });
+                else convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3(x, y, hi, mid, lo); });
             }
             publish(job);
         }
@@ -700,6 +636,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             return ok;
         };
         uint32_t n = 0;   // tiles that these rows see, so far
+        // The products of parts, the small ones first: of fp32 (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0)
+        constexpr int kTerms = F::kFp32 ? 6 : 1;
+        auto left = [](int term) -> uint32_t { return F::kFp32 ? 0x021010u >> (4 * (5 - term)) & 0xFu : 0u; };
+        auto right = [](int term) -> uint32_t { return F::kFp32 ? 0x201100u >> (4 * (5 - term)) & 0xFu : 0u; };
         if (role == 0) {
             const uint32_t k_steps = (dim + 15) / 16, idesc = idesc_f16<T>(kKeys);
             bool ok = wait_warp(smem_u32(&bar.q_full), 0, &s_abort);
@@ -708,22 +648,22 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     ok = hand_back(2 * j);
                     continue;
                 }
-                // S = Q K^T goes where the weights of the tile before the last lie: its product has to be done
-                if (n > 1) ok = wait_warp(smem_u32(&bar.done[n & 1u]), ((n >> 1) - 1) & 1u, &s_abort);
+                // S = Q K^T goes where the weights of the last tile, or of the one before, lie: its product has to be done
+                if (n >= F::kBufs) ok = wait_warp(smem_u32(&bar.done[(n - F::kBufs) & 1u]), ((n - F::kBufs) >> 1) & 1u, &s_abort);
                 ok = ok && wait_full(2 * j);
                 if (!ok) break;
                 tc_fence_after_sync();
-                if (elect_one()) {   // the small products first
-                    const uint32_t d = my_tmem + F::kScores + (n & 1u) * kKeys;
+                if (elect_one()) {
+                    const uint32_t d = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
                     const uint64_t keys = umma_desc_k_sw128(smem_at + 2 * j % kSlots * F::kTile);
                     auto issue = [&](uint32_t steps) {
 #pragma unroll
-                        for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+                        for (int term = 0; term < kTerms; ++term) {
 #pragma unroll
                             for (uint32_t s = 0; s < DP / 16; ++s) {
                                 if (s >= steps) break;
-                                const uint32_t at = (term == 0 ? F::kPanels * kPanel : 0) + s / 4 * kPanel + s % 4 * 32;
-                                umma_f16_ts(d, my_tmem + F::kQuery + (term == 1 ? DP / 2 : 0) + s * 8, keys + (at >> 4), idesc, term != (F::kParts == 2 ? 0 : 2) || s > 0);
+                                const uint32_t at = right(term) * F::kPart + s / 4 * kPanel + s % 4 * 32;
+                                umma_f16_ts(d, my_tmem + F::kQuery + left(term) * (DP / 2) + s * 8, keys + (at >> 4), idesc, term > 0 || s > 0);
                             }
                         }
                     };
@@ -749,18 +689,17 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
-                    const uint32_t p = my_tmem + F::kScores + (n & 1u) * kKeys;
+                    const uint32_t p = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
                     const uint64_t values = desc_rows(smem_at + (2 * j + 1) % kSlots * F::kTile);
-                    const uint32_t go_on = F::kSums ? n % kChunk != 0 : n > 0;
+                    const uint32_t go_on = !F::kFp32 && n > 0;
 #pragma unroll
                     for (int panel = 0; panel < F::kPanels; ++panel) {
 #pragma unroll
-                        for (int term = F::kParts == 2 ? 0 : 2; term < 3; ++term) {
+                        for (int term = 0; term < kTerms; ++term) {
 #pragma unroll
                             for (uint32_t s = 0; s < 4; ++s) {
-                                const uint32_t at = (term == 0 ? F::kPanels * kPanel : 0) + panel * kPanel + s * 2048;
-                                umma_f16_ts(my_tmem + F::kProduct + panel * 64, p + (term == 1 ? 16 : 0) + (F::kParts == 2 ? s / 2 * 32 + s % 2 * 8 : s * 8), values + (at >> 4),
-                                            idescs[panel], term != (F::kParts == 2 ? 0 : 2) || s > 0 ? 1u : go_on);
+                                const uint32_t at = right(term) * F::kPart + panel * kPanel + s * 2048;
+                                umma_f16_ts(my_tmem + F::kProduct + panel * 64, p + left(term) * 32 + s * 8, values + (at >> 4), idescs[panel], term > 0 || s > 0 ? 1u : go_on);
                             }
                         }
                     }

@@ -1,9 +1,11 @@
-"""GPU checks of attention where its inputs differ in size by far more than half the bits tell apart."""
+"""GPU checks of attention where its inputs differ in size by far more than half the bits tell apart: outliers in a column, keys that some rows of a tile do
+not see, values that change from tile to tile.  Bounds of each element by itself: attention_bound.py."""
 import math
 
 import pytest
 import torch
 
+import attention_bound as A
 import dense_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +58,80 @@ def test_a_tile_of_large_values_that_half_of_the_rows_do_not_see(ctx, Q):
     # fp32 all the way: 64 products and sums of a score and its exponential, 64 of the result
     O.close(got[:, :rows], want[:, :rows], torch.float32, floor=256 * 2.0 ** -24 * float(v[0, :64].abs().amax()))
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("D", [8, 64, 80, 128])
+@pytest.mark.parametrize("outlier", [1e4, 1e6, 1e9])
+def test_a_large_column_leaves_the_others_their_digits(ctx, Q, D, outlier):
+    q, k, v = _inputs(D + Q, Q, 260, D)
+    v[..., 3] *= outlier
+    k[..., 5] *= outlier
+    q[..., 5] = 0
+    A.check(_run(ctx, q, k, v), *A.attention(q, k, v))
+    q, k, v = _inputs(D + Q, Q, 260, D)
+    q[..., 5] *= outlier
+    k[..., 5] /= outlier
+    A.check(_run(ctx, q, k, v), *A.attention(q, k, v))
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("large", [1e4, 1e9, 1e30])
+def test_a_large_key_that_other_rows_see(ctx, Q, D, large):
+    """Rows in front of it do not see it, and have what they would have without it; the ones behind do."""
+    K = Q + 70
+    q, k, v = _inputs(D, Q, K, D)
+    at = 70 + Q // 2
+    v[0, at] *= large
+    k[0, at] *= large
+    window = (64, 0)
+    got, (want, bound) = _run(ctx, q, k, v, first=[70], window=window), A.attention(q, k, v, window=window, first=[70])
+    before = Q // 2
+    A.check(got[:, :before], want[:, :before], bound[:, :before])
+    k[0, at] /= large
+    got, (want, bound) = _run(ctx, q, k, v, first=[70], window=window), A.attention(q, k, v, window=window, first=[70])
+    A.check(got, want, bound)
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("D", [8, 40, 64, 80, 112])
+@pytest.mark.parametrize("drop", [10, 20, 30, 40])
+def test_values_that_fall_while_scores_rise(ctx, Q, D, drop):
+    """Large values of small weight in one tile, small values of large weight in the next; tensor memory holds large numbers from before."""
+    q, k, v = _inputs(D + drop, Q, 256, D)
+    q[..., 0] = 4.0
+    for tile in range(4):
+        k[0, 64 * tile:64 * tile + 64, 0, 0] = 20.0 * (tile - 2) * math.sqrt(D) / 4
+        v[0, 64 * tile:64 * tile + 64] *= 2.0 ** (-drop * (tile % 2))
+    want, bound = A.attention(q, k, v)
+    first = None
+    for _ in range(3):
+        _fill_tensor_memory(ctx)
+        got = _run(ctx, q, k, v)
+        A.check(got, want, bound)
+        assert first is None or torch.equal(got, first)
+        first = got
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("small,large", [(1e-27, 1e30), (1e-25, 1e37), (1e30, 1e-27), (1e37, 1e-25)])
+def test_values_of_two_ends_of_the_range(ctx, Q, small, large):
+    """One tile of values, then one of another size that half of the rows do not see."""
+    q, k, v = _inputs(7, Q, 128, 64)
+    v[0, :64] *= small
+    v[0, 64:] *= large
+    first = [63 - Q // 2]
+    A.check(_run(ctx, q, k, v, first=first, window=(63, 0)), *A.attention(q, k, v, window=(63, 0), first=first))
+
+
+@pytest.mark.parametrize("Q,K,H,G,D", [(1, 300, 2, 2, 64), (4, 200, 2, 1, 128), (17, 500, 3, 3, 80), (64, 64, 2, 2, 64), (128, 128, 3, 3, 64), (197, 197, 2, 2, 64), (300, 300, 1, 1, 64),
+                                       (100, 400, 4, 2, 128), (200, 200, 1, 1, 32), (130, 1000, 1, 1, 64), (9, 4000, 2, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((50, 50), 3)])
+def test_the_error_of_random_numbers(ctx, Q, K, H, G, D, window, sinks):
+    gen = torch.Generator().manual_seed(Q + K)
+    q, k, v = torch.randn(2, Q, H, D, generator=gen), torch.randn(2, K, G, D, generator=gen), torch.randn(2, K, G, D, generator=gen)
+    first = [K - Q, (K - Q) // 2]
+    assert A.rms(_run(ctx, q, k, v, first=first, window=window, sinks=sinks), O.attention(q, k, v, None, window, sinks, None, first)) <= A.RMS
+    v = v.abs()   # of one sign: what is lost towards zero adds up
+    assert A.rms(_run(ctx, q, k, v, first=first, window=window, sinks=sinks), O.attention(q, k, v, None, window, sinks, None, first)) <= A.RMS
