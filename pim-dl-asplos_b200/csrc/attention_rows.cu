@@ -8,7 +8,8 @@
 // each exchange a lane holds half as many rows, in the end the score of one.  The keys of one head and sequence are split
 // over the CTAs of a cluster where there would be too few CTAs; they join through distributed shared memory: no scratch
 // memory, no second launch, one order of summation.
-// Scores, maxima, sums and outputs are fp32; weights are not rounded.
+// Scores, maxima, sums and outputs are fp32; weights are not rounded, but all brought down by a power of two no less than the number of keys, so that sums
+// of values do not overflow where their mean does not.
 #include "attention.cuh"
 #include "ptx.cuh"
 
@@ -73,6 +74,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs 
     const int64_t p0 = first + (int64_t)(r0 / per_head), p1 = first + (int64_t)((r0 + n_rows - 1) / per_head);
     const KeySpan span = key_span(a, p0, p1, length);
     const uint32_t n_keys = (uint32_t)(span.sinks + (span.hi - span.lo));
+    const float down = __int_as_float((n_keys <= 1 ? 127 : 95 + __clz(n_keys - 1)) << 23);   // 2^-k, 2^k no less than n_keys
     const uint32_t t0 = (uint32_t)((uint64_t)n_keys * share / shares), t1 = (uint32_t)((uint64_t)n_keys * (share + 1) / shares);
 
     float q[RB][E];
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(AttentionArgs 
         l *= shrink;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            s[u] = exp2_approx(s[u] - against);
+            s[u] = exp2_approx(s[u] - against) * down;
             l += s[u];
         }
 #pragma unroll

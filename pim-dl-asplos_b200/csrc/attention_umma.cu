@@ -11,8 +11,9 @@
 // Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.  fp32 operands are split into
 // three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
 // its size.  Of the nine products the six down to 2^-16 of the whole are summed, the small ones first; b c + c b, 2^-25 of it, is left out.  So an element's
-// digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  In 16 bits weights
-// carry 2^6 and up to 2^8 more, the sum l with them.  Maxima, sums and outputs are fp32; maxima are taken up to whole numbers, so that what is against an older
+// digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  f16's weights
+// carry 2^6 and up to 2^8 more, the sum l with them; in bf16 and fp32 they, or the values, are brought down by the number of keys instead, exactly, so that a
+// row's sums stay below its largest value: results up to the type's largest number do not overflow on the way.  Maxima, sums and outputs are fp32; maxima are taken up to whole numbers, so that what is against an older
 // one is brought in line without rounding; the sum over tiles that fp32 makes outside of tensor memory rounds once each.
 //
 // Loading warps copy 16 bytes a piece (cp.async): no tensor maps to be made by the host, and rows behind the last key become zeros.  fp32 is
@@ -36,7 +37,7 @@ constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two byt
 constexpr uint32_t kMostShares = 8;
 // Tensor memory adds up towards zero: fp32's product of a tile takes four units of 2^-24 off the sum at most, its small terms being first, and would take
 // twenty-four off with the tiles before in there.  So each tile's is taken out and summed with rounding.  Half the bits do not show it.
-constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what weights are multiplied by, and of how far they may grow over 1: 2^14 in all
+constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what f16's weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 // DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
 template <typename T, int DP, int RT>
@@ -85,6 +86,7 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t smem_addr) {
     return umma_desc_k_sw128(smem_addr) | (static_cast<uint64_t>(1024u >> 4) << 16);
 }
 
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }   // |e| < 127
 __device__ __forceinline__ void sync_128(uint32_t id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
 // A warp's bounded wait, with one answer.  The hint lets the hardware hold a waiting warp for up to two microseconds a look: without it the fifteen warps
 // of a CTA that wait for one another took a third of all instructions.
@@ -219,6 +221,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     if (span.lo <= (span.sinks + kKeys - 1) / kKeys * kKeys) span.lo = span.sinks = 0;
     const uint32_t sink_tiles = (uint32_t)(span.sinks + kKeys - 1) / kKeys;
     const uint32_t all_tiles = sink_tiles + (uint32_t)(span.hi - span.lo + kKeys - 1) / kKeys;
+    const int log_keys = all_tiles <= 1 ? 6 : 38 - __clz(all_tiles - 1);   // 2^log_keys: no fewer than the keys of all tiles
     const uint32_t t0 = (uint32_t)((uint64_t)all_tiles * share / shares), t1 = (uint32_t)((uint64_t)all_tiles * (share + 1) / shares), tiles = t1 - t0;
     auto tile_keys = [&](uint32_t t, int32_t& k0, int32_t& end) {
         const bool sink = t < sink_tiles;
@@ -515,7 +518,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     m = m_new;
                 }
             }
-            const float more = (F::kFp32 ? 0.f : kBoost) - (m == -INFINITY ? 0.f : m);
+            const float boost = F::kFp32 ? 0.f : std::is_same<T, __half>::value ? kBoost : -kSlack - (float)log_keys;   // (fp32: in the values)
+            const float more = boost - (m == -INFINITY ? 0.f : m);
             const uint64_t off = pair(more, more), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
             // Weights of 16 keys: 8 columns, of fp32 three times.
@@ -553,7 +557,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
             const float2 sums = unpair(add2(sum[0], sum[1]));
-            l += sums.x + sums.y;
+            l = F::kFp32 ? fmaf(sums.x + sums.y, power2(-log_keys), l) : l + (sums.x + sums.y);
             ++n;
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
@@ -595,10 +599,14 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 unsigned char* at = smem + job % kSlots * F::kTile;
                 float4 buf[kPerThread];
                 uint64_t odd = 0;
+                const float down = power2(job & 1u ? -log_keys : 0);
+                const uint64_t down2 = pair(down, down);
 #pragma unroll
                 for (int i = 0; i < kPerThread; ++i) {
-                    buf[i] = *reinterpret_cast<const float4*>(at + i * 2048 + t * 16);
-                    odd = look(buf[i], odd);
+                    const float4 x = *reinterpret_cast<const float4*>(at + i * 2048 + t * 16);
+                    odd = look(x, odd);
+                    const float2 front = unpair(mul2(pair(x.x, x.y), down2)), back = unpair(mul2(pair(x.z, x.w), down2));
+                    buf[i] = make_float4(front.x, front.y, back.x, back.y);
                 }
                 sync_128(1 + wg);   // everybody has read
                 auto convert = [&](auto split) {

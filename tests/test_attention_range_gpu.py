@@ -1,5 +1,6 @@
 """GPU checks of attention where its inputs differ in size by far more than half the bits tell apart: outliers in a column, keys that some rows of a tile do
-not see, values that change from tile to tile.  Bounds of each element by itself: attention_bound.py."""
+not see, values that change from tile to tile, results
+near the type's largest number.  Bounds of each element by itself: attention_bound.py."""
 import math
 
 import pytest
@@ -9,6 +10,7 @@ import attention_bound as A
 import dense_oracle as O
 
 pytestmark = pytest.mark.gpu
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 ROWS = [1, 3, 6, 20, 100, 200]   # one, few and many rows: every kernel and form
 
 
@@ -135,3 +137,18 @@ def test_the_error_of_random_numbers(ctx, Q, K, H, G, D, window, sinks):
     assert A.rms(_run(ctx, q, k, v, first=first, window=window, sinks=sinks), O.attention(q, k, v, None, window, sinks, None, first)) <= A.RMS
     v = v.abs()   # of one sign: what is lost towards zero adds up
     assert A.rms(_run(ctx, q, k, v, first=first, window=window, sinks=sinks), O.attention(q, k, v, None, window, sinks, None, first)) <= A.RMS
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D,K", [(64, 130), (128, 700)])
+def test_values_near_the_types_largest(ctx, Q, dtype, D, K):
+    t = TYPES[dtype]
+    q, k, v = _inputs(3, Q, K, D)
+    q, k, v = (q / 4).to(t), k.to(t), (1e36 * (1 + v.abs() / 4)).to(t)
+    got, (want, bound) = _run(ctx, q, k, v), A.attention(q, k, v)
+    # (16-bit weights are rounded once)
+    A.check(got, want, bound + (0 if t == torch.float32 else torch.finfo(t).eps / 2 * want.abs()), dtype=t)
+    biggest = torch.full_like(v, 3.3e38)
+    got = _run(ctx, q, k, biggest)
+    A.check(got, biggest[:, :1].double().expand(got.shape), (24 + K / 4) * A.U * biggest[:, :1].double() * (1 if t == torch.float32 else 2.0 ** 16), dtype=t)
