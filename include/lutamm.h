@@ -305,8 +305,8 @@ int lutamm_rotary(lutamm_ctx* ctx, const lutamm_rotary_params* p, uint32_t flags
  * j < sinks); left or right negative: no bound on that side.  So a padded batch of whole sequences has lengths alone, new
  * tokens behind a cache have first = lengths - queries and right = 0, a sliding window has left, and sinks are the
  * first keys, which stay visible.  A query that sees no key gives zeros.  Keys from lengths[b] on are not read; lengths are taken between 0
- * and keys.  Head h reads key head h / (heads / kv_heads).  A key that a query does not see has no part in its result, whatever it holds,
- * with one exception: a value that is not finite spreads to the queries whose tile of up to 256 query rows has another one that sees it.
+ * and keys.  Head h reads key head h / (heads / kv_heads).  A key that a query does not see has no part in its result, whatever it holds; an
+ * infinity or NaN in the value of one that it sees shows in that column.
  * q and out are [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim]; out shares no memory with the
  * others.  For serving: there is no backward pass. */
 typedef struct lutamm_attention_params {

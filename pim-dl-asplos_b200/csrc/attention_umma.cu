@@ -20,6 +20,10 @@
 // converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
 // CTAs, the key tiles of one item are split over a cluster, whose CTAs join through distributed shared memory: no scratch memory and one order of summation.
 //
+// Infinities and NaN: a product over 64 keys would have each meet weights of zero, those of rows and warps that do not see its key, and parts of zero.  So values
+// that are not finite go into the product as zeros, and are added to the results of the rows that see them at the end; of keys and queries that are not finite fp32
+// forms the scores one by one.  A CTA that meets none pays for the look at what it loads.
+//
 // What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 96 us, 349 TFLOP/s; of 2850 warp instructions a
 // tile 680 form its weights.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 32 us, 540 TFLOP/s.  fp32,
 // three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 92 us, of which a CTA spends half before its first and behind its last tile.
@@ -148,13 +152,6 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t& hi, uint32_t&
     const float2 last = unpair(fma2(pair(m.x, m.y), minus, pair(rest.x, rest.y)));
     lo = pack2(last.x, last.y, static_cast<__nv_bfloat16*>(nullptr));
 }
-// ... of numbers that may be infinite: their rests are none
-__device__ __forceinline__ void split3_any(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-    split3(a, b, hi, mid, lo);
-    const uint32_t keep = (fabsf(a) == INFINITY ? 0u : 0xFFFFu) | (fabsf(b) == INFINITY ? 0u : 0xFFFF0000u);
-    mid &= keep;
-    lo &= keep;
-}
 // 0, or NaN where one of the numbers is none or infinite: what is added to `odd`
 __device__ __forceinline__ uint64_t look(const float4& x, uint64_t odd) {
     return fma2(pair(x.x, x.y), pair(0.f, 0.f), fma2(pair(x.z, x.w), pair(0.f, 0.f), odd));
@@ -162,6 +159,19 @@ __device__ __forceinline__ uint64_t look(const float4& x, uint64_t odd) {
 __device__ __forceinline__ bool is_odd(uint64_t odd) {
     const float2 v = unpair(odd);
     return v.x + v.y != 0.f;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// The same of two 16-bit numbers
+__device__ __forceinline__ __half2 look(uint32_t w, __half2 odd) { return __hfma2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0)), odd); }
+__device__ __forceinline__ __nv_bfloat162 look(uint32_t w, __nv_bfloat162 odd) {
+    return __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), __bfloat162bfloat162(__ushort_as_bfloat16(0)), odd);
+}
+// Zero in place of those that are none or infinite: whose exponents, all ones, carry into bit 15 of their half
+template <typename T>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {
+    constexpr bool half = std::is_same<T, __half>::value;
+    const uint32_t odd = ((w & (half ? 0x7C007C00u : 0x7F807F80u)) + (half ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+    return w & ~((odd >> 15) * 0xFFFFu);
 }
 
 // ones below bit n
@@ -197,9 +207,9 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     static_assert(!FEW || RT == 1);
     constexpr uint32_t kSlots = F::kSlots, kThreads = F::kThreads;
     extern __shared__ unsigned char s_raw[];
-    __shared__ __align__(8) uint64_t s_full_bar[kSlots], s_empty_bar[kSlots];
+    __shared__ __align__(8) uint64_t s_full_bar[kSlots], s_empty_bar[kSlots], s_looked_bar[F::kFp32 ? 1 : kSlots];   // (the last: of 16-bit values)
     __shared__ __align__(8) RowBars s_row[RT];
-    __shared__ uint32_t s_tmem, s_abort;
+    __shared__ uint32_t s_tmem, s_abort, s_odd_from[2], s_odd_to[2];   // keys, values that are not finite: in tiles from .. to - 1, so far
     __shared__ float s_m[RT * kRows], s_l[RT * kRows], s_join[FEW ? 2 : 1][32];
     unsigned char* smem = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const uint32_t smem_at = smem_u32(smem);
@@ -308,6 +318,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
     } else if (warp == F::kIssueAt + 1) {
         if (lane < kSlots) mbar_init(smem_u32(&s_full_bar[lane]), 4);
         if (lane < kSlots) mbar_init(smem_u32(&s_empty_bar[lane]), RT);
+        if (!F::kFp32 && lane < kSlots) mbar_init(smem_u32(&s_looked_bar[F::kFp32 ? 0 : lane]), 2);
         if (lane < RT) {
             RowBars& bar = s_row[lane];
             for (int i = 0; i < 2; ++i) {
@@ -318,6 +329,10 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             mbar_init(smem_u32(&bar.q_full), 4);
         }
         fence_barrier_init();
+        if (lane < 2) {
+            s_odd_from[lane] = ~0u;
+            s_odd_to[lane] = 0;
+        }
         if (lane == 0) s_abort = 0;
     }
     tc_fence_before_sync();
@@ -351,36 +366,34 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
         float factor = fabsf(a.scale);   // of this row's scores
+        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+        bool odd_queries = false;
+        if (a.scale == 0.f) factor = 1.f;
         {
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
             auto raw = [&](int i) -> uint4 { return *reinterpret_cast<const uint4*>(smem + q_stage + (lane * kPerQ + (i ^ (lane & (kPerQ - 1)))) * 16); };
             auto raw4 = [&](int i) -> float4 { const uint4 u = raw(i); return *reinterpret_cast<const float4*>(&u); };
-            const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
-            if (a.scale == 0.f) factor = 1.f;
             if constexpr (F::kFp32) {
                 uint64_t odd = 0;
 #pragma unroll
                 for (int i = 0; i < kPerQ; ++i) odd = look(raw4(i), odd);
                 const uint64_t sign2 = pair(sign, sign);
-                auto convert = [&](auto split) {   // 16 elements: 8 columns of each part
+                odd_queries = __any_sync(0xffffffffu, is_odd(odd));
 #pragma unroll 1
-                    for (int part = 0; part < kPerQ / 4; ++part) {
-                        uint32_t hi[8], mid[8], lo[8];
+                for (int part = 0; part < kPerQ / 4; ++part) {   // 16 elements: 8 columns of each part
+                    uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float4 x = raw4(part * 4 + i);
-                            const float2 front = unpair(mul2(pair(x.x, x.y), sign2)), back = unpair(mul2(pair(x.z, x.w), sign2));
-                            split(front.x, front.y, hi[2 * i], mid[2 * i], lo[2 * i]);
-                            split(back.x, back.y, hi[2 * i + 1], mid[2 * i + 1], lo[2 * i + 1]);
-                        }
-                        tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
-                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, mid);
-                        tmem_st_32x32b_x8(my_tmem + F::kQuery + DP + part * 8, lo);
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 x = raw4(part * 4 + i);
+                        const float2 front = unpair(mul2(pair(x.x, x.y), sign2)), back = unpair(mul2(pair(x.z, x.w), sign2));
+                        split3(front.x, front.y, hi[2 * i], mid[2 * i], lo[2 * i]);
+                        split3(back.x, back.y, hi[2 * i + 1], mid[2 * i + 1], lo[2 * i + 1]);
                     }
-                };
-                if (__any_sync(0xffffffffu, is_odd(odd))) convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3_any(x, y, hi, mid, lo); });
-                else convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3(x, y, hi, mid, lo); });
+                    tmem_st_32x32b_x8(my_tmem + F::kQuery + part * 8, hi);
+                    tmem_st_32x32b_x8(my_tmem + F::kQuery + DP / 2 + part * 8, mid);
+                    tmem_st_32x32b_x8(my_tmem + F::kQuery + DP + part * 8, lo);
+                }
             } else {
 #pragma unroll
                 for (int part = 0; part < kPerQ / 4; ++part) {   // 32 elements: 16 columns
@@ -437,6 +450,69 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             m_o = m;
             o_any = true;
         };
+        // Which of a tile's keys, from k0 on, this row sees
+        auto seen_of = [&](int32_t k0, int32_t end) -> uint64_t {
+            return below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+        };
+        const T* const k_head = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
+        // A tile's scores, one by one, to `at`: where keys or queries are not finite
+        auto scores_one_by_one = [&](uint32_t tile, uint32_t at) {
+            const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)qi * a.q_token + (int64_t)(g * per_head.d + (row - qi * per_head.d)) * a.q_head;
+            int32_t k0, end;
+            tile_keys(tile, k0, end);
+#pragma unroll 1
+            for (uint32_t i = FEW ? warp * 16 : 0; i < (FEW ? warp * 16 + 16 : 64); ++i) {
+                const int32_t key = k0 + (int32_t)i;
+                float d = 0.f;
+                if (key < end && (key < gap_from || key >= gap_to)) {
+                    const T* k = k_head + (int64_t)key * a.k_token;
+#pragma unroll 2
+                    for (uint32_t c = 0; c < dim; c += kPer16<T>) {
+                        float x[kPer16<T>], y[kPer16<T>];
+                        load_elems<T, kPer16<T>>(q + c, x);
+                        load_elems<T, kPer16<T>>(k + c, y);
+#pragma unroll
+                        for (int e = 0; e < kPer16<T>; ++e) d = fmaf(x[e], y[e], d);
+                    }
+                }
+                __syncwarp();
+                tmem_st_32x32b_x1(at + i, __float_as_uint(d * sign));
+            }
+            tmem_st_wait();
+        };
+        // What this row sees of values that are not finite, to its results
+        auto add_odd_values = [&] {
+            constexpr int kE = kPer16<T>, kBatch = 4;
+            const T* const v_head = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head;
+            const uint32_t to = min(tiles, *static_cast<volatile uint32_t*>(&s_odd_to[1]));
+#pragma unroll 1
+            for (uint32_t j = *static_cast<volatile uint32_t*>(&s_odd_from[1]); j < to; ++j) {
+                if (RT == 2 && !sees(t0 + j)) continue;
+                int32_t k0, end;
+                tile_keys(t0 + j, k0, end);
+                uint64_t seen = seen_of(k0, end);
+                if (FEW) seen &= 0xFFFFull << (16 * warp);
+#pragma unroll 1
+                for (uint32_t i = 0; i < 64; ++i) {
+                    const bool me = seen >> i & 1u;
+                    if (!__any_sync(0xffffffffu, me)) continue;
+                    const T* v = v_head + (int64_t)(k0 + (int32_t)i) * a.v_token;
+#pragma unroll 1
+                    for (uint32_t c0 = 0; c0 < dim; c0 += kBatch * kE) {
+                        float x[kBatch][kE];
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u) load_elems<T, kE>(v + (c0 + u * kE < dim ? c0 + u * kE : 0), x[u]);
+#pragma unroll
+                        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+                            for (int e = 0; e < kE; ++e) {
+                                const uint32_t c = c0 + u * kE + e;
+                                if (me && c < dim && !finite(x[u][e])) reinterpret_cast<float*>(&s_o[out_place(r, c / 4)])[c % 4] += x[u][e];
+                            }
+                    }
+                }
+            }
+        };
         uint32_t n = 0;   // tiles so far
         for (uint32_t j = 0; j < tiles; ++j) {
             if (RT == 2 && !sees(t0 + j)) continue;
@@ -456,6 +532,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             }
             const uint32_t at = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
             const float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
+            if constexpr (F::kFp32) {
+                if (__builtin_expect(__any_sync(0xffffffffu, odd_queries || j < *static_cast<volatile uint32_t*>(&s_odd_to[0])), 0)) {
+                    if (odd_queries || __any_sync(0xffffffffu, j >= *static_cast<volatile uint32_t*>(&s_odd_from[0]))) scores_one_by_one(t0 + j, at);
+                }
+            }
             constexpr int kGroups = FEW ? 1 : 2, kWide = FEW ? 16 : 32;
             uint32_t sc[kGroups][kWide];
             if constexpr (FEW) {
@@ -468,7 +549,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             if (t0 + j < full_from || t0 + j >= full_to) {
                 int32_t k0, end;
                 tile_keys(t0 + j, k0, end);
-                const uint64_t seen = below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
+                const uint64_t seen = seen_of(k0, end);
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
                     const uint32_t bits = (uint32_t)(seen >> (FEW ? 16 * warp : 32 * g));
@@ -564,6 +645,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         tc_fence_after_sync();
         const float norm = FEW || shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         add_chunk(done, norm);
+        if (__builtin_expect(__any_sync(0xffffffffu, done && *static_cast<volatile uint32_t*>(&s_odd_to[1])), 0) && first_row < n_rows) add_odd_values();
         if (FEW || shares > 1) {
             s_m[r] = m;
             s_l[r] = l;
@@ -609,20 +691,25 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     buf[i] = make_float4(front.x, front.y, back.x, back.y);
                 }
                 sync_128(1 + wg);   // everybody has read
-                auto convert = [&](auto split) {
+                if (is_odd(odd)) {
+                    atomicMin(&s_odd_from[job & 1u], job / 2);
+                    atomicMax(&s_odd_to[job & 1u], job / 2 + 1);
 #pragma unroll
                     for (int i = 0; i < kPerThread; ++i) {
-                        uint32_t hi[2], mid[2], lo[2];
-                        split(buf[i].x, buf[i].y, hi[0], mid[0], lo[0]);
-                        split(buf[i].z, buf[i].w, hi[1], mid[1], lo[1]);
-                        unsigned char* to = at + place_of(i);
-                        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(to + F::kPart) = make_uint2(mid[0], mid[1]);
-                        *reinterpret_cast<uint2*>(to + 2 * F::kPart) = make_uint2(lo[0], lo[1]);
+                        buf[i].x = finite(buf[i].x) ? buf[i].x : 0.f; buf[i].y = finite(buf[i].y) ? buf[i].y : 0.f;
+                        buf[i].z = finite(buf[i].z) ? buf[i].z : 0.f; buf[i].w = finite(buf[i].w) ? buf[i].w : 0.f;
                     }
-                };
-                if (is_odd(odd)) convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3_any(x, y, hi, mid, lo); });
-                else convert([](float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) { split3(x, y, hi, mid, lo); });
+                }
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+                    uint32_t hi[2], mid[2], lo[2];
+                    split3(buf[i].x, buf[i].y, hi[0], mid[0], lo[0]);
+                    split3(buf[i].z, buf[i].w, hi[1], mid[1], lo[1]);
+                    unsigned char* to = at + place_of(i);
+                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(to + F::kPart) = make_uint2(mid[0], mid[1]);
+                    *reinterpret_cast<uint2*>(to + 2 * F::kPart) = make_uint2(lo[0], lo[1]);
+                }
             }
             publish(job);
         }
@@ -693,7 +780,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     ok = hand_back(2 * j + 1);
                     continue;
                 }
-                ok = wait_full(2 * j + 1) && wait_warp(smem_u32(&bar.p_full[n & 1u]), (n >> 1) & 1u, &s_abort);
+                ok = F::kFp32 ? wait_full(2 * j + 1) : wait_warp(smem_u32(&s_looked_bar[(2 * j + 1) % kSlots]), ((2 * j + 1) / kSlots) & 1u, &s_abort);
+                ok = ok && wait_warp(smem_u32(&bar.p_full[n & 1u]), (n >> 1) & 1u, &s_abort);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elect_one()) {
@@ -716,6 +804,34 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 }
                 __syncwarp();
                 ++n;
+            }
+        } else if constexpr (!F::kFp32) {
+            // The two warps that are left look at the values, while weights are formed: were it the loading warps, single tokens behind eight caches would take 62 us for 48.
+            static_assert(RT == 1);
+            for (uint32_t job = 1; job < jobs; job += 2) {
+                if (!wait_full(job)) break;
+                uint4* at = reinterpret_cast<uint4*>(smem + job % kSlots * F::kTile) + (role - 2) * 32 + lane;
+                using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+                const uint32_t zero = 0;
+                T2 odd[2] = {*reinterpret_cast<const T2*>(&zero), *reinterpret_cast<const T2*>(&zero)};
+#pragma unroll
+                for (int i = 0; i < F::kTile / 1024; ++i) {
+                    const uint4 w = at[i * 64];
+                    odd[0] = look(w.x, odd[0]); odd[1] = look(w.y, odd[1]); odd[0] = look(w.z, odd[0]); odd[1] = look(w.w, odd[1]);
+                }
+                const T2 all = __hadd2(odd[0], odd[1]);
+                if (__builtin_expect(!(__low2float(all) == 0.f && __high2float(all) == 0.f), 0)) {
+                    atomicMin(&s_odd_from[1], job / 2);
+                    atomicMax(&s_odd_to[1], job / 2 + 1);
+#pragma unroll 1
+                    for (int i = 0; i < F::kTile / 1024; ++i) {
+                        const uint4 w = at[i * 64];
+                        at[i * 64] = make_uint4(only_finite<T>(w.x), only_finite<T>(w.y), only_finite<T>(w.z), only_finite<T>(w.w));
+                    }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_looked_bar[job % kSlots]));
             }
         }
     }

@@ -1,6 +1,6 @@
 """GPU checks of attention where its inputs differ in size by far more than half the bits tell apart: outliers in a column, keys that some rows of a tile do
 not see, values that change from tile to tile, results
-near the type's largest number.  Bounds of each element by itself: attention_bound.py."""
+near the type's largest number, infinities.  Bounds of each element by itself: attention_bound.py."""
 import math
 
 import pytest
@@ -152,3 +152,77 @@ def test_values_near_the_types_largest(ctx, Q, dtype, D, K):
     biggest = torch.full_like(v, 3.3e38)
     got = _run(ctx, q, k, biggest)
     A.check(got, biggest[:, :1].double().expand(got.shape), (24 + K / 4) * A.U * biggest[:, :1].double() * (1 if t == torch.float32 else 2.0 ** 16), dtype=t)
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 80])
+def test_values_that_are_not_finite(ctx, Q, dtype, D):
+    """An infinity or NaN in a value shows in the rows that see its key, in its column, and nowhere else."""
+    t, K = TYPES[dtype], Q + 130
+    q, k, v = (x.to(t) for x in _inputs(Q + D, Q, K, D))
+    q = q / 2
+    window, first = (100, 0), [K - Q]
+    clean = v.clone()
+    inf = float("inf")
+    spots = [(K - 1, 0, inf), (K - 1 - Q // 2, 1, inf), (K - 1 - Q // 2, 2, -inf), (K - 2, D - 1, float("nan")), (K - Q // 2 - 3, 3, inf), (K - Q // 2 - 5, 3, -inf), (K - Q - 90, 4, -inf),
+             (0, 5, inf)]
+    for key, col, value in spots:
+        v[0, key, 0, col] = value
+    got = _run(ctx, q, k, v, first=first, window=window)
+    seen = O.visible(Q, K, K, first[0], window, 0).double()
+    finite = v[0, :, 0].isfinite()
+    expected = O.attention(q, k, torch.where(v.isfinite(), v, torch.zeros((), dtype=t)), None, window, 0, None, first)
+    plus, minus, nan = (seen @ m.double() > 0 for m in (v[0, :, 0] == inf, v[0, :, 0] == -inf, v[0, :, 0].isnan()))
+    assert plus.any() and (seen @ (~finite).double() > 0).any() and not finite.all()
+    for i in range(Q):
+        for c in range(D):
+            x = float(got[0, i, 0, c])
+            if nan[i, c] or (plus[i, c] and minus[i, c]):
+                assert math.isnan(x), (i, c, x)
+            elif plus[i, c]:
+                assert x == inf, (i, c, x)
+            elif minus[i, c]:
+                assert x == -inf, (i, c, x)
+    plain = ~(plus | minus | nan)[None, :, None]
+    floor = 0.0 if t == torch.float32 else 2 * torch.finfo(t).eps * float(clean.double().abs().amax())
+    O.close(torch.where(plain, got, torch.zeros((), dtype=t)), torch.where(plain, expected, 0.0), t, floor=floor + 2 ** -18)
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_whole_tile_of_infinities(ctx, Q, dtype):
+    t = TYPES[dtype]
+    q, k, v = (x.to(t) for x in _inputs(Q, Q, 200, 64))
+    v[0, 64:128] = float("inf")
+    assert (_run(ctx, q / 4, k, v) == float("inf")).all()
+    v[0, 70] = float("nan")
+    assert _run(ctx, q / 4, k, v).isnan().all()
+
+
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_keys_and_queries_that_are_not_finite(ctx, Q, dtype):
+    """A score of minus infinity is a key without weight; one of plus infinity, or NaN, is NaN in its row; others have what they had."""
+    t, K = TYPES[dtype], Q + 130
+    q, k, v = (x.to(t) for x in _inputs(Q + 1, Q, K, 64))
+    inf = float("inf")
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q[..., 1] = -q[..., 1].abs() - 0.5
+    if Q > 2:
+        q[0, Q // 3, 0, 0] = inf       # a row of its own: scores of plus or minus infinity
+        q[0, Q // 2, 0, 7] = float("nan")
+    k[0, K - Q - 70, 0, 0] = -inf
+    k[0, K - 1, 0, 1] = inf            # the last row alone sees it
+    k[0, K - 1 - Q // 4, 0, 0] = inf
+    for window in ((-1, 0), (90, 0)):
+        got = _run(ctx, q, k, v, first=[K - Q], window=window)
+        seen = O.visible(Q, K, K, K - Q, window, 0)
+        for i in range(Q):
+            at = seen[i].nonzero()[:, 0]
+            s = (k[0, at, 0].double() @ q[0, i, 0].double()) / 8
+            w = torch.softmax(s, 0)
+            want = torch.full((64,), float("nan")) if w.isnan().any() else w @ v[0, at, 0].double()
+            assert torch.equal(got[0, i, 0].isnan(), want.isnan()), (window, i)
+            if not want.isnan().any():
+                O.close(got[0, i, 0], want, t, floor=2 ** -18 + (0.0 if t == torch.float32 else 2 * torch.finfo(t).eps * float(v.double().abs().amax())))
