@@ -44,7 +44,10 @@ def parse_args():
                    help="run attention and the norms in this library's own kernels instead of PyTorch's")
     p.add_argument('--window', type=int, default=-1, help='with --dense_kernels: keys seen on either side of a query (negative: all)')
     p.add_argument('--sinks', type=int, default=0, help='with --dense_kernels and --window: first tokens that stay visible')
-    return p.parse_args()
+    args = p.parse_args()
+    if not args.dense_kernels and (args.window >= 0 or args.sinks):
+        p.error("--window and --sinks need --dense_kernels: PyTorch's attention here sees all keys")
+    return args
 
 
 def run(args, whole_model: bool):
