@@ -314,7 +314,7 @@ typedef struct lutamm_attention_params {
                                                                          * 2^31 - 256, queries * heads below 2^31 */
     uint32_t sinks;
     int32_t  left, right;
-    float    scale;
+    float    scale;           /* finite, also times log2 e */
     lutamm_heads q, k, v, out;
     const int32_t* lengths;   /* [batch], device */
     const int32_t* first;     /* [batch], device */

@@ -1034,7 +1034,8 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     if (!p->head_dim || p->head_dim % 8 || p->head_dim > 128) return fail(c, LUTAMM_EINVAL, "head_dim must be a multiple of 8 up to 128");
     if (!p->kv_heads || p->heads % p->kv_heads) return fail(c, LUTAMM_EINVAL, "heads must be a multiple of kv_heads");
     if (p->keys > 0x7FFFFF00u || p->queries >> 31) return fail(c, LUTAMM_EINVAL, "keys must be at most 2^31 - 256 and queries below 2^31");
-    if (!std::isfinite(p->scale)) return fail(c, LUTAMM_EINVAL, "scale must be finite");
+    const float scale = p->scale * 1.4426950408889634f;
+    if (!std::isfinite(scale)) return fail(c, LUTAMM_EINVAL, "scale must be finite, also times log2 e");
     if (!p->batch || !p->queries || !p->heads) return LUTAMM_OK;
     if ((uint64_t)p->queries * p->heads >> 31 || (uint64_t)p->batch * p->queries > (1ull << 40) / p->heads)
         return fail(c, LUTAMM_EINVAL, "queries * heads must be below 2^31 and batch * queries * heads at most 2^40");
@@ -1061,7 +1062,7 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.sinks = p->sinks;
     a.left = p->left < 0 ? -1 : p->left;
     a.right = p->right < 0 ? -1 : p->right;
-    a.scale = p->scale * 1.4426950408889634f;
+    a.scale = scale;
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
     const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
