@@ -898,6 +898,7 @@ static int dense_strides(lutamm_ctx* c, const char* name, const int64_t* stride,
         const int i = order[k];
         if (extent[i] <= 1) continue;
         if ((uint64_t)stride[i] < covered) return fail(c, LUTAMM_EINVAL, std::string(name) + ": the elements of an output must lie apart");
+        if (((uint64_t)stride[i] >> 20) * (extent[i] - 1) >> 40) return fail(c, LUTAMM_EINVAL, std::string(name) + ": an output of more than 2^60 elements");
         covered += (extent[i] - 1) * (uint64_t)stride[i];
     }
     return LUTAMM_OK;
