@@ -151,6 +151,8 @@ class Dense:
 class LutTransformerLayer:
     """One encoder layer; `forward` takes and returns a device tensor [n, token_dim].  dense: a Dense, None for PyTorch's operators."""
 
+    dense: Dense | None = None
+
     def __init__(self, ctx: LutAmmContext, weights: dict, seq_len: int, batch_size: int, head_num: int,
                  first_layer_id: int = 0, plans: dict | None = None, fused_gelu: bool = True, dense: Dense | None = None):
         import torch
@@ -218,7 +220,7 @@ class LutTransformerLayer:
 
     def _finish(self, h, f):
         """The layer's last addition, into a tensor of the call's own: y = h + f, with a Dense y = h + LayerNorm_2(f)."""
-        if getattr(self, "dense", None) is None:
+        if self.dense is None:
             return h + f
         y = self.torch.empty_like(h)
         self.ctx.layer_norm(f, *self.ln["ln2"], y, eps=1e-6, residual=h, flags=FLAG_ASYNC)
@@ -243,7 +245,7 @@ class LutTransformerLayer:
         return (stream, self.ctx.generation, self.fused_gelu, torch.is_inference_mode_enabled(),
                 sdp.flash_sdp_enabled(), sdp.mem_efficient_sdp_enabled(), sdp.math_sdp_enabled(), sdp.cudnn_sdp_enabled(),
                 tuple(torch._C._get_sdp_priority_order()), sdp.matmul.fp32_precision, tuple(t.data_ptr() for t in norms),
-                self.dense.key() if getattr(self, "dense", None) is not None else None)
+                self.dense.key() if self.dense is not None else None)
 
     def _capture(self, x, key):
         """Record the layer up to its last addition on a copy of the input: 16 launches and their Python become one.
@@ -297,7 +299,7 @@ class LutTransformerLayer:
 
     def _body(self, x):
         """The layer up to its last addition: y = h + f."""
-        if getattr(self, "dense", None) is not None:
+        if self.dense is not None:
             return self._dense_body(x)
         torch, F = self.torch, self.torch.nn.functional
         B, S, H, D = self.batch, self.seq_len, self.heads, self.token_dim
