@@ -277,7 +277,7 @@ cudaError_t run(const AttentionArgs& a, int sm_count, cudaStream_t s) {
     while (shares < 16 && items * shares < 4ull * sm_count && a.keys / (2 * shares) >= 64) shares *= 2;
     if (items * shares > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     auto kernel = attention_rows_kernel<T, LPK, RB, false>;
-    if constexpr (RB <= attention_few_rows(sizeof(T), LPK * kPer16<T>)) {
+    if constexpr (RB <= attention_few_rows(sizeof(T))) {
         if (a.vec) kernel = attention_rows_kernel<T, LPK, RB, true>;
     }
     if (shares > 8) {   // clusters of 16 are to be asked for

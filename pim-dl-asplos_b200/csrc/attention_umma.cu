@@ -936,10 +936,13 @@ cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaSt
     const uint64_t rows = (uint64_t)a.queries * (a.heads / a.kv_heads);
     if (rows <= 32) return a.head_dim > 64 ? run<T, 128, 1, true>(a, sm_count, dev_err, s) : run<T, 64, 1, true>(a, sm_count, dev_err, s);
     if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
-    // fp32's keys and values are converted once for 256 rows (ViT's batch 97 us with 128, 92 with 256; BERT-large's 94 and 76); 16-bit types, which are only
-    // copied, do better with two CTAs of 128 rows on an SM (8192 tokens in bf16 96 us, 107 with 256).
+    // Two tiles of rows on one ring: fp32's keys and values are converted once for 256 rows, which pays where a window bounds them on both sides and there are CTAs for
+    // all SMs (BERT-large's batch 98 us, 106 with CTAs of 128 rows, two on an SM; 8192 tokens with a window of 512 + 512 244 and 259).  Otherwise two CTAs overlap more
+    // than that saves (ViT's batch 123 and 114 us, 16 x 512 tokens 139 and 127, one sequence of 256 18 and 13), as they do for 16-bit types, which are only copied (8192 tokens
+    // in bf16 107 and 96).
     if constexpr (sizeof(T) == 4) {
-        if (rows > kRows) return run<T, 64, 2>(a, sm_count, dev_err, s);
+        const uint64_t items = (rows + 2 * kRows - 1) / (2 * kRows) * a.batch * a.kv_heads;
+        if (a.left >= 0 && a.right >= 0 && rows > kRows && items >= (uint64_t)sm_count) return run<T, 64, 2>(a, sm_count, dev_err, s);
     }
     return run<T, 64, 1>(a, sm_count, dev_err, s);
 }

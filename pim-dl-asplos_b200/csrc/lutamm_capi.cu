@@ -1067,7 +1067,7 @@ int lutamm_attention(lutamm_ctx* c, const lutamm_attention_params* p, uint32_t f
     a.vec = on_16(p->q, size, p->batch, p->queries, p->heads) && on_16(k, size, p->batch, p->keys, p->kv_heads) &&
             on_16(v, size, p->batch, p->keys, p->kv_heads) && on_16(p->out, size, p->batch, p->queries, p->heads);
     const uint64_t rows = (uint64_t)p->queries * (p->heads / p->kv_heads);
-    const cudaError_t e = rows <= attention_few_rows(size, p->head_dim) || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
+    const cudaError_t e = rows <= attention_few_rows(size) || !a.vec ? launch_attention_rows(a, p->dtype, c->sm_count, c->stream)
                                                                                            : launch_attention_umma(a, p->dtype, c->sm_count, c->d_err, c->stream);
     return dense_done(c, e, "attention", 1, flags);
 }

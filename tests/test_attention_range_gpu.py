@@ -226,3 +226,66 @@ def test_keys_and_queries_that_are_not_finite(ctx, Q, dtype):
             assert torch.equal(got[0, i, 0].isnan(), want.isnan()), (window, i)
             if not want.isnan().any():
                 O.close(got[0, i, 0], want, t, floor=2 ** -18 + (0.0 if t == torch.float32 else 2 * torch.finfo(t).eps * float(v.double().abs().amax())))
+
+
+# ------------------------------------------------------------------------------------------------ CTAs of 256 rows
+def _run_many(ctx, q, k, v, **kw):
+    """One head's inputs as those of 150 heads, which gives every SM a CTA of 256 rows: the first one's results, which are the others', too."""
+    got = _run(ctx, *(t.cuda().expand(-1, -1, 150, -1) for t in (q, k, v)), **kw)
+    assert all(torch.equal(got[:, :, h].view(torch.int32), got[:, :, 0].view(torch.int32)) for h in range(1, 150))
+    return got[:, :, :1]
+
+
+@pytest.mark.parametrize("S,length,window,sinks", [(129, 129, (40, 10), 70), (197, 190, (64, 64), 1), (300, 300, (5, 0), 0), (512, 300, (128, 128), 1), (700, 700, (64, 0), 130),
+                                                   (700, 3, (700, 700), 0), (700, 650, (0, 0), 0), (520, 520, (1, 200), 4), (257, 0, (3, 3), 0)])
+@pytest.mark.parametrize("D", [8, 40, 64])
+def test_two_tiles_of_rows(ctx, S, length, window, sinks, D):
+    q, k, v = _inputs(S + D, S, S, D)
+    want, bound = A.attention(q, k, v, window=window, sinks=sinks, lengths=[length])
+    got = _run_many(ctx, q, k, v, lengths=[length], window=window, sinks=sinks)
+    A.check(got, want, bound)
+    if length:
+        assert A.rms(got, want) <= A.RMS
+    v[..., 3] *= 1e6
+    want, bound = A.attention(q, k, v, window=window, sinks=sinks, lengths=[length])
+    A.check(_run_many(ctx, q, k, v, lengths=[length], window=window, sinks=sinks), want, bound)
+
+
+@pytest.mark.parametrize("large", [1e4, 1e9, 1e30])
+def test_two_tiles_of_rows_and_a_large_key(ctx, large):
+    q, k, v = _inputs(5, 300, 300, 64)
+    v[0, 140] *= large
+    A.check(_run_many(ctx, q, k, v, window=(30, 10)), *A.attention(q, k, v, window=(30, 10)))
+    k[0, 140] *= large
+    want, bound = A.attention(q, k, v, window=(30, 10))
+    got = _run_many(ctx, q, k, v, window=(30, 10))
+    for rows in (slice(0, 130), slice(171, 300)):
+        A.check(got[:, rows], want[:, rows], bound[:, rows])
+
+
+def test_two_tiles_of_rows_and_infinities(ctx):
+    inf, nan = float("inf"), float("nan")
+    q, k, v = _inputs(6, 300, 300, 64)
+    q /= 2
+    spots = {(0, 0): inf, (127, 1): -inf, (140, 2): nan, (140, 3): inf, (299, 4): inf, (200, 5): -inf}
+    clean = v.clone()
+    for (key, col), value in spots.items():
+        v[0, key, 0, col], clean[0, key, 0, col] = value, 0
+    got = _run_many(ctx, q, k, v, window=(30, 10))
+    want, bound = A.attention(q, k, clean, window=(30, 10))
+    seen = O.visible(300, 300, 300, 0, (30, 10), 0)
+    for (key, col), value in spots.items():
+        at = seen[:, key]
+        assert (got[0, at, 0, col].isnan() if math.isnan(value) else got[0, at, 0, col] == value).all()
+        got[0, at, 0, col] = want[0, at, 0, col].float()
+    A.check(got, want, bound)
+    k[0, 150, 0, 7] = -inf     # queries of one sign there: a key without weight for them, NaN for the others
+    q[0, 100, 0, 9] = nan
+    got = _run_many(ctx, q, k, clean, window=(30, 10))
+    nans = seen[:, 150] & (q[0, :, 0, 7] < 0)
+    nans[100] = True
+    assert torch.equal(got[0, :, 0].isnan().all(1), nans) and torch.equal(got[0, :, 0].isnan().any(1), nans)
+    k[0, 150, 0, 7] = 0
+    hidden = torch.where((seen[:, 150] & (q[0, :, 0, 7] > 0))[:, None], 1, 0)[:, 0].bool()
+    want, bound = A.attention(q, k, clean, window=(30, 10))
+    A.check(got[:, ~(nans | hidden)], want[:, ~(nans | hidden)], bound[:, ~(nans | hidden)])
