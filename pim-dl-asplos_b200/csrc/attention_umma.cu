@@ -366,7 +366,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const KeyBounds mine = key_bounds(a, first + (int64_t)qi, length);
         const Seen sees = rows_see(rt);
         float factor = fabsf(a.scale);   // of this row's scores
-        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+        float up = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;   // of this row's queries
         bool odd_queries = false;
         if (a.scale == 0.f) factor = 1.f;
         {
@@ -376,9 +376,19 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             auto raw4 = [&](int i) -> float4 { const uint4 u = raw(i); return *reinterpret_cast<const float4*>(&u); };
             if constexpr (F::kFp32) {
                 uint64_t odd = 0;
+                float big = 0.f;
 #pragma unroll
-                for (int i = 0; i < kPerQ; ++i) odd = look(raw4(i), odd);
-                const uint64_t sign2 = pair(sign, sign);
+                for (int i = 0; i < kPerQ; ++i) {
+                    const float4 x = raw4(i);
+                    odd = look(x, odd);
+                    big = max3(big, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
+                }
+                // A row's queries have a power of two of their own, which no digits hang on, so that their largest is no more than 2: a score far below zero
+                // would else be the difference of its parts' infinities.
+                const int e = max(-126, min(60, 127 - (int)(__float_as_uint(big) >> 23)));
+                up *= power2(e);
+                factor = fminf(factor * power2(-e), 3.4e38f);
+                const uint64_t up2 = pair(up, up);
                 odd_queries = __any_sync(0xffffffffu, is_odd(odd));
 #pragma unroll 1
                 for (int part = 0; part < kPerQ / 4; ++part) {   // 16 elements: 8 columns of each part
@@ -386,7 +396,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 x = raw4(part * 4 + i);
-                        const float2 front = unpair(mul2(pair(x.x, x.y), sign2)), back = unpair(mul2(pair(x.z, x.w), sign2));
+                        const float2 front = unpair(mul2(pair(x.x, x.y), up2)), back = unpair(mul2(pair(x.z, x.w), up2));
                         split3(front.x, front.y, hi[2 * i], mid[2 * i], lo[2 * i]);
                         split3(back.x, back.y, hi[2 * i + 1], mid[2 * i + 1], lo[2 * i + 1]);
                     }
@@ -472,11 +482,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         load_elems<T, kPer16<T>>(q + c, x);
                         load_elems<T, kPer16<T>>(k + c, y);
 #pragma unroll
-                        for (int e = 0; e < kPer16<T>; ++e) d = fmaf(x[e], y[e], d);
+                        for (int e = 0; e < kPer16<T>; ++e) d = fmaf(x[e] * up, y[e], d);
                     }
                 }
                 __syncwarp();
-                tmem_st_32x32b_x1(at + i, __float_as_uint(d * sign));
+                tmem_st_32x32b_x1(at + i, __float_as_uint(d));
             }
             tmem_st_wait();
         };

@@ -289,3 +289,13 @@ def test_two_tiles_of_rows_and_infinities(ctx):
     hidden = torch.where((seen[:, 150] & (q[0, :, 0, 7] > 0))[:, None], 1, 0)[:, 0].bool()
     want, bound = A.attention(q, k, clean, window=(30, 10))
     A.check(got[:, ~(nans | hidden)], want[:, ~(nans | hidden)], bound[:, ~(nans | hidden)])
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_far_below_zero(ctx, Q, D):
+    """A key whose score passes fp32's range downwards has no weight; large queries on small keys are like others."""
+    q, k, v = _inputs(Q + D, Q, 150, D)
+    for size in (1e9, 1e25):
+        x, y = q.abs() * size, k / size
+        y[0, 77] = -1e30 * (1 + k[0, 77].abs())
+        want, bound = A.attention(x, torch.cat([y[:, :77], y[:, 78:]], 1), torch.cat([v[:, :77], v[:, 78:]], 1))
+        A.check(_run(ctx, x, y, v), want, bound)
