@@ -502,6 +502,13 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 tile_keys(t0 + j, k0, end);
                 uint64_t seen = seen_of(k0, end);
                 if (FEW) seen &= 0xFFFFull << (16 * warp);
+                bool settled = true;   // nothing changes NaN
+#pragma unroll 1
+                for (uint32_t c = 0; c < dim; c += 4) {
+                    const float4 x = s_o[out_place(r, c / 4)];
+                    settled &= x.x != x.x && x.y != x.y && x.z != x.z && x.w != x.w;
+                }
+                if (__all_sync(0xffffffffu, settled)) break;
 #pragma unroll 1
                 for (uint32_t i = 0; i < 64; ++i) {
                     const bool me = seen >> i & 1u;
@@ -544,7 +551,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             const float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             if constexpr (F::kFp32) {
                 if (__builtin_expect(__any_sync(0xffffffffu, odd_queries || j < *static_cast<volatile uint32_t*>(&s_odd_to[0])), 0)) {
-                    if (odd_queries || __any_sync(0xffffffffu, j >= *static_cast<volatile uint32_t*>(&s_odd_from[0]))) scores_one_by_one(t0 + j, at);
+                    // (not for rows whose sum is no number any more, and with it their result)
+                    if ((odd_queries || __any_sync(0xffffffffu, j >= *static_cast<volatile uint32_t*>(&s_odd_from[0]))) && !__all_sync(0xffffffffu, l != l)) scores_one_by_one(t0 + j, at);
                 }
             }
             constexpr int kGroups = FEW ? 1 : 2, kWide = FEW ? 16 : 32;
