@@ -464,7 +464,6 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         auto seen_of = [&](int32_t k0, int32_t end) -> uint64_t {
             return below((int64_t)min(end, mine.hi) - k0) & ~(below((int64_t)mine.lo - k0) & ~below((int64_t)a.sinks - k0));
         };
-        const T* const k_head = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head;
         // A tile's scores, one by one, to `at`: where keys or queries are not finite
         auto scores_one_by_one = [&](uint32_t tile, uint32_t at) {
             const T* q = static_cast<const T*>(a.q) + (int64_t)b * a.q_batch + (int64_t)qi * a.q_token + (int64_t)(g * per_head.d + (row - qi * per_head.d)) * a.q_head;
@@ -475,7 +474,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 const int32_t key = k0 + (int32_t)i;
                 float d = 0.f;
                 if (key < end && (key < gap_from || key >= gap_to)) {
-                    const T* k = k_head + (int64_t)key * a.k_token;
+                    const T* k = static_cast<const T*>(a.k) + (int64_t)b * a.k_batch + (int64_t)g * a.k_head + (int64_t)key * a.k_token;
 #pragma unroll 2
                     for (uint32_t c = 0; c < dim; c += kPer16<T>) {
                         float x[kPer16<T>], y[kPer16<T>];
