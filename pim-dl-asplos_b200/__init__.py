@@ -353,6 +353,8 @@ class LutAmmContext:
         self.close()
 
     def set_stream(self, cuda_stream: int | None):
+        """Run on this stream from now on (torch.cuda.current_stream().cuda_stream; for CUDA's default stream, which torch gives as 0, 1), None or
+        0: on the context's own.  Waits for what the context has queued."""
         self._check(self._L.lutamm_set_stream(self._h, cuda_stream or None))
         self.stream = cuda_stream or None
 
@@ -438,7 +440,9 @@ class LutAmmContext:
         M = int(n_tokens if n_tokens is not None else input_index.shape[0])
         self._check(self._L.lutamm_pim_lut(self._h, layer_id, _ptr(input_index), _ptr(output_tensor), M, flags))
 
-    # -- the layer's dense operators (device tensors; include/lutamm.h has the formulas)
+    # -- the layer's dense operators (device tensors; include/lutamm.h has the formulas).  All four run on the context's stream: the one given to
+    # set_stream(), else one of its own that no other waits for.  Without FLAG_ASYNC a call waits until it is done; what another stream makes
+    # has to be there, or that stream's event waited for by the context's, before the call.
     def _fast_dense(self, name: str, *args) -> bool:
         """The call through csrc/python/fastcall.c, where that takes these arguments."""
         if _fast is None or not self._h:
@@ -453,7 +457,7 @@ class LutAmmContext:
         """out = residual + layer norm of x over the last axis (layer_norm() of the reference, transformer_layer.cpp:50-90, and the
         addition behind it).  x, residual, out [rows, width] float32, float16 or bfloat16, rows of any stride; weight and bias
         float32 [width] or None; stats float32 [rows, 2] takes mean and 1 / sqrt(var + eps) for layer_norm_backward.  out may
-        be x or residual."""
+        be x or residual.  Runs on the context's stream."""
         if self._fast_dense("layer_norm", x, weight, bias, out, eps, residual, stats, flags):
             return
         import torch
@@ -469,7 +473,7 @@ class LutAmmContext:
     def layer_norm_backward(self, dout, x, weight, stats, dx=None, dweight=None, dbias=None, workspace=None, flags: int = 0):
         """Gradients of layer_norm: dx like x, dweight and dbias float32 [width], each only where a tensor is given (that of the
         residual is dout).  stats as layer_norm left them.  workspace: a uint8 tensor of layer_norm_backward_workspace() bytes
-        in place of the context's own, for captured calls that may run beside others of this context."""
+        in place of the context's own, for captured calls that may run beside others of this context.  Runs on the context's stream."""
         if workspace is None and self._fast_dense("layer_norm_backward", dout, x, weight, stats, dx, dweight, dbias, flags):
             return
         import torch
@@ -493,7 +497,7 @@ class LutAmmContext:
         """Rotary positions with several axes.  x and out [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], float32, float16
         or bfloat16, of any strides (the query and key heads of a fused projection are one view); out may be x.  positions
         int32 [tokens, axes], or [batch, tokens, axes]; inv_freq float32 [sum(sections)]; sections the pairs of each axis.
-        Pairs are (i, i + pairs) of a head, or (2i, 2i + 1) if interleaved.  inverse turns back: the gradient."""
+        Pairs are (i, i + pairs) of a head, or (2i, 2i + 1) if interleaved.  inverse turns back: the gradient.  Runs on the context's stream."""
         if self._fast_dense("rotary", x, positions, inv_freq, sections, out, interleaved, inverse, flags):
             return
         import torch
@@ -518,7 +522,7 @@ class LutAmmContext:
         strides; heads a multiple of kv_heads; head_dim a multiple of 8 up to 128; scale 1/sqrt(head_dim) by default.  Query i of
         sequence b is at position first[b] + i (first: int32 [batch] on the device, None: 0) and sees the keys from window[0]
         in front of it to window[1] behind it (negative: no bound), and of those in front also the first `sinks`, up to
-        lengths[b] (int32 [batch] on the device, None: all).  A query that sees none gives zeros."""
+        lengths[b] (int32 [batch] on the device, None: all).  A query that sees none gives zeros.  Runs on the context's stream."""
         if self._fast_dense("attention", q, k, v, out, scale, window, sinks, lengths, first, flags):
             return
         import torch
