@@ -234,8 +234,10 @@ int lutamm_pim_lut(lutamm_ctx* ctx, int layer_id, const uint8_t* index, float* o
  * layer norm with the residual behind it (layer_norm() and the additions of src/host/transformer_layer.cpp:50-90, :440-480),
  * attention (:217-229), here with a window and padded sequences, and rotary positions, which the reference has not.
  * All buffers are memory of the context's device.  A call queues its kernels on the context's stream; without
- * LUTAMM_FLAG_ASYNC, the only flag, it waits for them.  Tensors are of one `dtype`; parameters, their gradients and statistics
- * are fp32, and so is all arithmetic on the way; a result is rounded once, to nearest.  Strides count elements and are
+ * LUTAMM_FLAG_ASYNC, the only flag, it waits for them: what another stream makes or reads is to be ordered with that one by the caller
+ * (lutamm_set_stream, events).  Tensors are of one `dtype`; parameters, their gradients and statistics are fp32, and so are sums, maxima and
+ * results on the way, which are rounded once, to nearest; attention of more than one row to a key head (queries times the query heads
+ * that share it) in fp16 and bf16 rounds weights to that type, too, before they multiply the values.  Strides count elements and are
  * not negative; the last axis is contiguous; an output's elements lie apart from one another.  Tensors whose rows all start on
  * 16 bytes are read and written 16 bytes at a time, others an element at a time. */
 #define LUTAMM_F32   0u
@@ -306,7 +308,8 @@ int lutamm_rotary(lutamm_ctx* ctx, const lutamm_rotary_params* p, uint32_t flags
  * tokens behind a cache have first = lengths - queries and right = 0, a sliding window has left, and sinks are the
  * first keys, which stay visible.  A query that sees no key gives zeros.  Keys from lengths[b] on are not read; lengths are taken between 0
  * and keys.  Head h reads key head h / (heads / kv_heads).  A key that a query does not see has no part in its result, whatever it holds; an
- * infinity or NaN in the value of one that it sees shows in that column.
+ * infinity or NaN in the value of one that it sees shows in that column.  In fp32 an element's digits do not hang on others' size; of keys, values
+ * and products of weights and values below 1e-30 some are lost.
  * q and out are [batch][queries][heads][head_dim], k and v [batch][keys][kv_heads][head_dim]; out shares no memory with the
  * others.  For serving: there is no backward pass. */
 typedef struct lutamm_attention_params {

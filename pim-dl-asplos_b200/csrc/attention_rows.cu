@@ -2,7 +2,7 @@
 //   s_j = q k_j scale,  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)   over the keys that the query sees (attention.cuh)
 //
 // Bound by memory for one or two rows, by instructions for eight: keys and values are read once for up to eight rows.  8 x 8192 keys, 16 heads of
-// 128, one row: fp32 170 us, 6.3 TB/s, bf16 94 us, 5.7 TB/s; eight rows of fp32 314 us, 3.4 TB/s.  LPK lanes share a key, 16 bytes each; each such group of
+// 128, one row: fp32 172 us, 6.2 TB/s, bf16 94 us, 5.7 TB/s; eight rows of fp32 319 us, 3.4 TB/s.  LPK lanes share a key, 16 bytes each; each such group of
 // lanes walks keys of its own, four at a time, with a maximum, a sum and an output of its own (the running form of the softmax), so
 // nothing is exchanged between groups before the end.  The rows' partial products are summed over the lanes of a group by halves: after
 // each exchange a lane holds half as many rows, in the end the score of one.  The keys of one head and sequence are split

@@ -5,8 +5,8 @@
 // any of them sees, 64 keys a tile: first the tiles of the sinks, then those of the window; tiles in between are never loaded.  Scores S = Q K^T
 // (tcgen05.mma, queries in tensor memory, keys in shared memory) go to tensor memory, where a thread owns a row: it reads the 64 scores, takes the
 // largest, and writes weights p = exp2(s - m) back over S, where the next product P V reads them as its operand; their sum l stays with the thread.  The
-// output stays in tensor memory, too.  It is brought in line, multiplied by exp2(m_old - m), only where a row's maximum has grown by 2^8: until then
-// weights are formed against the old m.  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
+// output stays in tensor memory, too, in 16 bits.  It is brought in line, multiplied by exp2(m_old - m), only where a row's maximum has grown by 2^8: until then
+// weights are formed against the old m (a published technique, known as lazy or conditional rescaling).  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
 // Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.  fp32 operands are split into
 // three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
@@ -24,9 +24,10 @@
 // that are not finite go into the product as zeros, and are added to the results of the rows that see them at the end; of keys and queries that are not finite fp32
 // forms the scores one by one.  A CTA that meets none pays for the look at what it loads.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 96 us, 349 TFLOP/s; of 2850 warp instructions a
-// tile 680 form its weights.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 32 us, 540 TFLOP/s.  fp32,
-// three products for one: ViT's batch of 64 x 197 tokens, 12 heads, 92 us, of which a CTA spends half before its first and behind its last tile.
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 101 us, 331 TFLOP/s; of 3040 warp instructions a
+// tile 680 form its weights, 100 look at its values.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 33 us,
+// 510 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 115 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
+// an SM is a chain of copy, conversion, scores, weights, product and sum, four tiles long.
 #include "attention.cuh"
 #include "ptx.cuh"
 
@@ -61,7 +62,8 @@ struct Form {
     static_assert(RT * kUsed <= 512 && (RT == 1 || kUsed <= 256));
     static constexpr int kCtas = DP <= 64 && RT == 1 ? 2 : 1;        // per SM
     // Warpgroups: one for each tile of rows, a row a thread, one for each tile of rows that loads, one that issues.  Registers a thread of each; their sum is
-    // what the warpgroups are launched with, and none of them spills (the issuing warps did with 24: 24 rows of 8 x 8192 keys in bf16 59.9 us, 54.4 so).
+    // what the warpgroups are launched with.  None of 16-bit types and none of few rows spills (the issuing warps did with 24: 24 rows of 8 x 8192 keys in bf16
+    // 59.9 us, 54.4 so); fp32's others keep 16 to 48 bytes a thread in memory, with 136 as with 160 registers for a row.
     static constexpr int kRowWarps = 4 * RT, kIssueAt = 8 * RT, kThreads = (2 * RT + 1) * 128;
     static constexpr int kLaunchRegs = DP > 64 ? 168 : RT == 2 ? 96 : 80, kRowRegs = DP > 64 ? 232 : 136, kLoadRegs = DP > 64 ? 136 : RT == 2 ? 80 : 56;
     static constexpr int kIssueRegs = DP > 64 ? 136 : 48;
@@ -199,7 +201,7 @@ Divisor divisor(uint32_t d) {
 }
 
 // FEW: at most 32 rows.  All four warps of rows have them, each with sixteen keys of every tile and an output of its own; they join in the end.  One warp with
-// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 55 us so, 48 with four warps, 5.5 TB/s.
+// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 57 us so, 49 with four warps, 5.5 TB/s.
 template <typename T, int DP, int RT, bool FEW>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
@@ -927,8 +929,8 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     uint64_t keys = a.keys;
     if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + RT * kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
     // As many shares as the SMs hold, by twos (clusters of three do not all find room: 48 items in thirds 42 us, in halves 29), of at least four tiles,
-    // or two of fp32: joining them takes as long as those (256 tokens of 12 heads in bf16 in quarters 11.8 us, whole 9.8; 512 in fp32 in quarters 17.7,
-    // in halves 21.6).
+    // or two of fp32: joining them takes as long as those (256 tokens of 12 heads in bf16 in halves 10.0 us, whole 8.9; in fp32 in halves 13.0, whole
+    // 16.3).
     constexpr uint32_t kShareTiles = sizeof(T) == 4 ? 2 : 4;
     uint32_t shares = 1;
     while (shares < kMostShares && items * shares * 2 <= (uint64_t)F::kCtas * sm_count && keys >= 2ull * shares * kShareTiles * kKeys) shares *= 2;
@@ -956,7 +958,7 @@ cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaSt
     // Two tiles of rows on one ring: fp32's keys and values are converted once for 256 rows, which pays where a window bounds them on both sides and there are CTAs for
     // all SMs (BERT-large's batch 98 us, 106 with CTAs of 128 rows, two on an SM; 8192 tokens with a window of 512 + 512 244 and 259).  Otherwise two CTAs overlap more
     // than that saves (ViT's batch 123 and 114 us, 16 x 512 tokens 139 and 127, one sequence of 256 18 and 13), as they do for 16-bit types, which are only copied (8192 tokens
-    // in bf16 107 and 96).
+    // in bf16 107 and 96, when there was such a form of them).
     if constexpr (sizeof(T) == 4) {
         const uint64_t items = (rows + 2 * kRows - 1) / (2 * kRows) * a.batch * a.kv_heads;
         if (a.left >= 0 && a.right >= 0 && rows > kRows && items >= (uint64_t)sm_count) return run<T, 64, 2>(a, sm_count, dev_err, s);
