@@ -549,7 +549,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 continue;
             }
             const uint32_t at = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
-            const float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
+            float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
             if constexpr (F::kFp32) {
                 if (__builtin_expect(__any_sync(0xffffffffu, odd_queries || j < *static_cast<volatile uint32_t*>(&s_odd_to[0])), 0)) {
                     // (not for rows whose sum is no number any more, and with it their result)
@@ -590,17 +590,29 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 top = fmaxf(x, y) * c;
             }
             top = ceilf(top);
+            // The distance to the maximum is formed with one rounding, of itself.  Where a score's own is as large as that, its product is to be rounded as the
+            // maximum's is, or the largest would lie that far from it.
+            constexpr float kLarge = 4194304.f;
+            auto round_products = [&] {
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (int i = 0; i < kWide; ++i) sc[g][i] = __float_as_uint(__uint_as_float(sc[g][i]) * c);
+                c = 1.f;
+            };
             if constexpr (F::kFp32) {
                 const float m_new = fmaxf(m, top);
                 l *= m == -INFINITY ? 1.f : exp2_approx(m - m_new);
                 m = m_new;
+                if (__builtin_expect(fabsf(m) >= kLarge, 0)) round_products();
             } else {
                 // A maximum that has grown by far: the output so far is brought in line, where there is one.
                 if (m == -INFINITY) m = top;
-                if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                    const float m_new = top > m + kSlack ? top : m;
+                const bool grown = top > m + kSlack;
+                if (__any_sync(0xffffffffu, grown || (fabsf(m) >= kLarge && m > -INFINITY))) {
+                    const float m_new = grown ? top : m;
                     const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
-                    if (n > 0) {
+                    if (n > 0 && __any_sync(0xffffffffu, grown)) {
                         if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
                         tc_fence_after_sync();
 #pragma unroll 1
@@ -616,6 +628,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                     }
                     l *= shrink;
                     m = m_new;
+                    if (__builtin_expect(fabsf(m) >= kLarge, 0)) round_products();
                 }
             }
             const float boost = F::kFp32 ? 0.f : std::is_same<T, __half>::value ? kBoost : -kSlack - (float)log_keys;   // (fp32: in the values)

@@ -299,3 +299,29 @@ def test_scores_far_below_zero(ctx, Q, D):
         y[0, 77] = -1e30 * (1 + k[0, 77].abs())
         want, bound = A.attention(x, torch.cat([y[:, :77], y[:, 78:]], 1), torch.cat([v[:, :77], v[:, 78:]], 1))
         A.check(_run(ctx, x, y, v), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------ large scores
+@pytest.mark.parametrize("Q", ROWS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e12])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_largest_of_large_scores(ctx, Q, dtype, size, sign):
+    """Scores so far apart that one key has all the weight: its value is the result, whatever the scores' size and sign."""
+    t, K, D = TYPES[dtype], 200, 64
+    size = min(size, 1e4) if t == torch.float16 else size
+    q, k, v = _inputs(Q + 5, Q, K, D)
+    q, k = (q * size).to(t), (k * size).to(t)
+    if sign < 0:     # all scores below zero
+        q, k = q.abs(), -k.abs()
+    v = v.to(t)
+    s = q[0, :, 0].double() @ k[0, :, 0].double().T / 8
+    first, second = s.topk(2, 1).values.unbind(1)
+    a = q[0, :, 0].double().abs() @ k[0, :, 0].double().abs().T / 8
+    clear = first - second > torch.clamp(a.amax(1) * 2.0 ** -16, min=120)    # beyond what sums of 64 products in fp32 leave
+    assert clear.sum() * 2 > Q or Q < 4
+    got = _run(ctx, q, k, v)[0, :, 0]
+    assert got.isfinite().all()
+    # out = (p v) / p with one weight p, between 1/2 and 1: fp32's parts of p v are added up with four units lost at most, and rounded, as are 1 / p and its product
+    # (8 units; 16 are allowed); 16-bit types round p once, and the result, half a step each
+    O.close(got[clear], v[0, s.argmax(1)[clear], 0], t, steps=16.0 if t == torch.float32 else 2.0)
