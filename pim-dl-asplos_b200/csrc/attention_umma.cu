@@ -495,9 +495,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         auto add_odd_values = [&] {
             constexpr int kE = kPer16<T>, kBatch = 4;
             const T* const v_head = static_cast<const T*>(a.v) + (int64_t)b * a.v_batch + (int64_t)g * a.v_head;
-            const uint32_t to = min(tiles, *static_cast<volatile uint32_t*>(&s_odd_to[1]));
+            // (the loading warps may be at later tiles, and move the bounds: one lane reads them)
+            const uint32_t from = __shfl_sync(0xffffffffu, *static_cast<volatile uint32_t*>(&s_odd_from[1]), 0);
+            const uint32_t to = __shfl_sync(0xffffffffu, min(tiles, *static_cast<volatile uint32_t*>(&s_odd_to[1])), 0);
 #pragma unroll 1
-            for (uint32_t j = *static_cast<volatile uint32_t*>(&s_odd_from[1]); j < to; ++j) {
+            for (uint32_t j = from; j < to; ++j) {
                 if (RT == 2 && !sees(t0 + j)) continue;
                 int32_t k0, end;
                 tile_keys(t0 + j, k0, end);
