@@ -24,9 +24,9 @@
 // that are not finite go into the product as zeros, and are added to the results of the rows that see them at the end; of keys and queries that are not finite fp32
 // forms the scores one by one.  A CTA that meets none pays for the look at what it loads.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 101 us, 331 TFLOP/s; of 3040 warp instructions a
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 104 us, 322 TFLOP/s; of 3050 warp instructions a
 // tile 680 form its weights, 100 look at its values.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 33 us,
-// 510 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 115 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
+// 510 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 116 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
 // an SM is a chain of copy, conversion, scores, weights, product and sum, four tiles long.
 #include "attention.cuh"
 #include "ptx.cuh"
@@ -971,7 +971,7 @@ cudaError_t pick(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaSt
     if (rows <= 32) return a.head_dim > 64 ? run<T, 128, 1, true>(a, sm_count, dev_err, s) : run<T, 64, 1, true>(a, sm_count, dev_err, s);
     if (a.head_dim > 64) return run<T, 128, 1>(a, sm_count, dev_err, s);
     // Two tiles of rows on one ring: fp32's keys and values are converted once for 256 rows, which pays where a window bounds them on both sides and there are CTAs for
-    // all SMs (BERT-large's batch 98 us, 106 with CTAs of 128 rows, two on an SM; 8192 tokens with a window of 512 + 512 244 and 259).  Otherwise two CTAs overlap more
+    // all SMs (BERT-large's batch 98 us, 104 with CTAs of 128 rows, two on an SM; 8192 tokens with a window of 512 + 512 244 and 259).  Otherwise two CTAs overlap more
     // than that saves (ViT's batch 123 and 114 us, 16 x 512 tokens 139 and 127, one sequence of 256 18 and 13), as they do for 16-bit types, which are only copied (8192 tokens
     // in bf16 107 and 96, when there was such a form of them).
     if constexpr (sizeof(T) == 4) {
