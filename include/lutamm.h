@@ -235,9 +235,8 @@ int lutamm_pim_lut(lutamm_ctx* ctx, int layer_id, const uint8_t* index, float* o
  * attention (:217-229), here with a window and padded sequences, and rotary positions, which the reference has not.
  * All buffers are memory of the context's device.  A call queues its kernels on the context's stream; without
  * LUTAMM_FLAG_ASYNC, the only flag, it waits for them: what another stream makes or reads is to be ordered with that one by the caller
- * (lutamm_set_stream, events).  Tensors are of one `dtype`; parameters, their gradients and statistics are fp32, and so are sums, maxima and
- * results on the way, which are rounded once, to nearest; attention of more than one row to a key head (queries times the query heads
- * that share it) in fp16 and bf16 rounds weights to that type, too, before they multiply the values.  Strides count elements and are
+ * (lutamm_set_stream, events).  Tensors are of one `dtype`; parameters, their gradients and statistics are fp32, and so is all arithmetic on the
+ * way, or what takes its place on the tensor cores (weights of attention in 16 bits: two numbers of that type); a result is rounded once, to nearest.  Strides count elements and are
  * not negative; the last axis is contiguous; an output's elements lie apart from one another.  Tensors whose rows all start on
  * 16 bytes are read and written 16 bytes at a time, others an element at a time. */
 #define LUTAMM_F32   0u

@@ -8,7 +8,8 @@
 // output stays in tensor memory, too, in 16 bits.  It is brought in line, multiplied by exp2(m_old - m), only where a row's maximum has grown by 2^8: until then
 // weights are formed against the old m (a published technique, known as lazy or conditional rescaling).  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
-// Types: f16 and bf16 go through as they are; weights are rounded to that type, once, as an operand of the tensor core has to be.  fp32 operands are split into
+// Types: f16 and bf16 go through as they are, weights as two numbers of that type, the rounded one and what that leaves: results are rounded once, as where one row
+// takes the other kernel (rounded weights alone: 2.3e-3 off for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16; 8192 tokens 103 us for 116).  fp32 operands are split into
 // three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
 // its size.  Of the nine products the six down to 2^-16 of the whole are summed, the small ones first; b c + c b, 2^-25 of it, is left out.  So an element's
 // digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  f16's weights
@@ -153,6 +154,14 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t& hi, uint32_t&
     const float2 m = unpack2(mid, static_cast<__nv_bfloat16*>(nullptr));
     const float2 last = unpair(fma2(pair(m.x, m.y), minus, pair(rest.x, rest.y)));
     lo = pack2(last.x, last.y, static_cast<__nv_bfloat16*>(nullptr));
+}
+// x = hi + lo to nearest, in 16 bits
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2(a, b, static_cast<T*>(nullptr));
+    const float2 h = unpack2(hi, static_cast<T*>(nullptr));
+    const float2 rest = unpair(fma2(pair(h.x, h.y), pair(-1.f, -1.f), pair(a, b)));
+    lo = pack2(rest.x, rest.y, static_cast<T*>(nullptr));
 }
 // 0, or NaN where one of the numbers is none or infinite: what is added to `odd`
 __device__ __forceinline__ uint64_t look(const float4& x, uint64_t odd) {
@@ -637,7 +646,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             const float more = boost - (m == -INFINITY ? 0.f : m);
             const uint64_t off = pair(more, more), cc = pair(c, c);
             uint64_t sum[2] = {0, 0};
-            // Weights of 16 keys: 8 columns, of fp32 three times.
+            // Weights of 16 keys: 8 columns for each part.
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
@@ -650,13 +659,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                         const float p = exp2_approx(x.x), q = exp2_approx(x.y);
                         sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(p, q));
                         if constexpr (F::kFp32) split3(p, q, hi[i / 2], mid[i / 2], lo[i / 2]);
-                        else hi[i / 2] = pack2(p, q, static_cast<T*>(nullptr));
+                        else split2<T>(p, q, hi[i / 2], mid[i / 2]);
                     }
                     tmem_st_32x32b_x8(to, hi);
-                    if constexpr (F::kFp32) {
-                        tmem_st_32x32b_x8(to + 32, mid);
-                        tmem_st_32x32b_x8(to + 64, lo);
-                    }
+                    tmem_st_32x32b_x8(to + 32, mid);
+                    if constexpr (F::kFp32) tmem_st_32x32b_x8(to + 64, lo);
                 }
             }
             if constexpr (FEW) {   // the other warps' keys have no weight here
@@ -664,7 +671,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                 for (int i = 1; i < 4; ++i) {
 #pragma unroll
-                    for (int part = 0; part < F::kParts; ++part) tmem_st_32x32b_x8(at + ((warp + i) & 3u) * 8 + part * 32, none);
+                    for (int part = 0; part < (F::kFp32 ? 3 : 2); ++part) tmem_st_32x32b_x8(at + ((warp + i) & 3u) * 8 + part * 32, none);
                 }
             }
             tmem_st_wait();
@@ -765,10 +772,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             return ok;
         };
         uint32_t n = 0;   // tiles that these rows see, so far
-        // The products of parts, the small ones first: of fp32 (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0)
-        constexpr int kTerms = F::kFp32 ? 6 : 1;
+        // The products of parts, the small ones first: of fp32 (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0), of 16-bit types' weights (1, 0) (0, 0)
+        constexpr int kTerms = F::kFp32 ? 6 : 1, kWeightTerms = F::kFp32 ? 6 : 2;
         auto left = [](int term) -> uint32_t { return F::kFp32 ? 0x021010u >> (4 * (5 - term)) & 0xFu : 0u; };
         auto right = [](int term) -> uint32_t { return F::kFp32 ? 0x201100u >> (4 * (5 - term)) & 0xFu : 0u; };
+        auto weight = [&](int term) -> uint32_t { return F::kFp32 ? left(term) : 1u - term; };
         if (role == 0) {
             const uint32_t k_steps = (dim + 15) / 16, idesc = idesc_f16<T>(kKeys);
             bool ok = wait_warp(smem_u32(&bar.q_full), 0, &s_abort);
@@ -825,11 +833,11 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
 #pragma unroll
                     for (int panel = 0; panel < F::kPanels; ++panel) {
 #pragma unroll
-                        for (int term = 0; term < kTerms; ++term) {
+                        for (int term = 0; term < kWeightTerms; ++term) {
 #pragma unroll
                             for (uint32_t s = 0; s < 4; ++s) {
                                 const uint32_t at = right(term) * F::kPart + panel * kPanel + s * 2048;
-                                umma_f16_ts(my_tmem + F::kProduct + panel * 64, p + left(term) * 32 + s * 8, values + (at >> 4), idescs[panel], term > 0 || s > 0 ? 1u : go_on);
+                                umma_f16_ts(my_tmem + F::kProduct + panel * 64, p + weight(term) * 32 + s * 8, values + (at >> 4), idescs[panel], term > 0 || s > 0 ? 1u : go_on);
                             }
                         }
                     }

@@ -325,3 +325,19 @@ def test_the_largest_of_large_scores(ctx, Q, dtype, size, sign):
     # out = (p v) / p with one weight p, between 1/2 and 1: fp32's parts of p v are added up with four units lost at most, and rounded, as are 1 / p and its product
     # (8 units; 16 are allowed); 16-bit types round p once, and the result, half a step each
     O.close(got[clear], v[0, s.argmax(1)[clear], 0], t, steps=16.0 if t == torch.float32 else 2.0)
+
+
+# ------------------------------------------------------------------------------------------------ 16-bit types
+@pytest.mark.parametrize("Q,K,H,G,D", [(1, 300, 2, 2, 64), (4, 200, 2, 1, 128), (17, 500, 3, 3, 80), (64, 64, 2, 2, 64), (197, 197, 2, 2, 64), (100, 400, 4, 2, 128), (9, 1000, 2, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((50, 50), 3)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_half_the_bits_are_rounded_once(ctx, Q, K, H, G, D, window, sinks, dtype):
+    """The result's own rounding, half a step, and of weights what their second part leaves: the square of half a step, at most a step of
+    2^-24 where fp16's ends."""
+    t = TYPES[dtype]
+    gen = torch.Generator().manual_seed(Q + K)
+    q, k, v = (torch.randn(1, n, h, D, generator=gen).to(t) for n, h in ((Q, H), (K, G), (K, G)))
+    want, bound = A.attention(q, k, v, window=window, sinks=sinks, first=[K - Q])
+    size = A.attention(q, k, v.abs(), window=window, sinks=sinks, first=[K - Q])[0]     # sum of w |v|
+    half = torch.finfo(t).eps / 2
+    A.check(_run(ctx, q, k, v, first=[K - Q], window=window, sinks=sinks), want, bound + (half * half + (2.0 ** -24 if t == torch.float16 else 0)) * size, dtype=t)
