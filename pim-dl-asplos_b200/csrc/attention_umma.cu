@@ -9,7 +9,7 @@
 // weights are formed against the old m (a published technique, known as lazy or conditional rescaling).  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
 // Types: f16 and bf16 go through as they are, weights as two numbers of that type, the rounded one and what that leaves: results are rounded once, as where one row
-// takes the other kernel (rounded weights alone: 2.3e-3 off for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16; 8192 tokens 103 us for 116).  fp32 operands are split into
+// takes the other kernel (rounded weights alone: 2.3e-3 off for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16; 8192 tokens 103 us for 115).  fp32 operands are split into
 // three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
 // its size.  Of the nine products the six down to 2^-16 of the whole are summed, the small ones first; b c + c b, 2^-25 of it, is left out.  So an element's
 // digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  f16's weights
@@ -25,9 +25,9 @@
 // that are not finite go into the product as zeros, and are added to the results of the rows that see them at the end; of keys and queries that are not finite fp32
 // forms the scores one by one.  A CTA that meets none pays for the look at what it loads.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 104 us, 322 TFLOP/s; of 3050 warp instructions a
-// tile 680 form its weights, 100 look at its values.  The exponentials alone would take 34 us, the products 21.  2048 tokens, 8 heads of 128, all keys: 33 us,
-// 510 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 116 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 115 us, 291 TFLOP/s; of 3640 warp instructions a
+// tile 1300 form its weights, 100 look at its values.  The exponentials alone would take 34 us, the products, three for two, 31.  2048 tokens, 8 heads of 128, all keys: 38 us,
+// 450 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 116 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
 // an SM is a chain of copy, conversion, scores, weights, product and sum, four tiles long.
 #include "attention.cuh"
 #include "ptx.cuh"
@@ -210,7 +210,7 @@ Divisor divisor(uint32_t d) {
 }
 
 // FEW: at most 32 rows.  All four warps of rows have them, each with sixteen keys of every tile and an output of its own; they join in the end.  One warp with
-// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 57 us so, 49 with four warps, 5.5 TB/s.
+// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 67 us so, 54.5 with four warps, 4.9 TB/s.
 template <typename T, int DP, int RT, bool FEW>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
@@ -848,7 +848,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 ++n;
             }
         } else if constexpr (!F::kFp32) {
-            // The two warps that are left look at the values, while weights are formed: were it the loading warps, single tokens behind eight caches would take 62 us for 48.
+            // The two warps that are left look at the values, while weights are formed: where the loading warps did, single tokens behind eight caches took 62 us for 50.
             static_assert(RT == 1);
             for (uint32_t job = 1; job < jobs; job += 2) {
                 if (!wait_full(job)) break;
@@ -952,7 +952,7 @@ cudaError_t run(const AttentionArgs& a, int sm_count, uint32_t* dev_err, cudaStr
     uint64_t keys = a.keys;
     if (a.left >= 0 && a.right >= 0) keys = std::min<uint64_t>(keys, (uint64_t)a.left + a.right + RT * kRows / (a.heads / a.kv_heads) + 1 + a.sinks);
     // As many shares as the SMs hold, by twos (clusters of three do not all find room: 48 items in thirds 42 us, in halves 29), of at least four tiles,
-    // or two of fp32: joining them takes as long as those (256 tokens of 12 heads in bf16 in halves 10.0 us, whole 8.9; in fp32 in halves 13.0, whole
+    // or two of fp32: joining them takes as long as those (256 tokens of 12 heads in bf16 in halves 12.0 us, whole 10.4; in fp32 in halves 13.0, whole
     // 16.3).
     constexpr uint32_t kShareTiles = sizeof(T) == 4 ? 2 : 4;
     uint32_t shares = 1;

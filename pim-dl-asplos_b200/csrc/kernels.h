@@ -208,7 +208,7 @@ struct AttentionArgs {
 };
 // Few rows (query tokens x heads of a key head), up to eight of them in one pass over keys and values, on the CUDA cores.  fp32, for which the
 // tensor cores take six products and a conversion, eight rows of 8 x 8192 keys, 16 heads of 64: 172 us there, 198 on the tensor cores, of 128: 319
-// and 526; twelve 301 (of 128 576) and 181 to 195 (526).  bf16, one row of heads of 64: 55 and 53 us, of 64 x 197 keys 17 and 26, two of 8 x 8192 75 and 54.  What does not
+// and 526; twelve 301 (of 128 576) and 181 to 195 (526).  bf16, one row of heads of 64: 55 and 58 us, of 64 x 197 keys 17 and 28, two of 8 x 8192 75 and 58, of 64 x 197 19 and 28.  What does not
 // start on 16 bytes goes there too, element by element.
 constexpr uint64_t attention_few_rows(size_t element) { return element == 2 ? 1 : 8; }
 cudaError_t launch_attention_rows(const AttentionArgs& a, uint32_t dtype, int sm_count, cudaStream_t s);
