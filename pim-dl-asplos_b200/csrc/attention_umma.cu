@@ -42,7 +42,8 @@ constexpr int kRows = 128, kKeys = 64;
 constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two bytes, swizzled rows of 128 bytes
 constexpr uint32_t kMostShares = 8;
 // Tensor memory adds up towards zero: fp32's product of a tile takes four units of 2^-24 off the sum at most, its small terms being first, and would take
-// twenty-four off with the tiles before in there.  So each tile's is taken out and summed with rounding.  Half the bits do not show it.
+// twenty-four off with the tiles before in there.  So each tile's is taken out and summed with rounding; of 16-bit types, whose tiles take eight units off at most,
+// every 64 (400000 keys of one sign in f16 came out 1e-3 too small without).
 constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what f16's weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 // DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
@@ -57,6 +58,7 @@ struct Form {
     static constexpr int kSmem = kSlots * kTile + kOut + 1024;
     // Columns of tensor memory of a tile of rows: scores, over which its weights are written, kBufs times; the product; the queries.  Where two buffers of scores
     // find no room, the next tile's are formed behind the product, while the other tile of rows, or the other CTA on the SM, has its weights formed.
+    static constexpr uint32_t kChunk = kFp32 ? 1 : 64;                       // tiles whose products are summed in tensor memory
     static constexpr int kScoreCols = kFp32 ? 96 : 64, kBufs = kFp32 && DP <= 64 ? 1 : 2;
     static constexpr int kScores = 0, kProduct = kBufs * kScoreCols, kQuery = kProduct + DP, kUsed = kQuery + kParts * DP / 2;
     static constexpr int kColumns = RT * kUsed <= 256 ? 256 : 512;
@@ -442,13 +444,13 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
         const uint32_t full_to = sink_tiles + (uint32_t)max(0, (min(span.hi, common_hi) - span.lo) / kKeys);
         float m = -INFINITY, l = 0.f;   // what weights are formed against; their sum, times 2^kBoost
         const uint32_t out_at = my_tmem + F::kProduct, columns = (dim + 15) / 16 * 16;   // the products write those; behind them lies what other kernels left
-        // fp32: the output of the last tile is in tensor memory; that of those before in shared memory, against m_o
+        // The output of the tiles since the last chunk's end is in tensor memory; that of those before in shared memory, against m_o
         float m_o = -INFINITY;
         bool o_any = false;
         // ... both together, times norm
         auto add_chunk = [&](bool chunk, float norm) {
             const float against = m == -INFINITY ? 0.f : m, f = exp2_approx(m_o - against) * norm;
-#pragma unroll 2
+#pragma unroll 1
             for (uint32_t col = 0; col < columns; col += 16) {
                 uint32_t v[16];
 #pragma unroll
@@ -461,7 +463,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 for (int i = 0; i < 16; i += 4) {
                     float4& at = s_o[out_place(r, (col + i) / 4)];
                     float4 x = make_float4(__uint_as_float(v[i]) * norm, __uint_as_float(v[i + 1]) * norm, __uint_as_float(v[i + 2]) * norm, __uint_as_float(v[i + 3]) * norm);
-                    if (F::kFp32 && o_any) {
+                    if (o_any) {
                         const float4 y = at;
                         x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
                     }
@@ -543,21 +545,24 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             }
         };
         uint32_t n = 0;   // tiles so far
-        for (uint32_t j = 0; j < tiles; ++j) {
-            if (RT == 2 && !sees(t0 + j)) continue;
-            if constexpr (F::kFp32) {
-                if (n > 0 && first_row < n_rows) {   // the last tile's output, while this one's scores are formed
-                    if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
-                    tc_fence_after_sync();
-                    add_chunk(true, 1.f);
-                }
+        // The last chunk's output, behind its last product
+        auto end_chunk = [&]() -> bool {
+            if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) return false;
+            tc_fence_after_sync();
+            add_chunk(true, 1.f);
+            return true;
+        };
+        auto tile = [&](uint32_t j) -> bool {
+            if (RT == 2 && !sees(t0 + j)) return true;
+            if (F::kFp32 && n > 0 && first_row < n_rows) {   // while this tile's scores are formed
+                if (!end_chunk()) return false;
             }
-            if (!wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) break;
+            if (!wait_warp(smem_u32(&bar.s_full[n & 1u]), (n >> 1) & 1u, &s_abort)) return false;
             tc_fence_after_sync();
             if (first_row >= n_rows) {   // a warp without rows: its weights are whatever lies there, and its output nobody's
                 if (lane == 0) mbar_arrive(smem_u32(&bar.p_full[n & 1u]));
                 ++n;
-                continue;
+                return true;
             }
             const uint32_t at = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
             float c = fmaxf(factor, 1.17549435e-38f);   // hidden scores, minus infinity, stay that
@@ -623,8 +628,8 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 if (__any_sync(0xffffffffu, grown || (fabsf(m) >= kLarge && m > -INFINITY))) {
                     const float m_new = grown ? top : m;
                     const float shrink = m == -INFINITY ? 1.f : exp2_approx(m - m_new);
-                    if (n > 0 && __any_sync(0xffffffffu, grown)) {
-                        if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) break;
+                    if (n % F::kChunk != 0 && __any_sync(0xffffffffu, grown)) {
+                        if (!wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort)) return false;
                         tc_fence_after_sync();
 #pragma unroll 1
                         for (uint32_t col = 0; col < columns; col += 16) {
@@ -681,6 +686,12 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
             const float2 sums = unpair(add2(sum[0], sum[1]));
             l = F::kFp32 ? fmaf(sums.x + sums.y, power2(-log_keys), l) : l + (sums.x + sums.y);
             ++n;
+            return true;
+        };
+        for (uint32_t j = 0, ok = 1; ok && j < tiles;) {
+            const uint32_t end = F::kFp32 ? tiles : min(tiles, j + F::kChunk);   // (16-bit types: one tile of rows, which sees all tiles)
+            for (; ok && j < end; ++j) ok = tile(j);
+            if (!F::kFp32 && ok && j < tiles && first_row < n_rows) ok = end_chunk();
         }
         const bool done = n > 0 && wait_warp(smem_u32(&bar.done[(n - 1) & 1u]), ((n - 1) >> 1) & 1u, &s_abort);
         tc_fence_after_sync();
@@ -829,7 +840,7 @@ attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row
                 if (elect_one()) {
                     const uint32_t p = my_tmem + F::kScores + n % F::kBufs * F::kScoreCols;
                     const uint64_t values = desc_rows(smem_at + (2 * j + 1) % kSlots * F::kTile);
-                    const uint32_t go_on = !F::kFp32 && n > 0;
+                    const uint32_t go_on = n % F::kChunk != 0;
 #pragma unroll
                     for (int panel = 0; panel < F::kPanels; ++panel) {
 #pragma unroll

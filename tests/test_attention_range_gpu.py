@@ -341,3 +341,18 @@ def test_half_the_bits_are_rounded_once(ctx, Q, K, H, G, D, window, sinks, dtype
     size = A.attention(q, k, v.abs(), window=window, sinks=sinks, first=[K - Q])[0]     # sum of w |v|
     half = torch.finfo(t).eps / 2
     A.check(_run(ctx, q, k, v, first=[K - Q], window=window, sinks=sinks), want, bound + (half * half + (2.0 ** -24 if t == torch.float16 else 0)) * size, dtype=t)
+
+
+@pytest.mark.parametrize("Q", [20, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sums_over_hundreds_of_thousands_of_keys(ctx, Q, dtype):
+    """Equal weights, values of one sign: what is lost towards zero at each step would add up."""
+    t, K = TYPES[dtype], 400000
+    gen = torch.Generator().manual_seed(Q)
+    v = (1 + torch.rand(1, K, 1, 64, generator=gen)).to(t).cuda()
+    q, k = torch.zeros(1, Q, 150, 64, dtype=t, device="cuda"), torch.zeros(1, 1, 1, 64, dtype=t, device="cuda")
+    out = torch.empty_like(q)
+    ctx.attention(q, k.expand(-1, K, 150, -1), v.expand(-1, -1, 150, -1), out)
+    want = v.double().mean(1, keepdim=True).cpu()
+    # sums of some thousand tiles, each rounded to nearest, of tiles or some dozens of them, which lose up to two units at each of eight steps a tile
+    O.close(out, want.expand(out.shape), t, floor=(512 + math.sqrt(K / 64)) * 2.0 ** -24 * 2)
