@@ -9,13 +9,13 @@
 // weights are formed against the old m (a published technique, known as lazy or conditional rescaling).  While a tile's weights are formed, the tensor core works on the next tile's scores and the last tile's product.
 //
 // Types: f16 and bf16 go through as they are, weights as two numbers of that type, the rounded one and what that leaves: results are rounded once, as where one row
-// takes the other kernel (rounded weights alone: 2.3e-3 off for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16; 8192 tokens 103 us for 115).  fp32 operands are split into
+// takes the other kernel (rounded weights alone: 2.3e-3 off for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in f16; 8192 tokens 103 us for 115 when this was taken).  fp32 operands are split into
 // three bf16 numbers, x = a + b + c: a the leading bits, b and c the rests to nearest, together all 24 bits of x and, bf16 having fp32's exponents, whatever
 // its size.  Of the nine products the six down to 2^-16 of the whole are summed, the small ones first; b c + c b, 2^-25 of it, is left out.  So an element's
 // digits do not hang on its neighbours', as they would under a power of two for a row or a tile, which half the products of f16 parts need.  f16's weights
 // carry 2^6 and up to 2^8 more, the sum l with them; in bf16 and fp32 they, or the values, are brought down by the number of keys instead, exactly, so that a
 // row's sums stay below its largest value: results up to the type's largest number do not overflow on the way.  Maxima, sums and outputs are fp32; maxima are taken up to whole numbers, so that what is against an older
-// one is brought in line without rounding; the sum over tiles that fp32 makes outside of tensor memory rounds once each.
+// one is brought in line without rounding; the sums over tiles, or chunks of them, outside of tensor memory round once each.
 //
 // Loading warps copy 16 bytes a piece (cp.async): no tensor maps to be made by the host, and rows behind the last key become zeros.  fp32 is
 // converted in place.  Tensors that do not start on 16 bytes throughout take the other kernel (attention_rows.cu), element by element.  Where there are few
@@ -25,9 +25,9 @@
 // that are not finite go into the product as zeros, and are added to the results of the rows that see them at the end; of keys and queries that are not finite fp32
 // forms the scores one by one.  A CTA that meets none pays for the look at what it loads.
 //
-// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 115 us, 291 TFLOP/s; of 3640 warp instructions a
+// What bounds it: issuing instructions.  8192 tokens, 16 heads of 64 in bf16, a window of 512 on either side: 118 us, 283 TFLOP/s; of 3690 warp instructions a
 // tile 1300 form its weights, 100 look at its values.  The exponentials alone would take 34 us, the products, three for two, 31.  2048 tokens, 8 heads of 128, all keys: 38 us,
-// 450 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 116 us, issue in 47 % of the cycles, the tensor cores busy in 29 %: each of the two CTAs on
+// 450 TFLOP/s.  fp32, six products for one: ViT's batch of 64 x 197 tokens, 12 heads, 113 us, issue in 48 % of the cycles, the tensor cores busy in 30 %: each of the two CTAs on
 // an SM is a chain of copy, conversion, scores, weights, product and sum, four tiles long.
 #include "attention.cuh"
 #include "ptx.cuh"
@@ -43,7 +43,7 @@ constexpr int kPanel = kKeys * 128;   // bytes: 64 keys x 64 elements of two byt
 constexpr uint32_t kMostShares = 8;
 // Tensor memory adds up towards zero: fp32's product of a tile takes four units of 2^-24 off the sum at most, its small terms being first, and would take
 // twenty-four off with the tiles before in there.  So each tile's is taken out and summed with rounding; of 16-bit types, whose tiles take eight units off at most,
-// every 64 (400000 keys of one sign in f16 came out 1e-3 too small without).
+// every 64 (400000 keys of one sign in f16 came out 3e-3 too small without).
 constexpr float kBoost = 6.f, kSlack = 8.f;   // log2 of what f16's weights are multiplied by, and of how far they may grow over 1: 2^14 in all
 
 // DP: columns of a head, up to a multiple of 64.  RT: tiles of rows of a CTA, which read the same keys and values.
@@ -212,7 +212,7 @@ Divisor divisor(uint32_t d) {
 }
 
 // FEW: at most 32 rows.  All four warps of rows have them, each with sixteen keys of every tile and an output of its own; they join in the end.  One warp with
-// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 67 us so, 54.5 with four warps, 4.9 TB/s.
+// all 64 keys would have the three others idle: tokens of 16 heads on 4 of 128 behind 8 caches of up to 32768, four rows, 67 us so, 54.5 with four warps (57 with the sums out of tensor memory, 4.7 TB/s).
 template <typename T, int DP, int RT, bool FEW>
 __global__ void __launch_bounds__(Form<T, DP, RT>::kThreads, Form<T, DP, RT>::kCtas)
 attention_umma_kernel(const __grid_constant__ AttentionArgs a, const Divisor row_tiles, const Divisor kv_heads, const Divisor per_head, uint32_t* dev_err) {
